@@ -57,7 +57,7 @@ def listed():
               layout="interleaved", rot=32, theta=1e4, scaling="linear", factor=4.0),
         # two long prompts continued far out, frequencies blended for the long context
         _case("append", "append_far", seqs=2, q=(4001, 4096), past=(99_000, 101_000), norm=True, scaling="bands",
-              factor=32.0, low=1.0, high=32.0, amplitude=0.1 * math.log(32.0) + 1.0),
+              factor=32.0, low=1.0, high=32.0, amplitude=1.34375),
         # one request's decode step (the batch-1 talker step at 1024 cached keys)
         _case("attend", "attend_one", past=(1023, 1023)),
         # the decode frame of 64 requests with the serving workload's ragged lengths
