@@ -512,6 +512,117 @@ q3t_status q3t_sample_logits(q3t_model *model, const float *logits, int vocab, c
                              const int64_t *suppress_ids, int num_suppress, double u, int64_t *token,
                              uint8_t *kept);
 
+/* -------------------- 4-bit paged key/value cache ------------------------ */
+/* No reference counterpart (the reference keeps a dense bf16 cache, kv.rs):
+ * a decoder layer's keys and values in 4 bits, in pages of 16 tokens.  These
+ * calls take device pointers on `device` and run on `stream` (a cudaStream_t
+ * of that device; NULL is its default stream): they enqueue one kernel and
+ * return without waiting, allocate nothing, keep nothing between calls, may
+ * be captured into a CUDA graph, and leave the calling thread's current
+ * device as it was.
+ *
+ * Every 32 dims of a head's key or value share a bf16 scale s and a bf16
+ * zero z: z is their minimum rounded down, s is (maximum - z) / 15, and a
+ * value x is kept as the digit n = round((x - z) / s) in 0..15, which stands
+ * for n s + z, within s / 2 of x.  A group with a value that is not finite
+ * reads back as NaN.
+ *
+ * The pool holds one block of 20 x head_dim bytes for each (page, kv head),
+ * [num_pages][num_kv_heads][20 head_dim].  With D = head_dim, G = D / 32:
+ *   K digits at 0      token c, dim 32 j + 8 t + 4 b0 + 2 h + b1: nibble h of
+ *                      byte c D / 2 + 4 (G t + j) + 2 b1 + b0
+ *   V digits at 8 D    token 8 b0 + 2 t + b1, dim 64 M + 16 m + 8 h + g:
+ *                      nibble h of byte 512 M + 16 (4 g + t) + 4 m + 2 b1 + b0
+ *   scales at 16 D     token 8 p1 + 2 t + p0, group j: bf16 K scale, K zero,
+ *                      V scale, V zero at byte 8 (4 (4 j + t) + 2 p1 + p0)
+ * Every byte belongs to one token, and an append writes its tokens' bytes
+ * only.  The pool needs no initialisation. */
+typedef struct {
+  int device;                /* CUDA device ordinal of every pointer of the call */
+  int num_kv_heads;          /* 1..1024 */
+  int head_dim;              /* 64 or 128 */
+  int table_rows;
+  int table_stride;          /* page-table entries of a row */
+  int64_t num_pages;         /* pages of the pool */
+  void *pool;                /* device, on a 16-byte boundary */
+  const int32_t *page_table; /* device [table_rows][table_stride]: entry i of a row is the page of
+                                positions 16 i .. 16 i + 15; entries outside 0..num_pages-1 are no page */
+} q3t_kv4_cache;
+
+/* The token rows of a call.  Sequence s owns rows q_start[s] .. q_start[s+1]-1
+ * (ascending), at positions kv_len[s] - count .. kv_len[s] - 1: the newest
+ * tokens of its kv_len[s] keys.  Rows of no sequence are neither read nor
+ * written; a sequence may have none.  Rows at negative positions (padding in
+ * front) are skipped by an append and come back as zeros from attend and
+ * read. */
+typedef struct {
+  int num_seqs;              /* 0..2^20 */
+  int num_tokens;            /* rows of the call's q / k / v / out, 0..2^28 */
+  int max_q_len;             /* most rows of a sequence, 0: unknown (a hint: it only chooses the launch) */
+  int max_kv_len;            /* most keys of a sequence, 0: unknown (the same) */
+  const int32_t *q_start;    /* device [num_seqs + 1] */
+  const int32_t *kv_len;     /* device [num_seqs] */
+  const int32_t *table_row;  /* device [num_seqs], nullable: page-table row of a sequence (its index without) */
+} q3t_kv4_batch;
+
+/* Rotary positions.  The leading rotary_dim dims of a head turn in pairs by
+ * position x frequency, the others pass; frequency i is theta^(-2 i /
+ * rotary_dim), and in the long-context forms
+ *   LINEAR  divided by factor
+ *   BANDS   blended by the turns original x frequency / (2 pi) it makes in
+ *           the original context: divided by factor up to `low` turns, kept
+ *           from `high` turns on, linear in between
+ * amplitude multiplies the turned dims (1: none). */
+typedef enum { Q3T_ROPE_HALF = 0, Q3T_ROPE_INTERLEAVED = 1 } q3t_rope_layout;
+typedef enum { Q3T_ROPE_NONE = 0, Q3T_ROPE_LINEAR = 1, Q3T_ROPE_BANDS = 2 } q3t_rope_scaling;
+typedef struct {
+  int rotary_dim;            /* a multiple of 8 up to head_dim; 0: no rotation */
+  int layout;                /* q3t_rope_layout: pairs (i, i + rotary_dim / 2) or (2 i, 2 i + 1) */
+  int scaling;               /* q3t_rope_scaling */
+  int original;              /* BANDS: tokens of the original context */
+  float theta;
+  float factor;              /* LINEAR, BANDS */
+  float low, high;           /* BANDS: turns */
+  float amplitude;
+} q3t_rope;
+
+/* The frequencies [rotary_dim / 2] in radians per position.  Host code, no GPU. */
+q3t_status q3t_rope_freqs(const q3t_rope *rope, double *freqs);
+
+/* Rows of an append: token rows of heads, head h at element h x head_dim.
+ * Strides are elements between token rows, at least a row's heads. */
+typedef struct {
+  int dtype;                 /* q3t_dtype of q, k and v */
+  int num_heads;             /* query heads; 0: no queries */
+  const void *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;
+  const float *q_gamma;      /* device [head_dim], nullable: RMSNorm of every query head before the rotation */
+  const float *k_gamma;      /* the same for keys */
+  float eps;                 /* of both norms */
+  uint16_t *q_out;           /* bf16 rows: the queries, normed and rotated (may be q itself if that is bf16) */
+  int64_t q_out_stride;
+} q3t_kv4_rows;
+
+/* Norms and rotates the queries and keys of the batch's rows and appends the
+ * keys and values to the cache (rope == NULL: no rotation).  Angles are
+ * computed in 64 bits.  Rows whose position has no page are dropped (their
+ * queries are still written).  No position of a page may be appended twice in
+ * one call, nor while another call reads it. */
+q3t_status q3t_kv4_append(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, const q3t_kv4_rows *rows,
+                          const q3t_rope *rope, void *stream);
+/* Attention of the batch's query rows over the cache: the row at position p
+ * sees the sequence's keys 0..p (window > 0: the last `window` of them), the
+ * appended ones among them; out = softmax(scale q . k) v in bf16, query head h
+ * reading kv head h / (num_heads / num_kv_heads).  Keys whose position has no
+ * page are not seen; a row that sees no key gives zeros.  out must not
+ * overlap q. */
+q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, int num_heads, const uint16_t *q,
+                          int64_t q_stride, float scale, int window, uint16_t *out, int64_t out_stride, void *stream);
+/* What the cache holds for the batch's rows, as bf16 rows (k or v nullable):
+ * n s + z rounded once; zeros where a position has no page. */
+q3t_status q3t_kv4_read(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, uint16_t *k, int64_t k_stride,
+                        uint16_t *v, int64_t v_stride, void *stream);
+
 /* ------------------------------- misc ----------------------------------- */
 /* Struct layout as this library was compiled (no reference counterpart: the
  * reference is one Rust crate, so its structs need no cross-language check).

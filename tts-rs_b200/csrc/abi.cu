@@ -115,6 +115,28 @@ const FieldRow k_spk_desc[] = {
     Q3T_F(q3t_speaker_encoder_desc, device),  Q3T_F(q3t_speaker_encoder_desc, config),
     Q3T_F(q3t_speaker_encoder_desc, tensors), Q3T_F(q3t_speaker_encoder_desc, num_tensors),
 };
+const FieldRow k_kv4_cache[] = {
+    Q3T_F(q3t_kv4_cache, device),     Q3T_F(q3t_kv4_cache, num_kv_heads), Q3T_F(q3t_kv4_cache, head_dim),
+    Q3T_F(q3t_kv4_cache, table_rows), Q3T_F(q3t_kv4_cache, table_stride), Q3T_F(q3t_kv4_cache, num_pages),
+    Q3T_F(q3t_kv4_cache, pool),       Q3T_F(q3t_kv4_cache, page_table),
+};
+const FieldRow k_kv4_batch[] = {
+    Q3T_F(q3t_kv4_batch, num_seqs), Q3T_F(q3t_kv4_batch, num_tokens), Q3T_F(q3t_kv4_batch, max_q_len),
+    Q3T_F(q3t_kv4_batch, max_kv_len), Q3T_F(q3t_kv4_batch, q_start), Q3T_F(q3t_kv4_batch, kv_len),
+    Q3T_F(q3t_kv4_batch, table_row),
+};
+const FieldRow k_rope[] = {
+    Q3T_F(q3t_rope, rotary_dim), Q3T_F(q3t_rope, layout), Q3T_F(q3t_rope, scaling),
+    Q3T_F(q3t_rope, original),   Q3T_F(q3t_rope, theta),  Q3T_F(q3t_rope, factor),
+    Q3T_F(q3t_rope, low),        Q3T_F(q3t_rope, high),   Q3T_F(q3t_rope, amplitude),
+};
+const FieldRow k_kv4_rows[] = {
+    Q3T_F(q3t_kv4_rows, dtype),    Q3T_F(q3t_kv4_rows, num_heads), Q3T_F(q3t_kv4_rows, q),
+    Q3T_F(q3t_kv4_rows, k),        Q3T_F(q3t_kv4_rows, v),         Q3T_F(q3t_kv4_rows, q_stride),
+    Q3T_F(q3t_kv4_rows, k_stride), Q3T_F(q3t_kv4_rows, v_stride),  Q3T_F(q3t_kv4_rows, q_gamma),
+    Q3T_F(q3t_kv4_rows, k_gamma),  Q3T_F(q3t_kv4_rows, eps),       Q3T_F(q3t_kv4_rows, q_out),
+    Q3T_F(q3t_kv4_rows, q_out_stride),
+};
 #undef Q3T_F
 
 #define Q3T_S(S, table) {#S, sizeof(S), alignof(S), table, (int)(sizeof(table) / sizeof(table[0]))}
@@ -133,6 +155,10 @@ const StructRow k_structs[] = {
     Q3T_S(q3t_codec_encoder_desc, k_enc_desc),
     Q3T_S(q3t_speaker_encoder_config, k_spk_config),
     Q3T_S(q3t_speaker_encoder_desc, k_spk_desc),
+    Q3T_S(q3t_kv4_cache, k_kv4_cache),
+    Q3T_S(q3t_kv4_batch, k_kv4_batch),
+    Q3T_S(q3t_rope, k_rope),
+    Q3T_S(q3t_kv4_rows, k_kv4_rows),
 };
 #undef Q3T_S
 

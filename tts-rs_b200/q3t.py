@@ -136,6 +136,7 @@ EXPORTS = [
     "q3t_codec_encoder_frames", "q3t_codec_encode", "q3t_codec_encoder_hidden",
     "q3t_speaker_encoder_load", "q3t_speaker_encoder_free", "q3t_speaker_embed", "q3t_speaker_mel",
     "q3t_session_seed_voice_clone", "q3t_wav_read", "q3t_resample_linear",
+    "q3t_rope_freqs", "q3t_kv4_append", "q3t_kv4_attend", "q3t_kv4_read",
 ]
 
 
@@ -144,6 +145,32 @@ class SeedControls(C.Structure):
     _fields_ = [("tts_bos_token_id", C.c_int64), ("tts_eos_token_id", C.c_int64),
                 ("tts_pad_token_id", C.c_int64), ("codec_prefix_ids", C.POINTER(C.c_int64)),
                 ("n_codec_prefix", C.c_int), ("codec_pad_id", C.c_int64), ("codec_bos_id", C.c_int64)]
+
+
+
+class KV4CacheView(C.Structure):
+    _fields_ = [("device", C.c_int), ("num_kv_heads", C.c_int), ("head_dim", C.c_int), ("table_rows", C.c_int),
+                ("table_stride", C.c_int), ("num_pages", C.c_int64), ("pool", C.c_void_p),
+                ("page_table", C.c_void_p)]
+
+
+class KV4BatchView(C.Structure):
+    _fields_ = [("num_seqs", C.c_int), ("num_tokens", C.c_int), ("max_q_len", C.c_int), ("max_kv_len", C.c_int),
+                ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("table_row", C.c_void_p)]
+
+
+class RopeView(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int), ("layout", C.c_int), ("scaling", C.c_int), ("original", C.c_int),
+                ("theta", C.c_float), ("factor", C.c_float), ("low", C.c_float), ("high", C.c_float),
+                ("amplitude", C.c_float)]
+
+
+class KV4Rows(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("num_heads", C.c_int), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("q_gamma", C.c_void_p), ("k_gamma", C.c_void_p), ("eps", C.c_float), ("q_out", C.c_void_p),
+                ("q_out_stride", C.c_int64)]
+
 
 _F = C.POINTER(C.c_float)
 _I64 = C.POINTER(C.c_int64)
@@ -220,6 +247,13 @@ def lib():
         L.q3t_speaker_encoder_free.restype = None
         L.q3t_speaker_embed.argtypes = [C.c_void_p, _F, C.c_int64, _F]
         L.q3t_speaker_mel.argtypes = [C.c_void_p, _F, C.c_int64, _F, C.c_int, C.POINTER(C.c_int)]
+        L.q3t_rope_freqs.argtypes = [C.POINTER(RopeView), C.POINTER(C.c_double)]
+        L.q3t_kv4_append.argtypes = [C.POINTER(KV4CacheView), C.POINTER(KV4BatchView), C.POINTER(KV4Rows),
+                                     C.POINTER(RopeView), C.c_void_p]
+        L.q3t_kv4_attend.argtypes = [C.POINTER(KV4CacheView), C.POINTER(KV4BatchView), C.c_int, C.c_void_p,
+                                     C.c_int64, C.c_float, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]
+        L.q3t_kv4_read.argtypes = [C.POINTER(KV4CacheView), C.POINTER(KV4BatchView), C.c_void_p, C.c_int64,
+                                   C.c_void_p, C.c_int64, C.c_void_p]
         L.q3t_abi_struct.argtypes = [C.c_char_p, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t),
                                      C.POINTER(C.c_int)]
         L.q3t_abi_field.argtypes = [C.c_char_p, C.c_int, C.POINTER(C.c_char_p), C.POINTER(C.c_size_t),
@@ -248,7 +282,8 @@ STRUCTS = {"q3t_lm_config": LMConfig, "q3t_talker_config": TalkerConfig, "q3t_co
            "q3t_session_desc": SessionDesc, "q3t_seed_controls": SeedControls, "q3t_batch_desc": BatchDesc,
            "q3t_step_stats": StepStats, "q3t_codec_encoder_config": CodecEncoderConfig,
            "q3t_codec_encoder_desc": CodecEncoderDesc, "q3t_speaker_encoder_config": SpeakerEncoderConfig,
-           "q3t_speaker_encoder_desc": SpeakerEncoderDesc}
+           "q3t_speaker_encoder_desc": SpeakerEncoderDesc, "q3t_kv4_cache": KV4CacheView,
+           "q3t_kv4_batch": KV4BatchView, "q3t_rope": RopeView, "q3t_kv4_rows": KV4Rows}
 
 
 def check(rc):
@@ -803,6 +838,166 @@ class Batch:
 
     def __del__(self):
         self.close()
+
+
+# ---------------------------------------------------------------------------
+# 4-bit paged key/value cache on torch CUDA tensors (q3t_kv4_*).  Calls run on
+# torch's current stream of the cache's device and return without waiting.
+# ---------------------------------------------------------------------------
+def _bad(message):
+    raise Q3TError(INVALID_INPUT, message)
+
+
+class Rope:
+    """Rotary positions (q3t_rope): the leading rotary_dim dims (default all of
+    head_dim) turn in pairs (i, i + rotary_dim / 2) ("half") or (2 i, 2 i + 1)
+    ("interleaved"); scaling "none", "linear" or "bands" for long contexts."""
+
+    def __init__(self, head_dim, rotary_dim=None, layout="half", theta=1e4, scaling="none", factor=1.0, low=1.0,
+                 high=4.0, original=4096, amplitude=1.0):
+        layouts, scalings = ("half", "interleaved"), ("none", "linear", "bands")
+        if layout not in layouts or scaling not in scalings:
+            _bad(f"Rope: unknown layout {layout!r} or scaling {scaling!r}")
+        rot = head_dim if rotary_dim is None else rotary_dim
+        if rot > head_dim:
+            _bad(f"Rope: rotary_dim {rot} exceeds head_dim {head_dim}")
+        self.view = RopeView(rot, layouts.index(layout), scalings.index(scaling), original, theta, factor, low, high,
+                             amplitude)
+        self.ref = C.byref(self.view)
+        self.freqs()  # rejects what the append would
+
+    def freqs(self):
+        """The frequencies [rotary_dim / 2] in radians per position (host code, no GPU)."""
+        out = np.zeros(max(1, self.view.rotary_dim // 2), np.float64)
+        check(lib().q3t_rope_freqs(self.ref, out.ctypes.data_as(C.POINTER(C.c_double))))
+        return out[:self.view.rotary_dim // 2]
+
+
+def _int32(t, name, device, ndim):
+    if str(t.dtype) != "torch.int32" or t.dim() != ndim or not t.is_contiguous() or t.device != device:
+        _bad(f"{name}: a contiguous int32 tensor of {ndim} dims on {device} is needed")
+    return t.data_ptr()
+
+
+class KV4Batch:
+    """The token rows of a call (q3t_kv4_batch): sequence s owns rows
+    q_start[s] .. q_start[s + 1] - 1, the newest of its kv_len[s] keys.
+    max_q / max_kv: the most rows and keys of a sequence, where the program
+    knows them (they only choose the launch)."""
+
+    def __init__(self, q_start, kv_len, num_tokens, table_row=None, max_q=0, max_kv=0):
+        dev, n = kv_len.device, kv_len.shape[0]
+        if not kv_len.is_cuda:
+            _bad("KV4Batch: kv_len must be on a CUDA device")
+        if q_start.shape[0] != n + 1 or (table_row is not None and table_row.shape[0] != n):
+            _bad(f"KV4Batch: q_start needs {n + 1} entries, and table_row {n}, for {n} sequences")
+        self.device, self.tokens = dev, int(num_tokens)
+        self.view = KV4BatchView(n, self.tokens, int(max_q), int(max_kv), _int32(q_start, "q_start", dev, 1),
+                                 _int32(kv_len, "kv_len", dev, 1),
+                                 None if table_row is None else _int32(table_row, "table_row", dev, 1))
+        self.ref = C.byref(self.view)
+        self._keep = (q_start, kv_len, table_row)
+
+
+class KV4Cache:
+    """One layer's 4-bit key/value cache (q3t_kv4_cache) over a torch pool
+    [pages, kv heads, 20 head_dim] of uint8 and a page table [rows, stride] of
+    int32.  Allocate the pool with KV4Cache.new_pool, or by those shapes."""
+
+    def __init__(self, pool, page_table, num_kv_heads, head_dim):
+        if not pool.is_cuda or str(pool.dtype) != "torch.uint8" or not pool.is_contiguous() or \
+                tuple(pool.shape[1:]) != (num_kv_heads, 20 * head_dim):
+            _bad(f"KV4Cache: the pool is a contiguous uint8 CUDA tensor [pages, {num_kv_heads}, {20 * head_dim}]")
+        self.device, self.kv_heads, self.head_dim = pool.device, num_kv_heads, head_dim
+        self.view = KV4CacheView(pool.device.index, num_kv_heads, head_dim, page_table.shape[0], page_table.shape[-1],
+                                 pool.shape[0], pool.data_ptr(), _int32(page_table, "page_table", pool.device, 2))
+        self.ref = C.byref(self.view)
+        self.pool, self.page_table = pool, page_table
+        self._bf16 = self._empty = self._stream = None
+
+    @staticmethod
+    def new_pool(num_pages, num_kv_heads, head_dim, device="cuda"):
+        import torch
+        return torch.empty(num_pages, num_kv_heads, 20 * head_dim, dtype=torch.uint8, device=device)
+
+    def _torch(self):
+        import torch
+        self._bf16, self._empty, self._stream = torch.bfloat16, torch.empty, torch.cuda.current_stream
+        self._f32 = torch.float32
+
+    def _rows(self, t, name, batch, heads, dtype):
+        D = self.head_dim
+        if t.dtype != dtype or t.device != self.device or t.shape != (batch.tokens, heads, D):
+            _bad(f"{name}: {dtype} rows [{batch.tokens}, {heads}, {D}] on {self.device} are needed, got {t.dtype} "
+                 f"{list(t.shape)} on {t.device}")
+        st = t.stride()
+        if t.shape[0] and (st[2] != 1 or (st[1] != D and heads > 1)):
+            _bad(f"{name}: a token's heads must be contiguous")
+        return t.data_ptr(), st[0] if t.shape[0] > 1 else heads * D
+
+    def _gamma(self, g, name):
+        if g is None:
+            return None
+        if g.dtype != self._f32 or g.device != self.device or g.shape != (self.head_dim,) or not g.is_contiguous():
+            _bad(f"{name}: a contiguous float32 tensor [{self.head_dim}] on {self.device} is needed")
+        return g.data_ptr()
+
+    def append(self, batch, k, v, q=None, rope=None, q_gamma=None, k_gamma=None, eps=1e-6, q_out=None):
+        """Appends keys and values [tokens, kv heads, D] (f32 or bf16), keys
+        normed (k_gamma) and rotated (rope); returns the queries q [tokens,
+        heads, D] normed and rotated in bf16 (None without q)."""
+        if self._bf16 is None:
+            self._torch()
+        if batch.device != self.device:
+            _bad(f"append: the batch is on {batch.device}, the cache on {self.device}")
+        dt = k.dtype
+        if dt != self._bf16 and dt != self._f32:
+            _bad(f"append: rows are float32 or bfloat16, got {dt}")
+        r = KV4Rows(0 if dt == self._f32 else 1)
+        r.k, r.k_stride = self._rows(k, "k", batch, self.kv_heads, dt)
+        r.v, r.v_stride = self._rows(v, "v", batch, self.kv_heads, dt)
+        if q is not None:
+            heads = q.shape[1]
+            r.num_heads = heads
+            r.q, r.q_stride = self._rows(q, "q", batch, heads, dt)
+            if q_out is None:
+                q_out = self._empty(q.shape, dtype=self._bf16, device=self.device)
+            r.q_out, r.q_out_stride = self._rows(q_out, "q_out", batch, heads, self._bf16)
+        r.q_gamma, r.k_gamma, r.eps = self._gamma(q_gamma, "q_gamma"), self._gamma(k_gamma, "k_gamma"), eps
+        check(lib().q3t_kv4_append(self.ref, batch.ref, C.byref(r), None if rope is None else rope.ref,
+                                   self._stream(self.device).cuda_stream))
+        return q_out if q is not None else None
+
+    def attend(self, batch, q, scale=None, window=0, out=None):
+        """softmax(scale q . k) v over the cached keys each row may see (bf16
+        [tokens, heads, D]); scale defaults to head_dim ** -0.5."""
+        if self._bf16 is None:
+            self._torch()
+        if batch.device != self.device:
+            _bad(f"attend: the batch is on {batch.device}, the cache on {self.device}")
+        if out is None:
+            out = self._empty(q.shape, dtype=self._bf16, device=self.device)
+        heads = q.shape[1]
+        qp, qs = self._rows(q, "q", batch, heads, self._bf16)
+        op, os_ = self._rows(out, "out", batch, heads, self._bf16)
+        check(lib().q3t_kv4_attend(self.ref, batch.ref, heads, qp, qs,
+                                   self.head_dim ** -0.5 if scale is None else scale, window, op, os_,
+                                   self._stream(self.device).cuda_stream))
+        return out
+
+    def read(self, batch, k=None, v=None):
+        """(keys, values) the cache holds for the batch's rows, bf16 [tokens, kv heads, D]."""
+        if self._bf16 is None:
+            self._torch()
+        if batch.device != self.device:
+            _bad(f"read: the batch is on {batch.device}, the cache on {self.device}")
+        shape = (batch.tokens, self.kv_heads, self.head_dim)
+        k = self._empty(shape, dtype=self._bf16, device=self.device) if k is None else k
+        v = self._empty(shape, dtype=self._bf16, device=self.device) if v is None else v
+        kp, ks = self._rows(k, "k", batch, self.kv_heads, self._bf16)
+        vp, vs = self._rows(v, "v", batch, self.kv_heads, self._bf16)
+        check(lib().q3t_kv4_read(self.ref, batch.ref, kp, ks, vp, vs, self._stream(self.device).cuda_stream))
+        return k, v
 
 
 def kernel_launches():
