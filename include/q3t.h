@@ -192,8 +192,18 @@ q3t_status q3t_session_decode_embeds(q3t_session *s, const float *inputs_embeds,
  * and set the session's current hidden state [hidden] (nullable). */
 q3t_status q3t_session_load_kv(q3t_session *s, const uint16_t *k, const uint16_t *v,
                                int len, const float *hidden);
+/* The session's talker cache, k/v as q3t_session_load_kv takes them (bf16 bit
+ * patterns [num_layers][num_kv_heads][*len][head_dim]): saves a prompt's cache
+ * (a voice-clone reference, say) for later sessions to load.  k == v == NULL
+ * only reports *len; a capacity (positions) below it is INVALID_INPUT.  Of a
+ * 4-bit cache: the values its digits stand for. */
+q3t_status q3t_session_read_kv(q3t_session *s, uint16_t *k, uint16_t *v, int capacity, int *len);
 /* Device time (ms) of the last step / decode call on this session. */
 q3t_status q3t_session_last_ms(q3t_session *s, float *ms);
+/* q3t_session_start with the talker's keys and values in 4 bits (the
+ * q3t_kv4_* format below): 0.31 of the bf16 cache's bytes per token, single
+ * steps on the per-layer kernels.  The other session calls are the same. */
+q3t_status q3t_session_start_kv4(q3t_model *model, const q3t_session_desc *desc, q3t_session **out);
 void q3t_session_free(q3t_session *s);
 
 /* Speech-tokenizer encoder of the voice-clone path (codec/config.rs:79-121,
@@ -463,6 +473,11 @@ typedef struct {
 typedef struct q3t_batch q3t_batch;
 
 q3t_status q3t_batch_create(q3t_model *model, const q3t_batch_desc *desc, q3t_batch **out);
+/* The same with the talker's keys and values in 4 bits (the q3t_kv4_* format
+ * below): a pool of kv_pages pages takes 0.31 of the bf16 pool's memory, and
+ * the frame's attention reads 0.31 of its bytes.  The code predictor's
+ * 17-key caches stay bf16. */
+q3t_status q3t_batch_create_kv4(q3t_model *model, const q3t_batch_desc *desc, q3t_batch **out);
 /* Queue a request; its inputs are copied to device memory now, so a later
  * step finds them resident.  forced_codes (nullable) [max_new_tokens][G]
  * teacher-forces every frame (then EOS is ignored and the request runs
@@ -519,7 +534,8 @@ q3t_status q3t_sample_logits(q3t_model *model, const float *logits, int vocab, c
  * of that device; NULL is its default stream): they enqueue one kernel and
  * return without waiting, allocate nothing, keep nothing between calls, may
  * be captured into a CUDA graph, and leave the calling thread's current
- * device as it was.
+ * device as it was.  q3t_batch_create_kv4 and q3t_session_start_kv4 run the
+ * talker on them.
  *
  * Every 32 dims of a head's key or value share a bf16 scale s and a bf16
  * zero z: z is their minimum rounded down, s is (maximum - z) / 15, and a

@@ -328,9 +328,10 @@ static int bucket_tok(int B) {
   return n;
 }
 
-static void batch_init(q3t_batch *b, q3t_model *m, const q3t_batch_desc &d) {
+static void batch_init(q3t_batch *b, q3t_model *m, const q3t_batch_desc &d, bool kv4) {
   b->m = m;
   b->desc = d;
+  b->kv4 = kv4;
   const auto &tc = m->tc;
   b->A = d.max_active;
   b->G = tc.num_code_groups;
@@ -356,8 +357,13 @@ static void batch_init(q3t_batch *b, q3t_model *m, const q3t_batch_desc &d) {
   const int nkv = tc.talker.num_key_value_heads, L = tc.talker.num_hidden_layers;
   b->n_pages = (int)std::min<int64_t>(m->kv_pages, (int64_t)A * kPtStride);
   b->t_layer_stride = (int64_t)b->n_pages * nkv * kPage * 128;
-  b->tk = ar.alloc<uint16_t>((size_t)b->t_layer_stride * L);
-  b->tv = ar.alloc<uint16_t>((size_t)b->t_layer_stride * L);
+  if (kv4) {
+    b->kv4_layer_stride = (int64_t)b->n_pages * nkv * kv4_block_bytes(128);
+    b->kv4_pool = ar.alloc<uint8_t>((size_t)b->kv4_layer_stride * L);
+  } else {
+    b->tk = ar.alloc<uint16_t>((size_t)b->t_layer_stride * L);
+    b->tv = ar.alloc<uint16_t>((size_t)b->t_layer_stride * L);
+  }
   for (int p = b->n_pages - 1; p >= 0; p--) b->free_pages.push_back(p);
   CK(cudaMallocHost(&b->h_pt, (size_t)A * kPtStride * sizeof(int)));
   memset(b->h_pt, 0, (size_t)A * kPtStride * sizeof(int));
@@ -417,6 +423,7 @@ static void batch_init(q3t_batch *b, q3t_model *m, const q3t_batch_desc &d) {
   b->q = ar.zalloc<uint16_t>((size_t)T * 128 * std::max(tc.talker.num_attention_heads, tc.predictor.num_attention_heads));
   b->attn = ar.zalloc<uint16_t>((size_t)T * 128 * std::max(tc.talker.num_attention_heads, tc.predictor.num_attention_heads));
   b->act = ar.zalloc<uint16_t>((size_t)T * b->I2 / 2);
+  if (kv4) b->qkv = ar.zalloc<float>((size_t)T * b->NQKV);
   b->tlog = ar.zalloc<float>((size_t)T * b->V);
   b->plog = ar.zalloc<float>((size_t)(G - 1) * A * b->PV);
   b->d_err = ar.zalloc<int>(1);
@@ -429,7 +436,7 @@ static void batch_init(q3t_batch *b, q3t_model *m, const q3t_batch_desc &d) {
   {
     const char *e = getenv("Q3T_MK");
     b->mk_grid = mk_grid(m->device);
-    b->use_mk = !(e && e[0] == '0') && b->mk_grid > 0;
+    b->use_mk = !(e && e[0] == '0') && b->mk_grid > 0 && !kv4;  // the streamed kernel reads bf16 pages
     if (!(e && e[0] == '0') && b->mk_grid <= 0)
       fprintf(stderr, "q3t: the streamed small-batch kernel cannot be resident on device %d; "
                       "single-token steps use the per-layer kernels\n", m->device);
@@ -460,7 +467,7 @@ static void batch_init(q3t_batch *b, q3t_model *m, const q3t_batch_desc &d) {
     }
   }
   // metadata
-  b->meta_n = M_HDR + 8 * A + 5 * b->TT();
+  b->meta_n = kv4 ? b->off_krow() + A : b->off_kq();
   b->d_meta = ar.zalloc<int>(b->meta_n);
   CK(cudaMallocHost(&b->h_meta, b->meta_n * sizeof(int)));
   memset(b->h_meta, 0, b->meta_n * sizeof(int));
@@ -568,6 +575,12 @@ static KVView talker_kv(q3t_batch *b) {
   return KVView{b->tk, b->tv, b->t_layer_stride, b->d_pt, kPtStride,
                 b->m->tc.talker.num_key_value_heads};
 }
+// One layer of the talker's 4-bit cache, and the sequences of a talker pass:
+// q_start / kv_len / slot device arrays, n of them.
+static Kv4View talker_kv4(q3t_batch *b, int layer) {
+  return Kv4View{b->kv4_pool + layer * b->kv4_layer_stride, b->d_pt, b->n_pages,
+                 b->m->tc.talker.num_key_value_heads, 128, b->A, kPtStride};
+}
 static KVView pred_kv(q3t_batch *b) {
   return KVView{b->pk, b->pv, b->p_layer_stride, b->d_ppt, 2, b->m->tc.predictor.num_key_value_heads};
 }
@@ -639,6 +652,18 @@ struct ProgBuilder {
     }
     push(p);
   }
+  void kv4(const Kv4Step &s, int max_tok) {
+    const Kv4Step *p = &s;
+    if (!direct) {  // the program outlives this call
+      b->kv4_steps.push_back(s);
+      p = &b->kv4_steps.back();
+    }
+    for (int type : {PH_KV4_APPEND, PH_KV4_ATTEND}) {
+      Phase at = phase(type, max_tok);
+      at.kv4 = p;
+      push(at);
+    }
+  }
   // X = bf16 rows [Tmax][ldx] of a batch buffer, loaded by TMA
   GemmArgs bf16_x(GemmArgs g, const uint16_t *x, int ldx) const { return gemm_bf16_x(b, g, x, ldx); }
   // X = RMSNorm(x rows t * row_mul + row_add) from the residual stream and
@@ -694,8 +719,11 @@ struct ProgBuilder {
   // built the input rows x and their normalised bf16 copy xn.  Afterwards x
   // holds the output residual rows and ss their sum-of-squares partials,
   // and with out_gamma xg holds bf16(x * out_gamma) for a scaled_x reader.
+  // With seqs (the same tokens by sequence) K and V go to the talker's 4-bit
+  // cache instead of kv: the projection leaves raw rows, and append (norms,
+  // rotation, quantisation) and attend follow as kernels of their own.
   void stack(const LMStack &S, KVView kv, TokView tv, int max_tok, int max_units, int pw,
-             const float *out_gamma = nullptr) {
+             const float *out_gamma = nullptr, const Kv4Batch *seqs = nullptr, int max_q = 0, int max_kv = 0) {
     const auto &c = S.cfg;
     const int H = c.hidden_size, I = c.intermediate_size, nh = c.num_attention_heads, nkv = c.num_key_value_heads;
     const int QD = nh * 128;
@@ -703,30 +731,68 @@ struct ProgBuilder {
     for (int l = 0; l < c.num_hidden_layers; l++) {
       GemmArgs q = gemm_args(S.qkv[l], tv.ntok, max_tok);
       q = l == 0 ? bf16_x(q, b->xn, H) : scaled_x(q, S.in_norm[l], eps);
-      q.epi = GE_QKV;
-      q.q_norm = S.q_norm[l];
-      q.k_norm = S.k_norm[l];
-      q.inv_freq = S.inv_freq;
-      q.nh = nh;
-      q.nkv = nkv;
-      q.tv = tv;
-      q.q = b->q;
-      q.kv = kv;
-      q.layer = l;
-      gemm(q, max_tok);
-      Phase at = phase(PH_ATTN, max_tok);
-      AttnArgs &aa = at.attn;
-      aa.q = b->q;
-      aa.kv = kv;
-      aa.layer = l;
-      aa.tv = tv;
-      aa.nh = nh;
-      aa.pw = pw;
-      aa.max_units = max_units;
-      aa.scale = 1.0f / sqrtf(128.0f);
-      aa.ws = b->ws;
-      aa.out = b->attn;
-      push(at);
+      if (seqs) {
+        q.epi = GE_F32;
+        q.y = b->qkv;
+        q.ldy = b->NQKV;
+        gemm(q, max_tok);
+        Kv4Step st{};
+        Kv4AppendArgs &ap = st.append;
+        ap.c = talker_kv4(b, l);
+        ap.b = *seqs;
+        ap.rope.rot = 128;
+        ap.rope.amplitude = 1.f;
+        for (int i = 0; i < 64; i++) ap.rope.freq_pi[i] = std::pow((double)c.rope_theta, -i / 64.0) / M_PI;
+        ap.n_heads = nh;
+        ap.q = b->qkv;
+        ap.k = b->qkv + QD;
+        ap.v = b->qkv + QD + nkv * 128;
+        ap.ldq = ap.ldk = ap.ldv = b->NQKV;
+        ap.q_gamma = S.q_norm[l];
+        ap.k_gamma = S.k_norm[l];
+        ap.eps = eps;
+        ap.q_out = b->q;
+        ap.ldqo = QD;
+        ap.vec = 1;
+        Kv4AttendArgs &at = st.attend;
+        at.c = ap.c;
+        at.b = *seqs;
+        at.n_heads = nh;
+        at.q = b->q;
+        at.ldq = QD;
+        at.out = b->attn;
+        at.ldo = QD;
+        at.scale = (float)(M_LOG2E / std::sqrt(128.0));
+        at.vec = 1;
+        st.max_q = max_q;
+        st.max_kv = max_kv;
+        kv4(st, max_tok);
+      } else {
+        q.epi = GE_QKV;
+        q.q_norm = S.q_norm[l];
+        q.k_norm = S.k_norm[l];
+        q.inv_freq = S.inv_freq;
+        q.nh = nh;
+        q.nkv = nkv;
+        q.tv = tv;
+        q.q = b->q;
+        q.kv = kv;
+        q.layer = l;
+        gemm(q, max_tok);
+        Phase at = phase(PH_ATTN, max_tok);
+        AttnArgs &aa = at.attn;
+        aa.q = b->q;
+        aa.kv = kv;
+        aa.layer = l;
+        aa.tv = tv;
+        aa.nh = nh;
+        aa.pw = pw;
+        aa.max_units = max_units;
+        aa.scale = 1.0f / sqrtf(128.0f);
+        aa.ws = b->ws;
+        aa.out = b->attn;
+        push(at);
+      }
       gemm(resid(bf16_x(gemm_args(S.o[l], tv.ntok, max_tok), b->attn, QD), S.post_norm[l]), max_tok);
       GemmArgs gu = scaled_x(gemm_args(S.gu[l], tv.ntok, max_tok), S.post_norm[l], eps);
       gu.epi = GE_SILU;
@@ -881,13 +947,14 @@ static void check_device_error(q3t_batch *b, const char *what) {
 
 // Prompt chunk / isolated step: input rows already in x; normalises them,
 // runs the talker stack.
-static void run_stack(q3t_batch *b, const LMStack &S, KVView kv, TokView tv, int max_tok, int max_units) {
+static void run_stack(q3t_batch *b, const LMStack &S, KVView kv, TokView tv, int max_tok, int max_units,
+                      const Kv4Batch *seqs = nullptr, int max_kv = 0) {
   const auto &c = S.cfg;
   ProgBuilder P{b, true, {}};
   P.norm(rms_args(b->x, c.hidden_size, 1, 0, Part{}, S.in_norm[0], b->xn, c.hidden_size, c.hidden_size,
                   c.rms_norm_eps, tv.ntok, nullptr, nullptr),
          max_tok);
-  P.stack(S, kv, tv, max_tok, max_units, attn_pw(max_tok));
+  P.stack(S, kv, tv, max_tok, max_units, attn_pw(max_tok), nullptr, seqs, seqs ? max_tok : 0, max_kv);
 }
 
 static SampleArgs base_sample(q3t_batch *b) {
@@ -1008,7 +1075,11 @@ static void build_talker(q3t_batch *b, int mt, int max_units, bool with_prefill,
                     nullptr),
            mt);
   TokView tvt{ntokT, meta + b->off_tseq(), meta + b->off_ttpos(), 0};
-  P.stack(m->talker, talker_kv(b), tvt, mt, max_units, attn_pw(mt));
+  // by sequence: the decode tokens one each, then the chunks, empty ones behind
+  const Kv4Batch seqs{with_prefill ? b->A : std::min(b->A, mt), mt, meta + b->off_kq(), meta + b->off_kkv(),
+                      meta + b->off_krow()};
+  P.stack(m->talker, talker_kv(b), tvt, mt, max_units, attn_pw(mt), nullptr, b->kv4 ? &seqs : nullptr,
+          with_prefill ? 0 : 1, kMaxSeq);
   RmsArgs fn = rms_args(b->x, H, 1, 0, Part{}, m->talker.final_norm, b->xn, H, H, tc.talker.rms_norm_eps, ntokH,
                         b->d_hidden, hslot);
   fn.row_idx = meta + b->off_hrow();
@@ -1323,6 +1394,9 @@ static void prefill(q3t_batch *b, Req *r) {
     hm[0] = n;
     hm[1] = 1;
     hm[2] = s;
+    hm[3] = 0;  // the chunk as one sequence (4-bit cache): q_start, kv_len
+    hm[4] = n;
+    hm[5] = c0 + n;
     for (int i = 0; i < n; i++) {
       hm[8 + i] = s;
       hm[8 + kPrefillTok + i] = c0 + i;
@@ -1331,7 +1405,8 @@ static void prefill(q3t_batch *b, Req *r) {
     CK(cudaMemcpyAsync(dm, hm, ps * sizeof(int), cudaMemcpyHostToDevice, b->st));
     CK(cudaMemcpyAsync(b->x, d_prompt + (size_t)c0 * H, (size_t)n * H * 4, cudaMemcpyDeviceToDevice, b->st));
     TokView tv{dm, dm + 8, dm + 8 + kPrefillTok, 0};
-    run_stack(b, m->talker, talker_kv(b), tv, n, bucket_units(c0 + n, attn_pw(n)));
+    const Kv4Batch seq{1, n, dm + 3, dm + 5, dm + 2};
+    run_stack(b, m->talker, talker_kv(b), tv, n, bucket_units(c0 + n, attn_pw(n)), b->kv4 ? &seq : nullptr, c0 + n);
     last_n = n;
   }
   int *dm = b->d_pmeta + (size_t)(blk0 + nch - 1) * ps;
@@ -1571,14 +1646,24 @@ static void batch_step(q3t_batch *b, q3t_step_stats *stats) {
     hm[b->off_hrow() + i] = i;
     hm[b->off_hslot() + i] = r->slot;
     hm[b->off_hframe() + i] = r->step_idx;
+    if (b->kv4) {
+      hm[b->off_kq() + i] = i;
+      hm[b->off_kkv() + i] = r->cache_len + 1;
+      hm[b->off_krow() + i] = r->slot;
+    }
     S.kv_tokens += r->cache_len + 1;
   }
   // prompt-chunk tokens follow the decode tokens in the talker pass; a chunk
   // that completes its prompt adds its last token to the head
   std::vector<PromptCopy> copies;
   std::vector<Req *> firsts;
-  int t = B, h = B;
+  int t = B, h = B, nseq = B;
   for (const Chunk &c : chunks) {
+    if (b->kv4) {
+      hm[b->off_kq() + nseq] = t;
+      hm[b->off_kkv() + nseq] = c.pos0 + c.n;
+      hm[b->off_krow() + nseq++] = c.r->slot;
+    }
     for (int j = 0; j < c.n; j++) {
       hm[b->off_tseq() + t + j] = c.r->slot;
       hm[b->off_ttpos() + t + j] = c.pos0 + j;
@@ -1594,6 +1679,8 @@ static void batch_step(q3t_batch *b, q3t_step_stats *stats) {
     }
     t += c.n;
   }
+  if (b->kv4)
+    for (int i = nseq; i <= b->A; i++) hm[b->off_kq() + i] = t;  // no rows
   const int F = (int)firsts.size();
   flush_pages(b);
   hm[M_NTOK_B] = B;
@@ -1737,7 +1824,7 @@ static Req *new_request(q3t_batch *b, const q3t_session_desc *d, const int64_t *
 // ----------------------------------------------------------------------------
 // C ABI: batches
 // ----------------------------------------------------------------------------
-extern "C" q3t_status q3t_batch_create(q3t_model *m, const q3t_batch_desc *d, q3t_batch **out) {
+static q3t_status batch_create(q3t_model *m, const q3t_batch_desc *d, bool kv4, q3t_batch **out) {
   if (!m || !d || !out) {
     set_error("q3t_batch_create: null argument");
     return Q3T_INVALID_INPUT;
@@ -1758,7 +1845,7 @@ extern "C" q3t_status q3t_batch_create(q3t_model *m, const q3t_batch_desc *d, q3
   auto *b = new q3t_batch();
   q3t_status rc = guard([&] {
     CK(cudaSetDevice(m->device));
-    batch_init(b, m, *d);
+    batch_init(b, m, *d, kv4);
     if (d->codec_mode == 2) codec_stream_init(m, b);
   });
   if (rc != Q3T_OK) {
@@ -1769,6 +1856,14 @@ extern "C" q3t_status q3t_batch_create(q3t_model *m, const q3t_batch_desc *d, q3
   }
   *out = b;
   return Q3T_OK;
+}
+
+extern "C" q3t_status q3t_batch_create(q3t_model *m, const q3t_batch_desc *d, q3t_batch **out) {
+  return batch_create(m, d, false, out);
+}
+
+extern "C" q3t_status q3t_batch_create_kv4(q3t_model *m, const q3t_batch_desc *d, q3t_batch **out) {
+  return batch_create(m, d, true, out);
 }
 
 extern "C" q3t_status q3t_batch_submit(q3t_batch *b, const q3t_session_desc *req, const int64_t *forced,
@@ -1900,7 +1995,7 @@ struct q3t_session {
   q3t::Req *r = nullptr;
 };
 
-extern "C" q3t_status q3t_session_start(q3t_model *m, const q3t_session_desc *d, q3t_session **out) {
+static q3t_status session_start(q3t_model *m, const q3t_session_desc *d, bool kv4, q3t_session **out) {
   if (!m || !d || !out) {
     set_error("q3t_session_start: null argument");
     return Q3T_INVALID_INPUT;
@@ -1911,7 +2006,7 @@ extern "C" q3t_status q3t_session_start(q3t_model *m, const q3t_session_desc *d,
   bd.codec_mode = 0;
   bd.keep_output = 1;
   q3t_batch *b = nullptr;
-  q3t_status rc = q3t_batch_create(m, &bd, &b);
+  q3t_status rc = batch_create(m, &bd, kv4, &b);
   if (rc != Q3T_OK) return rc;
   b->session_mode = true;
   auto *s = new q3t_session();
@@ -1935,6 +2030,14 @@ extern "C" q3t_status q3t_session_start(q3t_model *m, const q3t_session_desc *d,
   }
   *out = s;
   return Q3T_OK;
+}
+
+extern "C" q3t_status q3t_session_start(q3t_model *m, const q3t_session_desc *d, q3t_session **out) {
+  return session_start(m, d, false, out);
+}
+
+extern "C" q3t_status q3t_session_start_kv4(q3t_model *m, const q3t_session_desc *d, q3t_session **out) {
+  return session_start(m, d, true, out);
 }
 
 static q3t_status session_step(q3t_session *s, const int64_t *forced, float *tl, float *pl, float *hid,
@@ -2061,6 +2164,12 @@ extern "C" q3t_status q3t_session_decode_embeds(q3t_session *s, const float *emb
     int *hm = b->h_meta;
     hm[b->off_slot()] = r->slot;
     hm[b->off_tpos()] = r->cache_len;
+    if (b->kv4) {
+      hm[b->off_kq()] = 0;
+      hm[b->off_kq() + 1] = 1;
+      hm[b->off_kkv()] = r->cache_len + 1;
+      hm[b->off_krow()] = r->slot;
+    }
     hm[M_NTOK_B] = 1;
     hm[M_NTOK_2B] = 2;
     hm[M_ONE] = 1;
@@ -2097,7 +2206,8 @@ extern "C" q3t_status q3t_session_decode_embeds(q3t_session *s, const float *emb
     run_graph(b, std::make_tuple(1, 1, ms), [&] {
       const int *ntok = b->d_meta + M_NTOK_B, *slot = b->d_meta + b->off_slot();
       TokView tvt{ntok, slot, b->d_meta + b->off_tpos(), 0};
-      run_stack(b, m->talker, talker_kv(b), tvt, 1, ms);
+      const Kv4Batch seq{1, 1, b->d_meta + b->off_kq(), b->d_meta + b->off_kkv(), b->d_meta + b->off_krow()};
+      run_stack(b, m->talker, talker_kv(b), tvt, 1, ms, b->kv4 ? &seq : nullptr, kMaxSeq);
       rmsnorm(b->x, b->H, 1, 0, Part{}, m->talker.final_norm, b->xn, b->H, b->H, m->tc.talker.rms_norm_eps, ntok, 1,
               b->d_hidden, slot, b->st);
       GemmArgs hg = gemm_bf16_x(b, gemm_args(m->codec_head, ntok, 1), b->xn, b->H);
@@ -2118,6 +2228,77 @@ extern "C" q3t_status q3t_session_decode_embeds(q3t_session *s, const float *emb
   });
 }
 
+// Runs f for every talker layer with the layer's cache and the first `len`
+// positions of `slot` as one sequence, and two device buffers for its rows.
+template <class F>
+static void kv4_copy(q3t_batch *b, int slot, int len, F &&f) {
+  const auto &c = b->m->tc.talker;
+  DevArena ar;
+  const size_t n = (size_t)len * c.num_key_value_heads * 128;
+  uint16_t *dk = ar.alloc<uint16_t>(n), *dv = ar.alloc<uint16_t>(n);
+  int *seq = ar.alloc<int>(4);
+  const int h[4] = {0, len, len, slot};
+  CK(cudaMemcpyAsync(seq, h, sizeof h, cudaMemcpyHostToDevice, b->st));
+  for (int l = 0; l < c.num_hidden_layers; l++) {
+    Kv4AppendArgs a{};
+    a.c = talker_kv4(b, l);
+    a.b = Kv4Batch{1, len, seq, seq + 2, seq + 3};
+    f(a, dk, dv, l);
+    CK(cudaStreamSynchronize(b->st));
+  }
+}
+
+extern "C" q3t_status q3t_session_read_kv(q3t_session *s, uint16_t *k, uint16_t *v, int capacity, int *len) {
+  if (!s || capacity < 0 || (!k != !v)) {
+    set_error("q3t_session_read_kv: bad argument");
+    return Q3T_INVALID_INPUT;
+  }
+  return guard([&] {
+    q3t_batch *b = s->b;
+    Req *r = s->r;
+    q3t_model *m = b->m;
+    CK(cudaSetDevice(m->device));
+    if (r->slot < 0) FAIL(Q3T_INVALID_INPUT, "session is finished");
+    const int n = r->cache_len;
+    if (len) *len = n;
+    if (!k) return;
+    if (capacity < n) FAIL(Q3T_INVALID_INPUT, "cache of %d positions exceeds the capacity %d", n, capacity);
+    if (n == 0) return;
+    const auto &c = m->tc.talker;
+    const int nkv = c.num_key_value_heads;
+    if (b->kv4) {
+      std::vector<uint16_t> row((size_t)n * nkv * 128);
+      kv4_copy(b, r->slot, n, [&](const Kv4AppendArgs &a, uint16_t *dk, uint16_t *dv, int l) {
+        Kv4ReadArgs rd{};
+        rd.c = a.c;
+        rd.b = a.b;
+        rd.k = dk;
+        rd.v = dv;
+        rd.ldk = rd.ldv = nkv * 128;
+        rd.vec = 1;
+        CK(kv4_read(rd, b->st, false));
+        for (int x = 0; x < 2; x++) {
+          CK(cudaMemcpyAsync(row.data(), x ? dv : dk, row.size() * 2, cudaMemcpyDeviceToHost, b->st));
+          CK(cudaStreamSynchronize(b->st));
+          uint16_t *dst = (x ? v : k) + (size_t)l * nkv * n * 128;
+          for (int h = 0; h < nkv; h++)
+            for (int p = 0; p < n; p++)
+              memcpy(dst + ((size_t)h * n + p) * 128, &row[((size_t)p * nkv + h) * 128], 256);
+        }
+      });
+      return;
+    }
+    DevArena ar;
+    const size_t e = (size_t)c.num_hidden_layers * nkv * n * 128;
+    uint16_t *dk = ar.alloc<uint16_t>(e), *dv = ar.alloc<uint16_t>(e);
+    kv_export(dk, dv, c.num_hidden_layers, n, talker_kv(b), r->slot, b->st);
+    check_launches();
+    CK(cudaMemcpyAsync(k, dk, e * 2, cudaMemcpyDeviceToHost, b->st));
+    CK(cudaMemcpyAsync(v, dv, e * 2, cudaMemcpyDeviceToHost, b->st));
+    CK(cudaStreamSynchronize(b->st));
+  });
+}
+
 extern "C" q3t_status q3t_session_load_kv(q3t_session *s, const uint16_t *k, const uint16_t *v, int len,
                                           const float *hidden) {
   if (!s || (len > 0 && (!k || !v)) || len < 0) {
@@ -2134,7 +2315,25 @@ extern "C" q3t_status q3t_session_load_kv(q3t_session *s, const uint16_t *k, con
     flush_pages(b);
     const auto &c = m->tc.talker;
     const size_t n = (size_t)c.num_hidden_layers * c.num_key_value_heads * len * 128;
-    if (len > 0) {
+    if (len > 0 && b->kv4) {
+      kv4_copy(b, r->slot, len, [&](Kv4AppendArgs ap, uint16_t *dk, uint16_t *dv, int l) {
+        const int nkv = c.num_key_value_heads;
+        std::vector<uint16_t> row((size_t)len * nkv * 128);
+        for (int x = 0; x < 2; x++) {  // [head][position] to [position][head]
+          const uint16_t *src = (x ? v : k) + (size_t)l * nkv * len * 128;
+          for (int h = 0; h < nkv; h++)
+            for (int p = 0; p < len; p++)
+              memcpy(&row[((size_t)p * nkv + h) * 128], src + ((size_t)h * len + p) * 128, 256);
+          CK(cudaMemcpyAsync(x ? dv : dk, row.data(), row.size() * 2, cudaMemcpyHostToDevice, b->st));
+          CK(cudaStreamSynchronize(b->st));
+        }
+        ap.k = dk;
+        ap.v = dv;
+        ap.ldk = ap.ldv = nkv * 128;
+        ap.vec = 1;
+        CK(kv4_append(ap, false, b->st, false));
+      });
+    } else if (len > 0) {
       uint16_t *dk, *dv;
       CK(cudaMalloc(&dk, n * 2));
       CK(cudaMalloc(&dv, n * 2));

@@ -13,6 +13,7 @@
 
 #include "../../include/q3t.h"
 #include "frame.cuh"
+#include "kv4.cuh"
 #include "lm_kernels.cuh"
 #include "mk.cuh"
 
@@ -199,6 +200,13 @@ struct q3t_batch {
   uint16_t *tk = nullptr, *tv = nullptr;
   int64_t t_layer_stride = 0;
   int n_pages = 0;
+  // 4-bit talker pool instead of tk / tv: blocks [layer][page][n_kv], the
+  // projections' raw q/k/v rows, and the steps that the frame programs point at
+  bool kv4 = false;
+  uint8_t *kv4_pool = nullptr;
+  int64_t kv4_layer_stride = 0;  // bytes
+  float *qkv = nullptr;          // [Tmax][NQKV]
+  std::deque<q3t::Kv4Step> kv4_steps;
   std::vector<int> free_pages;
   int *d_pt = nullptr;
   int *h_pt = nullptr;                   // pinned host copy of the page table [A][kPtStride]
@@ -289,6 +297,10 @@ struct q3t_batch {
   int off_hslot() const { return off_tseq() + 2 * TT(); }
   int off_hframe() const { return off_tseq() + 3 * TT(); }
   int off_hrow() const { return off_tseq() + 4 * TT(); }
+  // the talker pass by sequence (4-bit cache): q_start [A + 1], kv_len [A], slot [A]
+  int off_kq() const { return off_tseq() + 5 * TT(); }
+  int off_kkv() const { return off_kq() + A + 1; }
+  int off_krow() const { return off_kkv() + A; }
   int64_t admit_counter = 0;
   int pmeta_stride() const { return 8 + 2 * q3t::kPrefillTok + 8; }
 };

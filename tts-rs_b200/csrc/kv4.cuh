@@ -75,6 +75,13 @@ struct Kv4ReadArgs {
   int splits;
 };
 
+// Append and attend of one layer of a talker pass.
+struct Kv4Step {
+  Kv4AppendArgs append;
+  Kv4AttendArgs attend;
+  int max_q, max_kv;
+};
+
 // max_q / max_kv: the most tokens and keys of a sequence, as the caller knows
 // them; they choose the launch shape only (0: unknown).  Launch errors are
 // returned; `pdl` lets the launch overlap the tail of the one before it.

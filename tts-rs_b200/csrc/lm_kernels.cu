@@ -17,6 +17,7 @@
 
 #include <cudaTypedefs.h>
 
+#include "kv4.cuh"
 #include "lm_device.cuh"
 #include "umma.cuh"
 
@@ -830,6 +831,23 @@ void kv_import(const uint16_t *k, const uint16_t *v, int layers, int len, KVView
   g_launches++;
 }
 
+__global__ void k_kv_export(uint16_t *k, uint16_t *v, int len, KVView kv, int seq) {
+  const int l = blockIdx.z, h = blockIdx.y, j = blockIdx.x;
+  const size_t dst = (((size_t)l * kv.n_kv + h) * len + j) * 128;
+  const size_t src = l * kv.layer_stride + page_elem(kv, seq, j, h);
+  for (int d = threadIdx.x; d < 128; d += blockDim.x) {
+    k[dst + d] = kv.k[src + d];
+    v[dst + d] = kv.v[src + d];
+  }
+}
+
+void kv_export(uint16_t *k, uint16_t *v, int layers, int len, KVView kv, int seq, cudaStream_t st) {
+  if (len <= 0) return;
+  k_kv_export<<<dim3(len, kv.n_kv, layers), 128, 0, st>>>(k, v, len, kv, seq);
+  note(cudaGetLastError(), "k_kv_export");
+  g_launches++;
+}
+
 void run_phases(const Phase *ph, int n, cudaStream_t st) {
   for (int i = 0; i < n; i++) {
     const Phase &p = ph[i];
@@ -838,6 +856,10 @@ void run_phases(const Phase *ph, int n, cudaStream_t st) {
       case PH_GEMM: gemm(p.gemm, p.max_tok, st); break;
       case PH_ATTN: attention_launch(p.attn, p.max_tok, st); break;
       case PH_SAMPLE: sample(p.smp, p.max_tok, st, p.has_tail ? &p.tail : nullptr); break;
+      case PH_KV4_APPEND: note(kv4_append(p.kv4->append, true, st, true), "k_kv4_append"); break;
+      case PH_KV4_ATTEND:
+        note(kv4_attend(p.kv4->attend, p.kv4->max_q, p.kv4->max_kv, st, true), "k_kv4_attend");
+        break;
       default: note(cudaErrorInvalidValue, "run_phases: unknown phase"); break;
     }
   }

@@ -278,7 +278,9 @@ void sample(const SampleArgs &a, int max_tok, cudaStream_t st, const RmsArgs *ta
 // A decode frame as a list of phases, each one kernel launch (captured once
 // into a CUDA graph and replayed).
 // ---------------------------------------------------------------------------
-enum PhaseType { PH_NORM = 1, PH_GEMM = 2, PH_ATTN = 3, PH_SAMPLE = 4 };
+enum PhaseType { PH_NORM = 1, PH_GEMM = 2, PH_ATTN = 3, PH_SAMPLE = 4, PH_KV4_APPEND = 5, PH_KV4_ATTEND = 6 };
+
+struct Kv4Step;  // kv4.cuh
 
 struct Phase {
   int type;
@@ -290,6 +292,7 @@ struct Phase {
     GemmArgs gemm;
     AttnArgs attn;
     SampleArgs smp;
+    const Kv4Step *kv4;  // PH_KV4_*: the layer's append and attend, owned by the batch
   };
   RmsArgs tail;
 };
@@ -310,5 +313,7 @@ void clone_rows(const float *spk, const int64_t *codes, int G, int T, const uint
 // Scatter dense bf16 K/V [layers][n_kv][len][hd] into the pages of `seq`.
 void kv_import(const uint16_t *k, const uint16_t *v, int layers, int len, KVView kv, int seq,
                cudaStream_t st);
+// The reverse: the pages of `seq` to dense k, v.
+void kv_export(uint16_t *k, uint16_t *v, int layers, int len, KVView kv, int seq, cudaStream_t st);
 
 }  // namespace q3t

@@ -137,6 +137,7 @@ EXPORTS = [
     "q3t_speaker_encoder_load", "q3t_speaker_encoder_free", "q3t_speaker_embed", "q3t_speaker_mel",
     "q3t_session_seed_voice_clone", "q3t_wav_read", "q3t_resample_linear",
     "q3t_rope_freqs", "q3t_kv4_append", "q3t_kv4_attend", "q3t_kv4_read",
+    "q3t_batch_create_kv4", "q3t_session_start_kv4", "q3t_session_read_kv",
 ]
 
 
@@ -247,6 +248,10 @@ def lib():
         L.q3t_speaker_encoder_free.restype = None
         L.q3t_speaker_embed.argtypes = [C.c_void_p, _F, C.c_int64, _F]
         L.q3t_speaker_mel.argtypes = [C.c_void_p, _F, C.c_int64, _F, C.c_int, C.POINTER(C.c_int)]
+        L.q3t_batch_create_kv4.argtypes = [C.c_void_p, C.POINTER(BatchDesc), C.POINTER(C.c_void_p)]
+        L.q3t_session_start_kv4.argtypes = [C.c_void_p, C.POINTER(SessionDesc), C.POINTER(C.c_void_p)]
+        L.q3t_session_read_kv.argtypes = [C.c_void_p, C.POINTER(C.c_uint16), C.POINTER(C.c_uint16), C.c_int,
+                                          C.POINTER(C.c_int)]
         L.q3t_rope_freqs.argtypes = [C.POINTER(RopeView), C.POINTER(C.c_double)]
         L.q3t_kv4_append.argtypes = [C.POINTER(KV4CacheView), C.POINTER(KV4BatchView), C.POINTER(KV4Rows),
                                      C.POINTER(RopeView), C.c_void_p]
@@ -565,9 +570,10 @@ class Model:
 
     # -- sessions -------------------------------------------------------------
     def session(self, prompt, trailing, pad, talker_sampling=None, predictor_sampling=None,
-                max_new_tokens=64, eos=-1, suppress=None, forced_first=-1, first_logits=False):
+                max_new_tokens=64, eos=-1, suppress=None, forced_first=-1, first_logits=False, kv_bits=16):
+        """kv_bits 4: the talker's keys and values in 4 bits (q3t_session_start_kv4)."""
         return Session(self, prompt, trailing, pad, talker_sampling, predictor_sampling,
-                       max_new_tokens, eos, suppress, forced_first, first_logits)
+                       max_new_tokens, eos, suppress, forced_first, first_logits, kv_bits)
 
     # -- codec ------------------------------------------------------------------
     def codec_out_len(self, T):
@@ -658,8 +664,9 @@ class Model:
                                       kept.ctypes.data_as(C.POINTER(C.c_uint8))))
         return tok.value, kept.astype(bool)
 
-    def batch(self, max_active=64, codec_mode=0, chunk_frames=16, left_context=8, keep_output=1):
-        return Batch(self, max_active, codec_mode, chunk_frames, left_context, keep_output)
+    def batch(self, max_active=64, codec_mode=0, chunk_frames=16, left_context=8, keep_output=1, kv_bits=16):
+        """kv_bits 4: the talker's keys and values in 4 bits (q3t_batch_create_kv4)."""
+        return Batch(self, max_active, codec_mode, chunk_frames, left_context, keep_output, kv_bits)
 
 
 def _session_desc(model, prompt, trailing, pad, ts, cs, max_new, eos, suppress, forced_first,
@@ -684,9 +691,15 @@ def _session_desc(model, prompt, trailing, pad, ts, cs, max_new, eos, suppress, 
     return d
 
 
+def _by_bits(kv_bits, bf16, kv4):
+    if kv_bits not in (16, 4):
+        raise Q3TError(INVALID_INPUT, f"kv_bits {kv_bits}: the talker cache holds bf16 (16) or 4 bits")
+    return kv4 if kv_bits == 4 else bf16
+
+
 class Session:
     def __init__(self, model, prompt, trailing, pad, ts, cs, max_new, eos, suppress, forced_first,
-                 want_first_logits):
+                 want_first_logits, kv_bits=16):
         self.model = model
         tc = model.talker_cfg
         self._keep = []
@@ -694,7 +707,7 @@ class Session:
         d = _session_desc(model, prompt, trailing, pad, ts, cs, max_new, eos, suppress,
                           forced_first, self.first_logits, self._keep)
         h = C.c_void_p()
-        check(lib().q3t_session_start(model.h, C.byref(d), C.byref(h)))
+        check(_by_bits(kv_bits, lib().q3t_session_start, lib().q3t_session_start_kv4)(model.h, C.byref(d), C.byref(h)))
         self.h = h
 
     def step(self):
@@ -745,6 +758,15 @@ class Session:
         check(lib().q3t_session_load_kv(self.h, k.ctypes.data_as(C.POINTER(C.c_uint16)),
                                         v.ctypes.data_as(C.POINTER(C.c_uint16)), length, _fp(h)))
 
+    def read_kv(self):
+        """The talker cache as load_kv takes it: (k, v) bf16 bits [layers][kv heads][len][head_dim]."""
+        n, c = C.c_int(), self.model.talker_cfg.talker
+        check(lib().q3t_session_read_kv(self.h, None, None, 0, C.byref(n)))
+        k, v = (np.zeros((c.n_layers, c.n_kv, n.value, c.head_dim), np.uint16) for _ in range(2))
+        p = C.POINTER(C.c_uint16)
+        check(lib().q3t_session_read_kv(self.h, k.ctypes.data_as(p), v.ctypes.data_as(p), n.value, C.byref(n)))
+        return k, v
+
     def last_ms(self):
         ms = C.c_float()
         check(lib().q3t_session_last_ms(self.h, C.byref(ms)))
@@ -762,11 +784,11 @@ class Session:
 class Batch:
     """Ragged continuous batching over one model (q3t_batch_*)."""
 
-    def __init__(self, model, max_active, codec_mode, chunk_frames, left_context, keep_output):
+    def __init__(self, model, max_active, codec_mode, chunk_frames, left_context, keep_output, kv_bits=16):
         self.model = model
         d = BatchDesc(max_active, codec_mode, chunk_frames, left_context, keep_output)
         h = C.c_void_p()
-        check(lib().q3t_batch_create(model.h, C.byref(d), C.byref(h)))
+        check(_by_bits(kv_bits, lib().q3t_batch_create, lib().q3t_batch_create_kv4)(model.h, C.byref(d), C.byref(h)))
         self.h = h
         self._keep = {}
 
