@@ -531,7 +531,7 @@ q3t_status q3t_sample_logits(q3t_model *model, const float *logits, int vocab, c
 /* No reference counterpart (the reference keeps a dense bf16 cache, kv.rs):
  * a decoder layer's keys and values in 4 bits, in pages of 16 tokens.  These
  * calls take device pointers on `device` and run on `stream` (a cudaStream_t
- * of that device; NULL is its default stream): they enqueue one kernel and
+ * of that device; NULL is its default stream): they enqueue their kernels and
  * return without waiting, allocate nothing, keep nothing between calls, may
  * be captured into a CUDA graph, and leave the calling thread's current
  * device as it was.  q3t_batch_create_kv4 and q3t_session_start_kv4 run the
@@ -631,9 +631,14 @@ q3t_status q3t_kv4_append(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch
  * appended ones among them; out = softmax(scale q . k) v in bf16, query head h
  * reading kv head h / (num_heads / num_kv_heads).  Keys whose position has no
  * page are not seen; a row that sees no key gives zeros.  out must not
- * overlap q. */
+ * overlap q.  workspace: device memory on a 16-byte boundary that this call
+ * alone uses while it runs (calls that may overlap, and graphs that may replay
+ * at once, need one each); it needs no initialisation and holds nothing
+ * between calls.  64 KiB at least; Q3T_KV4_WORKSPACE serves the widest launch. */
+#define Q3T_KV4_WORKSPACE (4 << 20)
 q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, int num_heads, const uint16_t *q,
-                          int64_t q_stride, float scale, int window, uint16_t *out, int64_t out_stride, void *stream);
+                          int64_t q_stride, float scale, int window, uint16_t *out, int64_t out_stride,
+                          void *workspace, int64_t workspace_bytes, void *stream);
 /* What the cache holds for the batch's rows, as bf16 rows (k or v nullable):
  * n s + z rounded once; zeros where a position has no page. */
 q3t_status q3t_kv4_read(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, uint16_t *k, int64_t k_stride,

@@ -62,7 +62,7 @@ BAD_ROPE = [dict(rotary_dim=136), dict(rotary_dim=-8), dict(rotary_dim=12), dict
 def test_bad_cache_is_refused(bad):
     L = q3t.lib()
     assert call_append(cache(**bad), batch(), rows()) == INVALID
-    assert L.q3t_kv4_attend(C.byref(cache(**bad)), C.byref(batch()), 16, 1 << 20, 2048, 0.1, 0, 1 << 20, 2048, None) == INVALID
+    assert L.q3t_kv4_attend(C.byref(cache(**bad)), C.byref(batch()), 16, 1 << 20, 2048, 0.1, 0, 1 << 20, 2048, 1 << 21, 1 << 22, None) == INVALID
     assert L.q3t_kv4_read(C.byref(cache(**bad)), C.byref(batch()), 1 << 20, 1024, 1 << 20, 1024, None) == INVALID
     assert L.q3t_last_error()
 
@@ -71,7 +71,7 @@ def test_bad_cache_is_refused(bad):
 def test_bad_batch_is_refused(bad):
     L = q3t.lib()
     assert call_append(cache(), batch(**bad), rows()) == INVALID
-    assert L.q3t_kv4_attend(C.byref(cache()), C.byref(batch(**bad)), 16, 1 << 20, 2048, 0.1, 0, 1 << 20, 2048, None) == INVALID
+    assert L.q3t_kv4_attend(C.byref(cache()), C.byref(batch(**bad)), 16, 1 << 20, 2048, 0.1, 0, 1 << 20, 2048, 1 << 21, 1 << 22, None) == INVALID
     assert L.q3t_kv4_read(C.byref(cache()), C.byref(batch(**bad)), 1 << 20, 1024, 1 << 20, 1024, None) == INVALID
 
 
@@ -100,7 +100,13 @@ def test_rotation_wider_than_the_head_is_refused():
     (16, (1 << 20) + 1, 2048, 0.1, 0, 1 << 20, 2048)])
 def test_bad_attend_is_refused(heads, q, qs, scale, window, out, os_):
     assert q3t.lib().q3t_kv4_attend(C.byref(cache()), C.byref(batch()), heads, q, qs, scale, window, out, os_,
-                                    None) == INVALID
+                                    1 << 21, 1 << 22, None) == INVALID
+
+
+@pytest.mark.parametrize("ws, size", [(None, 1 << 22), (1 << 21, (64 << 10) - 1), (1 << 21, 0), ((1 << 21) + 8, 1 << 22)])
+def test_bad_workspace_is_refused(ws, size):
+    assert q3t.lib().q3t_kv4_attend(C.byref(cache()), C.byref(batch()), 16, 1 << 20, 2048, 0.1, 0, 1 << 20, 2048, ws,
+                                    size, None) == INVALID
 
 
 def test_null_structs_and_read_without_outputs_are_refused():
@@ -118,7 +124,7 @@ def test_empty_batches_need_no_gpu():
     L = q3t.lib()
     for b in (batch(num_seqs=0, q_start=None, kv_len=None), batch(num_tokens=0)):
         assert call_append(cache(), b, rows(q=None, k=None, v=None, q_out=None)) == q3t.OK
-        assert L.q3t_kv4_attend(C.byref(cache()), C.byref(b), 16, None, 0, 0.1, 0, None, 0, None) == q3t.OK
+        assert L.q3t_kv4_attend(C.byref(cache()), C.byref(b), 16, None, 0, 0.1, 0, None, 0, None, 0, None) == q3t.OK
         assert L.q3t_kv4_read(C.byref(cache()), C.byref(b), None, 0, None, 0, None) == q3t.OK
 
 

@@ -423,7 +423,10 @@ static void batch_init(q3t_batch *b, q3t_model *m, const q3t_batch_desc &d, bool
   b->q = ar.zalloc<uint16_t>((size_t)T * 128 * std::max(tc.talker.num_attention_heads, tc.predictor.num_attention_heads));
   b->attn = ar.zalloc<uint16_t>((size_t)T * 128 * std::max(tc.talker.num_attention_heads, tc.predictor.num_attention_heads));
   b->act = ar.zalloc<uint16_t>((size_t)T * b->I2 / 2);
-  if (kv4) b->qkv = ar.zalloc<float>((size_t)T * b->NQKV);
+  if (kv4) {
+    b->qkv = ar.zalloc<float>((size_t)T * b->NQKV);
+    b->kv4_ws = ar.alloc<uint8_t>(kKv4Workspace);
+  }
   b->tlog = ar.zalloc<float>((size_t)T * b->V);
   b->plog = ar.zalloc<float>((size_t)(G - 1) * A * b->PV);
   b->d_err = ar.zalloc<int>(1);
@@ -766,6 +769,7 @@ struct ProgBuilder {
         at.vec = 1;
         st.max_q = max_q;
         st.max_kv = max_kv;
+        st.ws = b->kv4_ws;
         kv4(st, max_tok);
       } else {
         q.epi = GE_QKV;
@@ -1077,7 +1081,7 @@ static void build_talker(q3t_batch *b, int mt, int max_units, bool with_prefill,
   TokView tvt{ntokT, meta + b->off_tseq(), meta + b->off_ttpos(), 0};
   // by sequence: the decode tokens one each, then the chunks, empty ones behind
   const Kv4Batch seqs{with_prefill ? b->A : std::min(b->A, mt), mt, meta + b->off_kq(), meta + b->off_kkv(),
-                      meta + b->off_krow()};
+                      meta + b->off_krow(), 0};
   P.stack(m->talker, talker_kv(b), tvt, mt, max_units, attn_pw(mt), nullptr, b->kv4 ? &seqs : nullptr,
           with_prefill ? 0 : 1, kMaxSeq);
   RmsArgs fn = rms_args(b->x, H, 1, 0, Part{}, m->talker.final_norm, b->xn, H, H, tc.talker.rms_norm_eps, ntokH,
@@ -1405,7 +1409,7 @@ static void prefill(q3t_batch *b, Req *r) {
     CK(cudaMemcpyAsync(dm, hm, ps * sizeof(int), cudaMemcpyHostToDevice, b->st));
     CK(cudaMemcpyAsync(b->x, d_prompt + (size_t)c0 * H, (size_t)n * H * 4, cudaMemcpyDeviceToDevice, b->st));
     TokView tv{dm, dm + 8, dm + 8 + kPrefillTok, 0};
-    const Kv4Batch seq{1, n, dm + 3, dm + 5, dm + 2};
+    const Kv4Batch seq{1, n, dm + 3, dm + 5, dm + 2, 0};
     run_stack(b, m->talker, talker_kv(b), tv, n, bucket_units(c0 + n, attn_pw(n)), b->kv4 ? &seq : nullptr, c0 + n);
     last_n = n;
   }
@@ -2206,7 +2210,7 @@ extern "C" q3t_status q3t_session_decode_embeds(q3t_session *s, const float *emb
     run_graph(b, std::make_tuple(1, 1, ms), [&] {
       const int *ntok = b->d_meta + M_NTOK_B, *slot = b->d_meta + b->off_slot();
       TokView tvt{ntok, slot, b->d_meta + b->off_tpos(), 0};
-      const Kv4Batch seq{1, 1, b->d_meta + b->off_kq(), b->d_meta + b->off_kkv(), b->d_meta + b->off_krow()};
+      const Kv4Batch seq{1, 1, b->d_meta + b->off_kq(), b->d_meta + b->off_kkv(), b->d_meta + b->off_krow(), 0};
       run_stack(b, m->talker, talker_kv(b), tvt, 1, ms, b->kv4 ? &seq : nullptr, kMaxSeq);
       rmsnorm(b->x, b->H, 1, 0, Part{}, m->talker.final_norm, b->xn, b->H, b->H, m->tc.talker.rms_norm_eps, ntok, 1,
               b->d_hidden, slot, b->st);
@@ -2242,7 +2246,7 @@ static void kv4_copy(q3t_batch *b, int slot, int len, F &&f) {
   for (int l = 0; l < c.num_hidden_layers; l++) {
     Kv4AppendArgs a{};
     a.c = talker_kv4(b, l);
-    a.b = Kv4Batch{1, len, seq, seq + 2, seq + 3};
+    a.b = Kv4Batch{1, len, seq, seq + 2, seq + 3, 0};
     f(a, dk, dv, l);
     CK(cudaStreamSynchronize(b->st));
   }

@@ -206,6 +206,7 @@ struct q3t_batch {
   uint8_t *kv4_pool = nullptr;
   int64_t kv4_layer_stride = 0;  // bytes
   float *qkv = nullptr;          // [Tmax][NQKV]
+  uint8_t *kv4_ws = nullptr;     // kKv4Workspace bytes
   std::deque<q3t::Kv4Step> kv4_steps;
   std::vector<int> free_pages;
   int *d_pt = nullptr;

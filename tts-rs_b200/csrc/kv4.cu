@@ -47,7 +47,7 @@ Q3T_DEV void seq_rows(const Kv4Batch &b, int s, int &t0, int &n, int &pos0) {
 // Page of positions [16 p, 16 p + 16) of sequence s; -1 where the table or
 // the pool has none.
 Q3T_DEV int page_of(const Kv4View &c, const Kv4Batch &b, int s, int p) {
-  const int row = b.table_row ? b.table_row[s] : s;
+  const int row = b.table_row ? b.table_row[s] : b.first + s;
   if (p < 0 || p >= c.table_stride || row < 0 || row >= c.table_rows) return -1;
   const int id = c.table[(size_t)row * c.table_stride + p];
   return id >= 0 && id < c.num_pages ? id : -1;
@@ -386,27 +386,32 @@ __global__ void __launch_bounds__(kReadThreads) k_kv4_read(const __grid_constant
 //   score = sum_j [ s_j sum_{d in j} q_d n_d + z_j sum_{d in j} q_d ]
 //   out_d = sum_keys (p s_j) n_d + sum_keys p z_j,  d in group j
 // so the tensor cores see digits only, and scales and zeros enter once per
-// (key, group).  The fragment rows are (query row r, group j): row (r, j) of
-// the score product holds q in the dims of group j and zeros elsewhere, its
-// accumulator is the group's share of the score, and the value product's
-// column (r, j) holds p s_j.  Every lane then scales its own group's four
-// keys of a page, two shuffles add the groups up, and the accumulators of
-// both products meet without a transpose.
+// (key, group).  The digits are the A operands (16 keys x 16 dims of K, 16
+// dims x 16 keys of V) and the 8 columns are (query row r, group j): column
+// (r, j) of the score product holds q in the dims of group j and zeros
+// elsewhere, its accumulator is the group's share of the score; column (r, j)
+// of the value product holds p s_j.  So no lane computes what no one needs:
+// a lane scales the shares of two columns for two keys, one shuffle joins the
+// groups of a row, and p s goes from the accumulator's order to the operand's
+// by one matrix transpose per 8 keys.
 //
-// A unit is (sequence, R query rows of one kv head), R = 8 NT / G; a cluster
-// of CTAs shares a unit's pages, a warp takes two pages at a time through a
-// cp.async ring, and the (m, l, o) parts of warps and CTAs are joined in
-// order through shared and distributed shared memory: one launch, nothing
-// kept between calls.
+// A unit is (sequence, R query rows of one kv head), R = 8 NT / G, and its
+// keys go by steps of two pages; a warp streams steps through a cp.async
+// ring.  Lengths are ragged, so the steps of a kv head's units are one list, cut
+// into equal runs for the warps of a grid that fills the GPU once; neighbouring
+// CTAs take the same run of different kv heads, whose blocks are neighbours.  A unit that
+// lies inside a warp's run is finished there; the (m, l, o) parts of one that
+// does not are joined in order, by the CTA where it has them all, otherwise
+// by k_kv4_combine from the workspace.  Nothing is kept between calls.
 //
 // f16 holds q times a power of two per row (its 11 bits keep a bf16 q whole
-// down to 2^-25 of the row's largest) and p s times a power of two per warp,
-// which follows the largest value scale: p s is rounded to 11 bits, as
-// against the 8 of the output.  All sums, m and l are in 32 bits.
+// down to 2^-25 of the row's largest) and p s, where p carries a power of two
+// per warp that follows the largest value scale (m is offset by its logarithm,
+// so l and o carry it too and it leaves with the division): p s is rounded to
+// 11 bits, as against the 8 of the output.  All sums, m and l are in 32 bits.
 // ---------------------------------------------------------------------------
 Q3T_DEV void mma_f16(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
       "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -415,97 +420,236 @@ Q3T_DEV uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
+Q3T_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 // 2^(14 - exponent of x), so that x times it lies in [2^14, 2^15)
 Q3T_DEV float to_2p14(float x) {
   const int e = (int)(__float_as_uint(x) >> 23 & 0xff);  // x >= 0
   const int f = min(max(127 + 14 + 127 - e, 1), 253);
   return __uint_as_float((uint32_t)f << 23);
 }
-Q3T_DEV float ld_cluster_f1(const float *p, uint32_t rank) {
-  uint32_t remote;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
+// exponent of x >= 0 as a float's field has it
+Q3T_DEV int exponent(float x) { return (int)(__float_as_uint(x) >> 23 & 0xff) - 127; }
+// an 8 x 8 tile of f16, rows in accumulator order, transposed
+Q3T_DEV uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 // weight of a part with running maximum m and sum l under the joint maximum
 // M; a part without keys has none, one with NaN scores keeps them
 Q3T_DEV float part_weight(float m, float l, float M) {
   if (m == -INFINITY) return l == 0.f ? 0.f : 1.f;
-  return exp2f(m - M);
+  return ex2(m - M);
 }
 
-constexpr int kAttendWarps = 4;
+// A sequence's rows, as the kernel keeps them: token rows from t0, n * heads
+// of a kv head = `total` query rows, the first at position pos0.
+struct SeqRows {
+  int t0, total, pos0, table_row;
+};
+// Query rows [row0, row0 + nrow) of it and the pages they see.
+struct Unit {
+  int row0, nrow, pos_lo, pos_hi, pg_lo, pages;
+};
+// token of a query row: a decode step has one, and no division then
+Q3T_DEV int token_of(int row, int gq) { return row < gq ? 0 : row / gq; }
+template <int R>
+Q3T_DEV Unit unit_of(const SeqRows &s, int row0, int gq, int window) {
+  Unit u;
+  u.row0 = row0;
+  u.nrow = min(R, s.total - row0);
+  u.pos_lo = s.pos0 + token_of(row0, gq);
+  u.pos_hi = s.pos0 + token_of(row0 + max(u.nrow, 1) - 1, gq);
+  u.pg_lo = window > 0 ? max(0, u.pos_lo - window + 1) >> 4 : 0;
+  u.pages = u.pos_hi < 0 ? 0 : max(0, (u.pos_hi >> 4) + 1 - u.pg_lo);
+  return u;
+}
+// steps of a unit: one at least, so that rows without keys are answered too
+constexpr int kStepPages = 2;
+Q3T_DEV int unit_steps(const Unit &u) { return u.nrow > 0 ? max(1, (u.pages + kStepPages - 1) / kStepPages) : 0; }
 
 template <int D, int NT>
 struct AttendCfg {
   static constexpr int G = D / 32, R = NT * 8 / G, BLK = kv4_block_bytes(D);
-  static constexpr int NP = 2, ST = 3;  // pages of a step, steps in the ring
+  static constexpr int NP = kStepPages, ST = 2;  // pages of a step, steps in the ring
+  static constexpr int W = 4;                    // warps of a CTA
   static constexpr int RING = ST * NP * BLK;
-  static constexpr size_t kSmem = (size_t)kAttendWarps * RING;
+  static constexpr int PART = R * (2 + G + D);   // floats of a part: m [R], l [R], z [R][G], o [R][D]
+  static constexpr int MAXSEQ = 512;             // sequences of a launch
+  static constexpr size_t smem(int seqs) {
+    return (size_t)W * RING + W * 2 * PART * 4 + seqs * sizeof(SeqRows) + (seqs + 1) * 4;
+  }
 };
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kAttendWarps * 32) k_kv4_attend(const __grid_constant__ Kv4AttendArgs a, int csize,
-                                                                  int direct) {
-  using Cfg = AttendCfg<D, NT>;
-  constexpr int G = Cfg::G, R = Cfg::R, BLK = Cfg::BLK, NP = Cfg::NP, ST = Cfg::ST, W = kAttendWarps, MT = D / 16;
-  extern __shared__ __align__(16) uint8_t ring_all[];
-  __shared__ float s_m[W][R], s_l[W][R], s_z[W][R][G];
-  __shared__ float c_m[R], c_l[R], c_o[R][D];
-  pdl_wait();
-  pdl_launch();
-  const int rank = blockIdx.x % csize, unit = blockIdx.x / csize, kvh = unit % a.c.n_kv;
-  const int gq = a.n_heads / a.c.n_kv;
-  int s, tile;
-  if (direct) {
-    s = unit / a.c.n_kv;
-    tile = 0;
-  } else if (!find_item(
-                 a.b.num_seqs, unit / a.c.n_kv,
-                 [&](int q) {
-                   int t0, n, pos0;
-                   seq_rows(a.b, q, t0, n, pos0);
-                   return (int)(((int64_t)n * gq + R - 1) / R);
-                 },
-                 s, tile)) {
-    return;
-  }
-  int t0, n, pos0;
-  seq_rows(a.b, s, t0, n, pos0);
-  const int total = n * gq, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, j = g % G;
-  uint8_t *ring = ring_all + warp * Cfg::RING;
-  // a sequence with more rows than the caller announced takes more turns
-  for (int row0 = tile * R; row0 < total; row0 += direct ? R : total) {
-    const int nrow = min(R, total - row0);
-    const int pos_lo = pos0 + row0 / gq, pos_hi = pos0 + (row0 + nrow - 1) / gq;
-    const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
-    const int pg_lo = key_lo >> 4, pg_hi = pos_hi < 0 ? pg_lo : (pos_hi >> 4) + 1;
-    const int per = (max(pg_hi - pg_lo, 0) + csize - 1) / csize;
-    const int p_beg = pg_lo + rank * per, p_end = min(p_beg + per, pg_hi);
-    const int n_it = max(0, (p_end - p_beg - warp * NP + W * NP - 1) / (W * NP));
+template <int D>
+Q3T_DEV void store_out(const Kv4AttendArgs &a, int t0, int row, int kvh, int d, float L, float o) {
+  const int gq = a.n_heads / a.c.n_kv, tok = token_of(row, gq), head = kvh * gq + row - tok * gq;
+  a.out[(size_t)(t0 + tok) * a.ldo + (size_t)head * D + d] = f2bf(L == 0.f ? 0.f : o / L);  // no keys: zeros
+}
 
-    // ---- queries ----
-    uint32_t qa[NT][2][2];
-    float qs[NT], sc[NT];
-    int lim[NT], low[NT];
+// The step list of a kv head: steps pre[i] .. pre[i + 1] - 1 are those of
+// rows [row0, row0 + R) of sequence i.
+struct StepList {
+  const int *pre;
+  const SeqRows *seq;
+  int n, row0;
+};
+
+// Where the copies of a warp's run are: the block of up to 16 steps of one
+// unit whose pages are in `ids` (by lane), and the block after it.
+template <int R>
+struct PageCursor {
+  int seq, step, end;   // sequence, next step of its unit, end of the unit's steps in the run
+  int block, left;      // first step of the block, steps of the run not yet taken
+  int pg_lo, pages;     // of the unit
+  int ids, next_ids;
+  int next_seq, next_step, next_end, next_lo, next_pages;
+  static constexpr int kBlock = 32 / kStepPages;
+
+  Q3T_DEV void look(const Kv4AttendArgs &a, const StepList &L, int s, int step, int lo, int n, int &out) {
+    const int p = lo + step * kStepPages + (threadIdx.x & 31);
+    out = -1;
+    if (p < lo + n && p < a.c.table_stride) {
+      const int row = L.seq[s].table_row;
+      if (row >= 0 && row < a.c.table_rows) out = a.c.table[(size_t)row * a.c.table_stride + p];
+    }
+  }
+  // the block after (seq, block), its pages on their way
+  Q3T_DEV void after(const Kv4AttendArgs &a, const StepList &L, int gq, int left_after) {
+    next_seq = seq, next_step = block + kBlock, next_end = end, next_lo = pg_lo, next_pages = pages;
+    if (next_step >= end) {
+      if (left_after <= 0) {
+        next_ids = -1;
+        return;
+      }
+      next_step = 0;
+      do next_seq++;
+      while (L.pre[next_seq + 1] == L.pre[next_seq]);
+      next_end = min(L.pre[next_seq + 1] - L.pre[next_seq], left_after);
+      const Unit u = unit_of<R>(L.seq[next_seq], L.row0, gq, a.window);
+      next_lo = u.pg_lo, next_pages = u.pages;
+    }
+    look(a, L, next_seq, next_step, next_lo, next_pages, next_ids);
+  }
+  Q3T_DEV void start(const Kv4AttendArgs &a, const StepList &L, int gq, int s, int at, int to) {
+    const Unit u = unit_of<R>(L.seq[s], L.row0, gq, a.window);
+    seq = s, step = block = at - L.pre[s], left = to - at;
+    end = min(L.pre[s + 1] - L.pre[s], step + left);
+    pg_lo = u.pg_lo, pages = u.pages;
+    look(a, L, s, step, pg_lo, pages, ids);
+  }
+  // one step taken (after() once before the first)
+  Q3T_DEV void advance(const Kv4AttendArgs &a, const StepList &L, int gq) {
+    step++, left = max(left - 1, 0);
+    if (left > 0 && (step == end || step == block + kBlock)) {
+      seq = next_seq, step = block = next_step, end = next_end, pg_lo = next_lo, pages = next_pages, ids = next_ids;
+      after(a, L, gq, left - (end - step));
+    }
+  }
+};
+
+// What became of a warp's run: up to two parts that are not a whole unit.
+struct RunSlot {
+  int seq, begins, ends;  // -1: none
+};
+
+// Steps [at, to) of kv head kvh's list, by one warp.  Units that lie inside
+// are written out, parts of others go to part[0] and part[1].
+template <int D, int NT>
+Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int at, int to, uint8_t *ring,
+                        float *part_base, RunSlot *slot) {
+  using Cfg = AttendCfg<D, NT>;
+  constexpr int G = Cfg::G, R = Cfg::R, BLK = Cfg::BLK, NP = Cfg::NP, ST = Cfg::ST, MT = D / 16;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, j = g % G, gq = a.n_heads / a.c.n_kv;
+  if (lane < 2) slot[lane].seq = -1;
+  if (at >= to) return;
+  int seq;
+  {
+    int lo = 0, hi = L.n;  // the last sequence whose steps begin at or before `at`: it has some
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (L.pre[mid] <= at)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    seq = lo;
+  }
+
+  // bf16 queries of a sequence's unit: column g, dims 32 j + 8 t .. + 7
+  auto load_q = [&](int s, uint32_t (&x)[NT][4]) {
+    const SeqRows sq = L.seq[s];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int r = nt * (8 / G) + g / G, flat = min(row0 + r, total - 1);  // a row past the end repeats the last one
-      const int tok = flat / gq, head = kvh * gq + flat - tok * gq;
-      lim[nt] = pos0 + tok;
-      low[nt] = a.window > 0 ? lim[nt] - a.window + 1 : 0;
-      const uint16_t *qp = a.q + (size_t)(t0 + tok) * a.ldq + (size_t)head * D + 32 * j + 8 * t;
-      float v[8];
+      const int flat = min(L.row0 + (nt * 8 + g) / G, sq.total - 1);  // a row past the end repeats the last one
+      const int tok = token_of(flat, gq), head = kvh * gq + flat - tok * gq;
+      const uint16_t *qp = a.q + (size_t)(sq.t0 + tok) * a.ldq + (size_t)head * D + 32 * j + 8 * t;
       if (a.vec) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(qp);
-        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[2 * i] = bf2f(x[i] & 0xffffu), v[2 * i + 1] = bf2f(x[i] >> 16);
+        const uint4 w = *reinterpret_cast<const uint4 *>(qp);
+        x[nt][0] = w.x, x[nt][1] = w.y, x[nt][2] = w.z, x[nt][3] = w.w;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = bf2f(qp[i]);
+        for (int i = 0; i < 4; i++) x[nt][i] = qp[2 * i] | (uint32_t)qp[2 * i + 1] << 16;
       }
+    }
+  };
+  uint32_t raw_q[NT][4];  // of the next unit
+  load_q(seq, raw_q);
+
+  // ---- ring ----
+  PageCursor<R> cur;
+  cur.start(a, L, gq, seq, at, to);
+  uint32_t has = 0;  // whether a page is there, the newest step in the low bits
+  int put = 0;       // the stage of the next copies
+  const uint8_t *pool = a.c.pool + (size_t)kvh * BLK + 16 * lane;
+  auto copies = [&] {
+    has <<= NP;
+    if (cur.left > 0) {
+      uint8_t *dst = ring + put * (NP * BLK) + 16 * lane;
+#pragma unroll
+      for (int k = 0; k < NP; k++) {
+        const int id = __shfl_sync(0xffffffffu, cur.ids, (cur.step - cur.block) * NP + k);
+        if (id >= 0 && id < a.c.num_pages) {
+          has |= 1u << k;
+          const uint8_t *src = pool + (size_t)id * a.c.n_kv * BLK;
+#pragma unroll
+          for (int i = 0; i < (BLK / 16 + 31) / 32; i++)
+            if (BLK % 512 == 0 || lane + 32 * i < BLK / 16) cp_async16(dst + k * BLK + 512 * i, src + 512 * i, 16);
+        }
+      }
+      put = put + 1 == ST ? 0 : put + 1;
+    }
+    cp_async_commit();
+  };
+  copies();
+  cur.after(a, L, gq, cur.left - (cur.end - cur.step));
+  cur.advance(a, L, gq);
+#pragma unroll
+  for (int i = 1; i < ST - 1; i++) {
+    copies();
+    cur.advance(a, L, gq);
+  }
+  int get = 0, parts = 0;
+  while (at < to) {
+    const SeqRows sq = L.seq[seq];
+    const Unit u = unit_of<R>(sq, L.row0, gq, a.window);
+    const int steps = L.pre[seq + 1] - L.pre[seq], i0 = at - L.pre[seq], i1 = min(steps, i0 + (to - at));
+    const int pos_lo = u.pos_lo, pos_hi = u.pos_hi;
+
+    // ---- queries ----
+    uint32_t qb[NT][G][2][2];  // zeros outside group j
+    float qs[NT][2], sc[NT];   // accumulator order: of columns 2 t and 2 t + 1, of their row
+    int lim[NT], low[NT];      // the keys that row sees
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        v[2 * i] = bf2f(raw_q[nt][i] & 0xffffu), v[2 * i + 1] = __uint_as_float(raw_q[nt][i] & 0xffff0000u);
       float top = 0.f, sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[i])), sum += v[i];
@@ -513,161 +657,151 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv4_attend(const __grid_c
       for (int o = 1; o < 4 * G; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       sum += __shfl_xor_sync(0xffffffffu, sum, 1);
       sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      const float f = to_2p14(top);
+      // a negative scale turns the queries and a scale of zero clears them, so
+      // that below sc > 0 and the largest x is the largest score
+      const float f = a.scale == 0.f ? 0.f : a.scale < 0.f ? -to_2p14(top) : to_2p14(top);
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] *= f;
       // dims 0, 1 meet digits n 2^-24, dims 2, 3 meet 16 n 2^-24
-      qa[nt][0][0] = pack_f16x2(v[0], v[1]);
-      qa[nt][0][1] = pack_f16x2(v[2] * 0.0625f, v[3] * 0.0625f);
-      qa[nt][1][0] = pack_f16x2(v[4], v[5]);
-      qa[nt][1][1] = pack_f16x2(v[6] * 0.0625f, v[7] * 0.0625f);
-      qs[nt] = sum * f * 0x1p-24f;
-      sc[nt] = a.scale * 0x1p24f / f;
+      const uint32_t q4[4] = {pack_f16x2(v[0], v[1]), pack_f16x2(v[2] * 0.0625f, v[3] * 0.0625f), pack_f16x2(v[4], v[5]),
+                              pack_f16x2(v[6] * 0.0625f, v[7] * 0.0625f)};
+#pragma unroll
+      for (int q = 0; q < G; q++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) qb[nt][q][i >> 1][i & 1] = q == j ? q4[i] : 0u;
+      sum *= f * 0x1p-24f;
+      qs[nt][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+      qs[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      sc[nt] = __shfl_sync(0xffffffffu, a.scale == 0.f ? 1.f : a.scale * 0x1p24f / f, 8 * t);
+      lim[nt] = sq.pos0 + token_of(min(u.row0 + (nt * 8 + 2 * t) / G, sq.total - 1), gq);
+      low[nt] = a.window > 0 ? lim[nt] - a.window + 1 : 0;
+    }
+    int next = seq;  // the unit after this one, its queries on their way
+    if (i1 - i0 < to - at) {
+      do next++;
+      while (L.pre[next + 1] == L.pre[next]);
+      load_q(next, raw_q);
     }
 
-    float m[NT], l[NT], zac[NT], acc[NT][MT][4];
+    // p = 2^(x sc - mu), mu = m sc - lv: m the largest x = score / sc so far,
+    // lv the power of two that p carries
+    float m[NT], mu[NT], l[NT], zac[NT][2], acc[NT][MT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       m[nt] = -INFINITY;
-      l[nt] = zac[nt] = 0.f;
+      mu[nt] = 0.f;
+      l[nt] = zac[nt][0] = zac[nt][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; i++) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
     }
-    float vf = 1.f, vcap = 0.f;  // factor of the value scales, and the largest scale it is good for
+    float lv = 0.f, vcap = 0.f;  // and the largest value scale that it is good for
 
-    // ---- ring ----
-    int ids = -1;           // pages of the next 32 / NP steps, by lane
-    uint32_t has = 0;       // whether a page is there, the newest step in the low bits
-    auto issue = [&](int it) {
-      if (it < n_it) {
-        if (it % (32 / NP) == 0) {
-          const int p = p_beg + ((it + lane / NP) * W + warp) * NP + lane % NP;
-          ids = p < p_end ? page_of(a.c, a.b, s, p) : -1;
-        }
-#pragma unroll
-        for (int k = 0; k < NP; k++) {
-          const int id = __shfl_sync(0xffffffffu, ids, (it % (32 / NP)) * NP + k);
-          has = has << 1 | (id >= 0);
-          if (id >= 0) {
-            const uint8_t *src = a.c.pool + ((size_t)id * a.c.n_kv + kvh) * BLK;
-            uint8_t *dst = ring + ((it % ST) * NP + k) * BLK;
-#pragma unroll
-            for (int i = 0; i < (BLK / 16 + 31) / 32; i++)
-              if (BLK % 512 == 0 || lane + 32 * i < BLK / 16)
-                cp_async16(dst + 16 * (lane + 32 * i), src + 16 * (lane + 32 * i), 16);
-          }
-        }
-      } else {
-        has <<= NP;
-      }
-      cp_async_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < ST - 1; i++) issue(i);
-    for (int it = 0; it < n_it; it++) {
-      issue(it + ST - 1);
+    for (int it = i0; it < i1; it++) {
+      copies();
+      cur.advance(a, L, gq);
       cp_async_wait<ST - 1>();
       __syncwarp();
-      const int p0 = p_beg + (it * W + warp) * NP;
-      const uint8_t *blk0 = ring + (it % ST) * NP * BLK;
-      const uint32_t here = has >> ((ST - 1) * NP);  // bit NP - 1 - k: page k of this step
-      // ---- scores of NP pages: y[nt][4 k + i], keys 2t, 2t+1, 2t+8, 2t+9 of page k ----
-      float y[NT][4 * NP], vs[4 * NP], vz[4 * NP];
+      const int p0 = u.pg_lo + it * NP;
+      const uint8_t *blk0 = ring + get * (NP * BLK);
+      get = get + 1 == ST ? 0 : get + 1;
+      const uint32_t here = has >> ((ST - 1) * NP);  // bit k: page k of this step
+      // ---- digits of q . k, then x[nt][k][h]: key g + 8 h of page k ----
+      float x[NT][NP][2];
+      uint32_t vz[NP][2][2];  // value scale and zero of key g + 8 h, groups of columns 2 t and 2 t + 1
 #pragma unroll
       for (int k = 0; k < NP; k++) {
         const uint8_t *blk = blk0 + k * BLK;
-        float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t w0[G], w1[G];
-        if (G == 4) {
-          const uint4 u = *reinterpret_cast<const uint4 *>(blk + g * (D / 2) + 4 * G * t);
-          const uint4 x = *reinterpret_cast<const uint4 *>(blk + (g + 8) * (D / 2) + 4 * G * t);
-          w0[0] = u.x, w0[1] = u.y, w0[G - 2] = u.z, w0[G - 1] = u.w;
-          w1[0] = x.x, w1[1] = x.y, w1[G - 2] = x.z, w1[G - 1] = x.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2 *>(blk + g * (D / 2) + 4 * G * t);
-          const uint2 x = *reinterpret_cast<const uint2 *>(blk + (g + 8) * (D / 2) + 4 * G * t);
-          w0[0] = u.x, w0[1] = u.y, w1[0] = x.x, w1[1] = x.y;
-        }
+        uint32_t kw[2][G];
 #pragma unroll
-        for (int q = 0; q < G; q++) {
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            const uint32_t a0 = q == j ? qa[0][h][0] : 0u, a2 = q == j ? qa[0][h][1] : 0u;
-            const uint32_t a1 = NT > 1 && q == j ? qa[NT - 1][h][0] : 0u, a3 = NT > 1 && q == j ? qa[NT - 1][h][1] : 0u;
-            const uint32_t x0 = w0[q] >> 8 * h, x1 = w1[q] >> 8 * h;
-            mma_f16(c0, a0, a1, a2, a3, x0 & 0x000f000fu, x0 & 0x00f000f0u);
-            mma_f16(c1, a0, a1, a2, a3, x1 & 0x000f000fu, x1 & 0x00f000f0u);
+        for (int h = 0; h < 2; h++) {
+          if (G == 4) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(blk + 16 * lane + 512 * h);
+            kw[h][0] = w.x, kw[h][1] = w.y, kw[h][G - 2] = w.z, kw[h][G - 1] = w.w;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2 *>(blk + 8 * lane + 256 * h);
+            kw[h][0] = w.x, kw[h][1] = w.y;
           }
         }
-        const uint4 *sp = reinterpret_cast<const uint4 *>(blk + 16 * D + 32 * (4 * j + t));
-        const uint4 u0 = sp[0], u1 = sp[1];
-        const uint32_t kw[4] = {u0.x, u0.z, u1.x, u1.z}, vw[4] = {u0.y, u0.w, u1.y, u1.w};
+        float c[NT][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float ks = bf2f(kw[i] & 0xffffu), kz = bf2f(kw[i] >> 16);
-          vs[4 * k + i] = bf2f(vw[i] & 0xffffu);
-          vz[4 * k + i] = bf2f(vw[i] >> 16);
+        for (int nt = 0; nt < NT; nt++) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+#pragma unroll
+        for (int q = 0; q < G; q++)
+#pragma unroll
+          for (int b = 0; b < 2; b++) {
+            const uint32_t y0 = kw[0][q] >> 8 * b, y1 = kw[1][q] >> 8 * b;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+              mma_f16(c[nt], y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, qb[nt][q][b][0],
+                      qb[nt][q][b][1]);
+          }
+        const uint8_t *kp = blk + 16 * D + 128 * (2 * t % G) + 32 * (g >> 1) + 8 * (g & 1);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint2 s0 = *reinterpret_cast<const uint2 *>(kp + 16 * h);
+          const uint2 s1 = *reinterpret_cast<const uint2 *>(kp + 16 * h + 128);
+          vz[k][h][0] = s0.y;
+          vz[k][h][1] = s1.y;
 #pragma unroll
           for (int nt = 0; nt < NT; nt++) {
-            const float c = i < 2 ? c0[2 * nt + i] : c1[2 * nt + i - 2];
-            float x = fmaf(ks, c, kz * qs[nt]);
-#pragma unroll
-            for (int o = 4; o < 4 * G; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            y[nt][4 * k + i] = x * sc[nt];
+            float y = __uint_as_float(s0.x & 0xffff0000u) * qs[nt][0];
+            y = fmaf(__uint_as_float(s1.x & 0xffff0000u), qs[nt][1], y);
+            y = fmaf(bf2f(s0.x & 0xffffu), c[nt][2 * h], y);
+            y = fmaf(bf2f(s1.x & 0xffffu), c[nt][2 * h + 1], y);
+            if (G == 4) y += __shfl_xor_sync(0xffffffffu, y, 1);
+            x[nt][k][h] = y;
           }
         }
         // keys that a row may not see, and pages that are not there: whatever
         // the slot holds, scales that are no numbers included, does not count
-        const bool there = here >> (NP - 1 - k) & 1;
+        const bool there = here >> k & 1;
         const int key0 = (p0 + k) * 16;
         if (!there || key0 + 15 > pos_lo || (a.window > 0 && key0 < pos_hi - a.window + 1)) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int key = key0 + 2 * t + (i & 1) + 8 * (i >> 1);
+          for (int h = 0; h < 2; h++) {
+            const int key = key0 + g + 8 * h;
             bool any = false;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
               const bool seen = there && key <= lim[nt] && key >= low[nt];
-              if (!seen) y[nt][4 * k + i] = -INFINITY;
+              if (!seen) x[nt][k][h] = -INFINITY;
               any |= seen;
             }
-            if (!any) vs[4 * k + i] = vz[4 * k + i] = 0.f;
+            if (!any) vz[k][h][0] = vz[k][h][1] = 0u;
           }
         }
       }
-      // ---- running maximum, factor of the value scales ----
-      float top = 0.f, cr[NT];
+      // ---- running maximum, largest value scale ----
+      float top = 0.f, mx[NT];
 #pragma unroll
-      for (int i = 0; i < 4 * NP; i++) top = fmaxf(top, vs[i]);
+      for (int i = 0; i < 4 * NP; i++) top = fmaxf(top, bf2f(vz[i >> 2][i >> 1 & 1][i & 1] & 0xffffu));
       bool moved = top > vcap;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        float mx = y[nt][0];
+        mx[nt] = m[nt];
 #pragma unroll
-        for (int i = 1; i < 4 * NP; i++) mx = fmaxf(mx, y[nt][i]);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[nt], mx);
-        cr[nt] = m[nt] == mn ? 1.f : exp2f(m[nt] - mn);
-        moved |= m[nt] != mn;
-        m[nt] = mn;
+        for (int i = 0; i < 2 * NP; i++) mx[nt] = fmaxf(mx[nt], x[nt][i >> 1][i & 1]);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mx[nt] = fmaxf(mx[nt], __shfl_xor_sync(0xffffffffu, mx[nt], o));
+        moved |= mx[nt] != m[nt];
       }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float fv = 1.f;
-        if (top > vcap) {
-          const float nf = to_2p14(top);
-          fv = nf * (1.f / vf);
-          vf = nf;
-          vcap = 0x1p15f / nf;
+        if (top > vcap) {  // p s < 2^15
+          const int e = max(exponent(top), -86);
+          lv = (float)(14 - e);
+          vcap = __uint_as_float((uint32_t)(min(e + 1, 127) + 127) << 23);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          l[nt] *= cr[nt];
-          zac[nt] *= cr[nt];
-          // columns 2t and 2t + 1 belong to one row, that of lanes 4 (2t) ..
-          const float f = __shfl_sync(0xffffffffu, cr[nt], 8 * t) * fv;
+          const float to = (mx[nt] == -INFINITY ? 0.f : mx[nt] * sc[nt]) - lv;
+          const float f = m[nt] == -INFINITY ? 0.f : ex2(mu[nt] - to);  // nothing summed yet, or as much as p shrinks
+          m[nt] = mx[nt];
+          mu[nt] = to;
+          l[nt] *= f;
+          zac[nt][0] *= f;
+          zac[nt][1] *= f;
 #pragma unroll
           for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -678,106 +812,293 @@ __global__ void __launch_bounds__(kAttendWarps * 32) k_kv4_attend(const __grid_c
 #pragma unroll
       for (int k = 0; k < NP; k++) {
         const uint8_t *blk = blk0 + k * BLK;
-        uint32_t b0[NT], b1[NT];
+        uint32_t b[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          const float mu = m[nt] == -INFINITY ? 0.f : m[nt];
-          float w[4];
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float yi = y[nt][4 * k + i], p = exp2f(yi - mu);
-            const bool out = yi == -INFINITY;  // p is 0: its value may be anything
+          for (int h = 0; h < 2; h++) {
+            const float p = ex2(fmaf(x[nt][k][h], sc[nt], -mu[nt]));
             l[nt] += p;
-            zac[nt] += out ? 0.f : p * vz[4 * k + i];
-            w[i] = out ? 0.f : p * (vs[4 * k + i] * vf);
+            // a key that only another row of this lane sees: its value may be anything
+            const bool out = NT > 1 && x[nt][k][h] == -INFINITY;
+            float w[2];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              w[e] = out ? 0.f : p * bf2f(vz[k][h][e] & 0xffffu);
+              zac[nt][e] = out ? zac[nt][e] : fmaf(p, __uint_as_float(vz[k][h][e] & 0xffff0000u), zac[nt][e]);
+            }
+            b[nt][h] = transpose8(pack_f16x2(w[0], w[1]));
           }
-          b0[nt] = pack_f16x2(w[0], w[1]);
-          b1[nt] = pack_f16x2(w[2], w[3]);
-        }
 #pragma unroll
         for (int M = 0; M < D / 64; M++) {
-          const uint4 u = *reinterpret_cast<const uint4 *>(blk + 8 * D + 512 * M + 16 * lane);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+          const uint4 w = *reinterpret_cast<const uint4 *>(blk + 8 * D + 512 * M + 16 * lane);
+          const uint32_t v4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const uint32_t x = w[i], x8 = x >> 8;
+            const uint32_t v = v4[i], v8 = v >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
-              mma_f16(acc[nt][4 * M + i], x & 0x000f000fu, x & 0x00f000f0u, x8 & 0x000f000fu, x8 & 0x00f000f0u, b0[nt],
-                      b1[nt]);
+              mma_f16(acc[nt][4 * M + i], v & 0x000f000fu, v & 0x00f000f0u, v8 & 0x000f000fu, v8 & 0x00f000f0u, b[nt][0],
+                      b[nt][1]);
           }
         }
       }
       __syncwarp();  // every lane is done with the stage that the next copies write
     }
-    cp_async_wait<0>();
-    __syncthreads();  // the ring is free: it takes the warps' parts
-    float *s_o = reinterpret_cast<float *>(ring_all);  // [W][R][D]
-    const float back = 1.f / vf;  // digits were n 2^-24 and 16 n 2^-24
+    float *part = part_base + parts * Cfg::PART;
+    float *p_m = part, *p_l = p_m + R, *p_z = p_l + R, *p_o = p_z + R * G;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      float lt = l[nt], zt = zac[nt];
-      lt += __shfl_xor_sync(0xffffffffu, lt, 1);
-      lt += __shfl_xor_sync(0xffffffffu, lt, 2);
-      zt += __shfl_xor_sync(0xffffffffu, zt, 1);
-      zt += __shfl_xor_sync(0xffffffffu, zt, 2);
-      const int rg = nt * (8 / G) + g / G, rt = nt * (8 / G) + 2 * t / G;
-      if (t == 0) {
-        s_z[warp][rg][j] = zt;
-        if (j == 0) {
-          s_m[warp][rg] = m[nt];
-          s_l[warp][rg] = lt;
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        l[nt] += __shfl_xor_sync(0xffffffffu, l[nt], o);
+        zac[nt][0] += __shfl_xor_sync(0xffffffffu, zac[nt][0], o);
+        zac[nt][1] += __shfl_xor_sync(0xffffffffu, zac[nt][1], o);
+      }
+      const int r = (nt * 8 + 2 * t) / G, ja = 2 * t % G;
+      if (g == 0) {
+        p_z[r * G + ja] = zac[nt][0];
+        p_z[r * G + ja + 1] = zac[nt][1];
+        if (ja == 0) {
+          p_m[r] = m[nt] == -INFINITY ? m[nt] : mu[nt];
+          p_l[r] = l[nt];
         }
       }
-      float *o = s_o + ((size_t)warp * R + rt) * D;
 #pragma unroll
       for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int e = 0; e < 2; e++)
-          if ((2 * t + e) % G == i / 2) {
-            o[16 * i + g] = acc[nt][i][e] * 0x1p24f * back;
-            o[16 * i + 8 + g] = acc[nt][i][2 + e] * 0x1p20f * back;
+          if (ja + e == i / 2) {  // digits were n 2^-24 and 16 n 2^-24
+            p_o[r * D + 16 * i + g] = acc[nt][i][e] * 0x1p24f;
+            p_o[r * D + 16 * i + 8 + g] = acc[nt][i][2 + e] * 0x1p20f;
           }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < R * D; i += W * 32) {
-      const int r = i / D, d = i - r * D;
-      float M = -INFINITY, L = 0.f, o = 0.f;
+    __syncwarp();
+    if (i0 == 0 && i1 == steps) {
+      for (int e = lane; e < u.nrow * D; e += 32)
+        store_out<D>(a, sq.t0, u.row0 + e / D, kvh, e % D, p_l[e / D], p_o[e] + p_z[e / 32]);
+      __syncwarp();
+    } else {
+      if (lane == 0) slot[parts] = RunSlot{seq, i0 == 0, i1 == steps};
+      parts++;
+    }
+    at += i1 - i0;
+    seq = next;
+  }
+  cp_async_wait<0>();
+  __syncwarp();
+}
+
+// What a CTA says of the unit that begins in its run and goes on in others:
+// n CTAs have parts of it (0: there is none), and where its rows are.
+struct PartNote {
+  int n, t0, row0, nrow;
+};
+// Workspace: notes [CTAs], parts [CTAs][2][PART]; CTA c works on kv head
+// c % n_kv, and c + n_kv goes on where it ends.  Part 0 belongs to a unit that
+// began in an earlier CTA, part 1 to one that begins here and goes on.
+
+// The steps of list L of kv head kvh that CTA ci of `ctas` has, and what is left of them.
+template <int D, int NT>
+Q3T_DEV void attend_list(const Kv4AttendArgs &a, const StepList &L, int kvh, int ci, int ctas, uint8_t *ring_all,
+                         float *s_part, RunSlot (*slot)[2], PartNote *note, float *parts) {
+  using Cfg = AttendCfg<D, NT>;
+  constexpr int R = Cfg::R, W = Cfg::W, PART = Cfg::PART;
+  const int warp = threadIdx.x >> 5;
+  const int64_t T = L.pre[L.n], runs = (int64_t)ctas * W, run = (int64_t)ci * W + warp;
+  attend_run<D, NT>(a, L, kvh, (int)(T * run / runs), (int)(T * (run + 1) / runs), ring_all + warp * Cfg::RING,
+                    s_part + warp * 2 * PART, slot[warp]);
+  __syncthreads();
+  PartNote left{0, 0, 0, 0};
+  // units that more than one run of this CTA, or of others, has parts of
+  int owner[2 * W];
 #pragma unroll
-      for (int w = 0; w < W; w++) M = fmaxf(M, s_m[w][r]);
+  for (int k = 0; k < 2 * W; k++) owner[k] = slot[k >> 1][k & 1].seq;
+  uint32_t left_to_join = 0;
 #pragma unroll
-      for (int w = 0; w < W; w++) {
-        const float f = part_weight(s_m[w][r], s_l[w][r], M);
-        L += f * s_l[w][r];
-        o += f * (s_o[((size_t)w * R + r) * D + d] + s_z[w][r][d / 32]);
+  for (int k = 0; k < 2 * W; k++) left_to_join |= (owner[k] >= 0 ? 1u : 0u) << k;
+  while (left_to_join) {
+    const int first = __ffs(left_to_join) - 1;
+    const RunSlot f = slot[first >> 1][first & 1];
+    uint32_t mine = 0;  // its parts: the next ones of the same sequence
+#pragma unroll
+    for (int k = 0; k < 2 * W; k++) mine |= (owner[k] == f.seq ? 1u : 0u) << k;
+    left_to_join &= ~mine;
+    const int last = 31 - __clz(mine), ends = slot[last >> 1][last & 1].ends;
+    const SeqRows sq = L.seq[f.seq];
+    const int nrow = min(R, sq.total - L.row0);
+    float *dst = parts + (f.begins ? PART : 0);
+#pragma unroll
+    for (int e0 = 0; e0 < R * D; e0 += 128) {
+      const int e = e0 + threadIdx.x, r = e / D, d = e - r * D;
+      float M = -INFINITY, l = 0.f, o = 0.f, pm[2 * W];
+#pragma unroll
+      for (int k = 0; k < 2 * W; k++) {
+        pm[k] = mine >> k & 1 ? s_part[k * PART + r] : -INFINITY;
+        M = fmaxf(M, pm[k]);
       }
-      c_o[r][d] = o;
-      if (d == 0) {
-        c_m[r] = M;
-        c_l[r] = L;
+#pragma unroll
+      for (int k = 0; k < 2 * W; k++) {
+        if (!(mine >> k & 1)) continue;
+        const float *p = s_part + k * PART;
+        const float w = part_weight(pm[k], p[R + r], M);
+        l += w * p[R + r];
+        o += w * (p[2 * R + R * Cfg::G + e] + p[2 * R + e / 32]);
+      }
+      if (f.begins && ends) {
+        if (r < nrow) store_out<D>(a, sq.t0, L.row0 + r, kvh, d, l, o);
+      } else {
+        dst[2 * R + R * Cfg::G + e] = o;  // with its zeros
+        if (d == 0) {
+          dst[r] = M;
+          dst[R + r] = l;
+        }
       }
     }
-    if (csize > 1)
-      cluster_sync();
-    else
-      __syncthreads();
-    if (rank == 0)
-      for (int i = threadIdx.x; i < nrow * D; i += W * 32) {
-        const int r = i / D, d = i - r * D, tok = (row0 + r) / gq, head = kvh * gq + (row0 + r) - tok * gq;
-        float M = c_m[r], L = c_l[r], o = c_o[r][d];
-        for (int k = 1; k < csize; k++) {
-          const float mk = ld_cluster_f1(&c_m[r], k), lk = ld_cluster_f1(&c_l[r], k), ok = ld_cluster_f1(&c_o[r][d], k);
-          const float Mn = fmaxf(M, mk), fa = part_weight(M, L, Mn), fb = part_weight(mk, lk, Mn);
-          L = fa * L + fb * lk;
-          o = fa * o + fb * ok;
-          M = Mn;
-        }
-        a.out[(size_t)(t0 + tok) * a.ldo + (size_t)head * D + d] = f2bf(L == 0.f ? 0.f : o / L);  // no keys: zeros
+    if (f.begins && !ends) {
+      const int64_t e = L.pre[f.seq + 1] - 1;  // the unit's last step, and the CTA that has it
+      int c = (int)(e * ctas / T);
+      while (c + 1 < ctas && T * (c + 1) / ctas <= e) c++;
+      left = PartNote{c - ci + 1, sq.t0, L.row0, nrow};
+    }
+  }
+  if (ctas > 1) {
+    if (threadIdx.x == 0) *note = left;
+    if (T * ci / ctas == T * (ci + 1) / ctas && threadIdx.x < R) {  // no steps: a part that weighs nothing
+      parts[threadIdx.x] = -INFINITY;
+      parts[R + threadIdx.x] = 0.f;
+    }
+  }
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) k_kv4_attend(const __grid_constant__ Kv4AttendArgs a,
+                                                                     PartNote *notes, float *parts) {
+  using Cfg = AttendCfg<D, NT>;
+  constexpr int R = Cfg::R, W = Cfg::W, PART = Cfg::PART;
+  extern __shared__ __align__(16) uint8_t ring_all[];
+  __shared__ int warp_tot[W], one_pre[2];
+  __shared__ SeqRows one_seq;
+  __shared__ RunSlot slot[W][2];
+  const int B = a.b.num_seqs, n_kv = a.c.n_kv, gq = a.n_heads / n_kv;
+  float *s_part = reinterpret_cast<float *>(ring_all + W * Cfg::RING);   // [W][2][PART]
+  SeqRows *seq = reinterpret_cast<SeqRows *>(s_part + W * 2 * PART);     // [B]
+  int *pre = reinterpret_cast<int *>(seq + B);                           // [B + 1]
+  pdl_wait();
+  pdl_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int carry = 0, more = 0;
+  for (int base = 0; base < B; base += 128) {
+    const int s = base + (int)threadIdx.x;
+    int incl = 0;
+    if (s < B) {
+      SeqRows q;
+      int n;
+      seq_rows(a.b, s, q.t0, n, q.pos0);
+      q.total = n * gq;
+      q.table_row = a.b.table_row ? a.b.table_row[s] : a.b.first + s;
+      seq[s] = q;
+      incl = unit_steps(unit_of<R>(q, 0, gq, a.window));
+      more |= q.total > R;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_tot[warp] = incl;
+    __syncthreads();
+    int before = carry;
+#pragma unroll
+    for (int k = 0; k < W; k++) {
+      if (k < warp) before += warp_tot[k];
+      carry += warp_tot[k];
+    }
+    if (s < B) pre[s + 1] = before + incl;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) pre[0] = 0;
+  more = __syncthreads_or(more);
+  attend_list<D, NT>(a, StepList{pre, seq, B, 0}, blockIdx.x % n_kv, blockIdx.x / n_kv, gridDim.x / n_kv, ring_all, s_part,
+                     slot, notes + blockIdx.x, parts + (size_t)blockIdx.x * 2 * PART);
+  // rows beyond the first R of a sequence (more than the caller announced): a CTA to each unit
+  for (int item = blockIdx.x; more; item += gridDim.x) {
+    int s, i;
+    __syncthreads();
+    if (!find_item(B, item, [&](int q) { return max(0, (seq[q].total + R - 1) / R - 1) * n_kv; }, s, i)) break;
+    const int row0 = (i / n_kv + 1) * R;
+    if (threadIdx.x == 0) {
+      one_seq = seq[s];
+      one_pre[0] = 0;
+      one_pre[1] = unit_steps(unit_of<R>(one_seq, row0, gq, a.window));
+    }
+    __syncthreads();
+    attend_list<D, NT>(a, StepList{one_pre, &one_seq, 1, row0}, i % n_kv, 0, 1, ring_all, s_part, slot, nullptr, nullptr);
+  }
+}
+
+// Joins the units whose parts several CTAs left: CTA b takes the one that
+// begins in CTA b of the attend launch, its warps a part each in turn, so that
+// the loads of a few parts are one latency and those of many are spread.
+template <int D, int NT>
+__global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4AttendArgs a, const PartNote *notes,
+                                                     const float *parts) {
+  using Cfg = AttendCfg<D, NT>;
+  constexpr int R = Cfg::R, G = Cfg::G, PART = Cfg::PART, PER = R * D / 32, WARPS = 8;
+  __shared__ float s_m[WARPS][R], s_l[WARPS][R], s_o[WARPS][R * D];
+  pdl_wait();
+  pdl_launch();
+  const int n_kv = a.c.n_kv, b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PartNote f = notes[b];
+  if (f.n == 0) return;
+  // lane's elements are lane + 32 i of row (32 i) / D
+  float m[R], l[R], o[PER];
+#pragma unroll
+  for (int r = 0; r < R; r++) m[r] = -INFINITY, l[r] = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; i++) o[i] = 0.f;
+  constexpr int BATCH = 4;  // parts whose loads are in flight together
+  for (int k0 = warp; k0 < f.n; k0 += WARPS * BATCH) {
+    float pm[BATCH][R], pl[BATCH][R], po[BATCH][PER];
+#pragma unroll
+    for (int x = 0; x < BATCH; x++) {
+      const int k = k0 + x * WARPS;
+      const float *p = parts + ((size_t)(b + k * n_kv) * 2 + (k == 0 ? 1 : 0)) * PART;
+#pragma unroll
+      for (int r = 0; r < R; r++) pm[x][r] = k < f.n ? p[r] : -INFINITY, pl[x][r] = k < f.n ? p[R + r] : 0.f;
+#pragma unroll
+      for (int i = 0; i < PER; i++) po[x][i] = k < f.n ? p[2 * R + R * G + lane + 32 * i] : 0.f;
+    }
+#pragma unroll
+    for (int x = 0; x < BATCH; x++)
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float M = fmaxf(m[r], pm[x][r]), f0 = part_weight(m[r], l[r], M), f1 = part_weight(pm[x][r], pl[x][r], M);
+        m[r] = M;
+        l[r] = f0 * l[r] + f1 * pl[x][r];
+#pragma unroll
+        for (int i = r * (D / 32); i < (r + 1) * (D / 32); i++)  // what weighs nothing may be anything
+          o[i] = (f0 == 0.f ? 0.f : f0 * o[i]) + (f1 == 0.f ? 0.f : f1 * po[x][i]);
       }
-    if (csize > 1)
-      cluster_sync();  // a CTA's part stays until rank 0 has read it
-    else
-      __syncthreads();
+  }
+  if (lane == 0)
+#pragma unroll
+    for (int r = 0; r < R; r++) s_m[warp][r] = m[r], s_l[warp][r] = l[r];
+#pragma unroll
+  for (int i = 0; i < PER; i++) s_o[warp][lane + 32 * i] = o[i];
+  __syncthreads();
+  for (int e = threadIdx.x; e < f.nrow * D; e += 256) {
+    const int r = e / D, d = e - r * D;
+    float M = -INFINITY, L = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) M = fmaxf(M, s_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+      const float f1 = part_weight(s_m[w][r], s_l[w][r], M);
+      L += f1 * s_l[w][r];
+      x += f1 * s_o[w][e];
+    }
+    store_out<D>(a, f.t0, f.row0 + r, b % n_kv, d, L, x);
   }
 }
 
@@ -856,27 +1177,33 @@ cudaError_t read_launch(const Kv4ReadArgs &a, int windows, cudaStream_t st, bool
 }
 
 template <int D, int NT>
-cudaError_t attend_launch(const Kv4AttendArgs &a, int max_q, int max_kv, cudaStream_t st, bool pdl) {
+cudaError_t attend_launch(const Kv4AttendArgs &a, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st, bool pdl) {
   using Cfg = AttendCfg<D, NT>;
   static std::atomic<uint64_t> done{0};
+  static std::atomic<int> resident{0};  // CTAs that one device holds at once
   cudaError_t e = once_per_device(done, [] {
     cudaError_t r = cudaFuncSetAttribute(k_kv4_attend<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)Cfg::kSmem);
-    if (r != cudaSuccess) return r;
-    return cudaFuncSetAttribute(k_kv4_attend<D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+                                         (int)Cfg::smem(Cfg::MAXSEQ));
+    int dev = 0, sms = 0, occ = 0;
+    if (r == cudaSuccess) r = cudaGetDevice(&dev);
+    if (r == cudaSuccess) r = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (r == cudaSuccess)
+      r = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k_kv4_attend<D, NT>, Cfg::W * 32, Cfg::smem(256));
+    if (r == cudaSuccess) resident.store(sms * std::max(occ, 1));
+    return r;
   });
   if (e != cudaSuccess) return e;
-  const int gq = a.n_heads / a.c.n_kv;
-  const bool direct = max_q > 0 && (int64_t)max_q * gq <= Cfg::R;
-  int64_t tiles = direct ? a.b.num_seqs : ((int64_t)a.b.num_tokens * gq + Cfg::R - 1) / Cfg::R + a.b.num_seqs;
-  const int64_t units = tiles * a.c.n_kv;
-  // CTAs of a unit: enough to occupy the SMs, while each warp still gets two steps of pages
-  const int pages = (a.window > 0 && (max_kv <= 0 || a.window < max_kv) ? a.window + 31 : max_kv > 0 ? max_kv : 4096) / 16 + 1;
-  int c = 1;
-  while (c < 16 && units * c < 296 && c * kAttendWarps * Cfg::NP * 2 < pages) c *= 2;
-  if (units * c > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return launch(k_kv4_attend<D, NT>, dim3((unsigned)(units * c)), kAttendWarps * 32, Cfg::kSmem, c, pdl, st, a, c,
-                direct ? 1 : 0);
+  // one grid that fills the GPU once, fewer where a warp would have less than one step
+  const int64_t pages = (a.window > 0 && (max_kv <= 0 || a.window < max_kv) ? a.window + 31 : max_kv > 0 ? max_kv : 1 << 20) / 16 + 1;
+  const int64_t steps = (pages + 1) / 2 * a.b.num_seqs;
+  const int64_t fit = ws_bytes / (int64_t)(sizeof(PartNote) + 2 * Cfg::PART * 4);
+  const int64_t most = std::min<int64_t>(std::min<int64_t>(resident.load(), fit) / a.c.n_kv, (steps + Cfg::W - 1) / Cfg::W);
+  const int ctas = (int)std::max<int64_t>(most, 1), grid = ctas * a.c.n_kv;  // of a kv head, of all
+  PartNote *notes = (PartNote *)ws;
+  float *parts = (float *)(notes + grid);
+  e = launch(k_kv4_attend<D, NT>, dim3(grid), Cfg::W * 32, Cfg::smem(a.b.num_seqs), 1, pdl, st, a, notes, parts);
+  if (e != cudaSuccess || ctas == 1) return e;
+  return launch(k_kv4_combine<D, NT>, dim3(grid), 256, 0, 1, false, st, a, (const PartNote *)notes, (const float *)parts);
 }
 
 }  // namespace
@@ -902,12 +1229,28 @@ cudaError_t kv4_read(const Kv4ReadArgs &a0, cudaStream_t st, bool pdl) {
   return a.c.head_dim == 128 ? read_launch<128>(a, windows, st, pdl) : read_launch<64>(a, windows, st, pdl);
 }
 
-cudaError_t kv4_attend(const Kv4AttendArgs &a, int max_q, int max_kv, cudaStream_t st, bool pdl) {
-  if (a.b.num_tokens <= 0 || a.b.num_seqs <= 0) return cudaSuccess;
-  const int rows = (max_q > 0 ? max_q : 2) * (a.n_heads / a.c.n_kv);  // rows of a kv head: one column tile, or two
-  if (a.c.head_dim == 128)
-    return rows <= 2 ? attend_launch<128, 1>(a, max_q, max_kv, st, pdl) : attend_launch<128, 2>(a, max_q, max_kv, st, pdl);
-  return rows <= 4 ? attend_launch<64, 1>(a, max_q, max_kv, st, pdl) : attend_launch<64, 2>(a, max_q, max_kv, st, pdl);
+cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st,
+                       bool pdl) {
+  if (a0.b.num_tokens <= 0 || a0.b.num_seqs <= 0) return cudaSuccess;
+  const int rows = (max_q > 0 ? max_q : 2) * (a0.n_heads / a0.c.n_kv);  // rows of a kv head: one column tile, or two
+  Kv4AttendArgs a = a0;
+  constexpr int kSeqs = AttendCfg<128, 1>::MAXSEQ;
+  for (int s0 = 0; s0 < a0.b.num_seqs; s0 += kSeqs) {  // sequences of one launch
+    a.b.num_seqs = std::min(kSeqs, a0.b.num_seqs - s0);
+    a.b.q_start = a0.b.q_start + s0;
+    a.b.kv_len = a0.b.kv_len + s0;
+    if (a0.b.table_row) a.b.table_row = a0.b.table_row + s0;
+    a.b.first = a0.b.first + s0;
+    cudaError_t e;
+    if (a.c.head_dim == 128)
+      e = rows <= 2 ? attend_launch<128, 1>(a, max_kv, ws, ws_bytes, st, pdl)
+                    : attend_launch<128, 2>(a, max_kv, ws, ws_bytes, st, pdl);
+    else
+      e = rows <= 4 ? attend_launch<64, 1>(a, max_kv, ws, ws_bytes, st, pdl)
+                    : attend_launch<64, 2>(a, max_kv, ws, ws_bytes, st, pdl);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 }  // namespace q3t
@@ -976,7 +1319,7 @@ Kv4Batch batch_of(const char *what, const q3t_kv4_batch *b) {
   if (b->max_q_len < 0 || b->max_kv_len < 0)
     FAIL(Q3T_INVALID_INPUT, "%s: negative max_q_len or max_kv_len", what);
   if (b->num_seqs > 0 && (!b->q_start || !b->kv_len)) FAIL(Q3T_INVALID_INPUT, "%s: null q_start or kv_len", what);
-  return Kv4Batch{b->num_seqs, b->num_tokens, b->q_start, b->kv_len, b->table_row};
+  return Kv4Batch{b->num_seqs, b->num_tokens, b->q_start, b->kv_len, b->table_row, 0};
 }
 
 // Rows of `heads` heads: non-null, on an element boundary, no two overlapping.
@@ -1076,7 +1419,7 @@ extern "C" q3t_status q3t_kv4_append(const q3t_kv4_cache *cache, const q3t_kv4_b
 
 extern "C" q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, int num_heads,
                                      const uint16_t *q, int64_t q_stride, float scale, int window, uint16_t *out,
-                                     int64_t out_stride, void *stream) {
+                                     int64_t out_stride, void *workspace, int64_t workspace_bytes, void *stream) {
   const char *what = "q3t_kv4_attend";
   return guarded([&] {
     Kv4AttendArgs a{};
@@ -1090,6 +1433,8 @@ extern "C" q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_b
     if (a.b.num_seqs == 0 || a.b.num_tokens == 0) return;
     check_rows(what, "q", q, q_stride, num_heads, a.c.head_dim, 2);
     check_rows(what, "out", out, out_stride, num_heads, a.c.head_dim, 2);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < (64 << 10))
+      FAIL(Q3T_INVALID_INPUT, "%s: a workspace of 64 KiB at least on a 16-byte boundary is needed", what);
     a.n_heads = num_heads;
     a.q = q;
     a.ldq = q_stride;
@@ -1099,7 +1444,7 @@ extern "C" q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_b
     a.window = window;
     a.vec = wide(q, q_stride, 2, 8) && wide(out, out_stride, 2, 8);
     DeviceScope dev(cache->device);
-    CK(kv4_attend(a, batch->max_q_len, batch->max_kv_len, (cudaStream_t)stream, true));
+    CK(kv4_attend(a, batch->max_q_len, batch->max_kv_len, workspace, workspace_bytes, (cudaStream_t)stream, true));
   });
 }
 

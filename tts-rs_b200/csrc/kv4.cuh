@@ -27,7 +27,8 @@ struct Kv4Batch {
   int num_seqs, num_tokens;
   const int *q_start;   // [num_seqs + 1]
   const int *kv_len;    // [num_seqs]
-  const int *table_row; // [num_seqs], nullable
+  const int *table_row; // [num_seqs], nullable: then row first + s
+  int first;
 };
 
 // Rotation of the leading `rot` dims: freq[i] = radians per position / pi.
@@ -80,13 +81,17 @@ struct Kv4Step {
   Kv4AppendArgs append;
   Kv4AttendArgs attend;
   int max_q, max_kv;
+  void *ws;  // kKv4Workspace bytes
 };
 
 // max_q / max_kv: the most tokens and keys of a sequence, as the caller knows
 // them; they choose the launch shape only (0: unknown).  Launch errors are
 // returned; `pdl` lets the launch overlap the tail of the one before it.
 cudaError_t kv4_append(const Kv4AppendArgs &a, bool f32_rows, cudaStream_t st, bool pdl);
-cudaError_t kv4_attend(const Kv4AttendArgs &a, int max_q, int max_kv, cudaStream_t st, bool pdl);
+// attend needs a workspace: 64 KiB at least, kKv4Workspace for the widest launch.
+constexpr int64_t kKv4Workspace = 4 << 20;
+cudaError_t kv4_attend(const Kv4AttendArgs &a, int max_q, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st,
+                       bool pdl);
 cudaError_t kv4_read(const Kv4ReadArgs &a, cudaStream_t st, bool pdl);
 
 }  // namespace q3t

@@ -858,7 +858,7 @@ void run_phases(const Phase *ph, int n, cudaStream_t st) {
       case PH_SAMPLE: sample(p.smp, p.max_tok, st, p.has_tail ? &p.tail : nullptr); break;
       case PH_KV4_APPEND: note(kv4_append(p.kv4->append, true, st, true), "k_kv4_append"); break;
       case PH_KV4_ATTEND:
-        note(kv4_attend(p.kv4->attend, p.kv4->max_q, p.kv4->max_kv, st, true), "k_kv4_attend");
+        note(kv4_attend(p.kv4->attend, p.kv4->max_q, p.kv4->max_kv, p.kv4->ws, kKv4Workspace, st, true), "k_kv4_attend");
         break;
       default: note(cudaErrorInvalidValue, "run_phases: unknown phase"); break;
     }

@@ -256,7 +256,8 @@ def lib():
         L.q3t_kv4_append.argtypes = [C.POINTER(KV4CacheView), C.POINTER(KV4BatchView), C.POINTER(KV4Rows),
                                      C.POINTER(RopeView), C.c_void_p]
         L.q3t_kv4_attend.argtypes = [C.POINTER(KV4CacheView), C.POINTER(KV4BatchView), C.c_int, C.c_void_p,
-                                     C.c_int64, C.c_float, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]
+                                     C.c_int64, C.c_float, C.c_int, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                     C.c_void_p]
         L.q3t_kv4_read.argtypes = [C.POINTER(KV4CacheView), C.POINTER(KV4BatchView), C.c_void_p, C.c_int64,
                                    C.c_void_p, C.c_int64, C.c_void_p]
         L.q3t_abi_struct.argtypes = [C.c_char_p, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t),
@@ -866,6 +867,9 @@ class Batch:
 # 4-bit paged key/value cache on torch CUDA tensors (q3t_kv4_*).  Calls run on
 # torch's current stream of the cache's device and return without waiting.
 # ---------------------------------------------------------------------------
+KV4_WORKSPACE = 4 << 20  # Q3T_KV4_WORKSPACE
+
+
 def _bad(message):
     raise Q3TError(INVALID_INPUT, message)
 
@@ -945,7 +949,7 @@ class KV4Cache:
     def _torch(self):
         import torch
         self._bf16, self._empty, self._stream = torch.bfloat16, torch.empty, torch.cuda.current_stream
-        self._f32 = torch.float32
+        self._f32, self._u8 = torch.float32, torch.uint8
 
     def _rows(self, t, name, batch, heads, dtype):
         D = self.head_dim
@@ -1002,9 +1006,10 @@ class KV4Cache:
         heads = q.shape[1]
         qp, qs = self._rows(q, "q", batch, heads, self._bf16)
         op, os_ = self._rows(out, "out", batch, heads, self._bf16)
+        ws = self._empty(KV4_WORKSPACE, dtype=self._u8, device=self.device)  # this call's own, from torch's allocator
         check(lib().q3t_kv4_attend(self.ref, batch.ref, heads, qp, qs,
-                                   self.head_dim ** -0.5 if scale is None else scale, window, op, os_,
-                                   self._stream(self.device).cuda_stream))
+                                   self.head_dim ** -0.5 if scale is None else scale, window, op, os_, ws.data_ptr(),
+                                   KV4_WORKSPACE, self._stream(self.device).cuda_stream))
         return out
 
     def read(self, batch, k=None, v=None):
