@@ -767,6 +767,7 @@ struct ProgBuilder {
         at.ldo = QD;
         at.scale = (float)(M_LOG2E / std::sqrt(128.0));
         at.vec = 1;
+        at.err = b->d_err;
         st.max_q = max_q;
         st.max_kv = max_kv;
         st.ws = b->kv4_ws;

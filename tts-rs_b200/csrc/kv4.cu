@@ -27,6 +27,7 @@
 #include "common.cuh"
 #include "engine.h"
 #include "kv4.cuh"
+#include "umma.cuh"
 
 namespace q3t {
 
@@ -997,6 +998,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) k_kv4_attend(const __gri
       seq_rows(a.b, s, q.t0, n, q.pos0);
       q.total = n * gq;
       q.table_row = a.b.table_row ? a.b.table_row[s] : a.b.first + s;
+      if (a.big > 0 && q.total > a.big) q.total = 0;  // k_kv4_prompt has it
       seq[s] = q;
       incl = unit_steps(unit_of<R>(q, 0, gq, a.window));
       more |= q.total > R;
@@ -1099,6 +1101,546 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
       x += f1 * s_o[w][e];
     }
     store_out<D>(a, f.t0, f.row0 + r, b % n_kv, d, L, x);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Attend for many rows: a prompt or a chunk of one.  128 query rows (tokens x
+// heads of a kv head) are one tile of tcgen05 products, so a block is unpacked
+// once for many rows, to f16 in the swizzled order the tensor core reads:
+//   S = Q K^T     M 128 rows, N 64 keys, K D        (TMEM, two buffers)
+//   O += P V      M 128 rows, N D, K 64 keys        (TMEM)
+// Two such halves share every unpacked tile of keys.  Warps 0-7 are the
+// softmax (a thread to a row), 8-11 unpack K and 12-15 V (a warp to a page of
+// the tile), 16-19 issue the products, one lane to each half's S and P V (one
+// lane for all four spent its time issuing: 540 cycles for an S).  K, V and S have two buffers each, so the unpacking of a
+// tile, its S, the softmax of the one before and its P V run at once.
+//
+// f16 holds q times a power of two per row, K and V times one per page and per
+// tile (from the largest value there, 11 bits of each), and p, with V's power
+// relative to the largest so far.  A page's power of K enters with the score's
+// scale.  m, l, S and O are in 32 bits; m is moved, and O with it, only when a
+// score passes it by 2^8, which p in f16 can hold.
+//
+// What a row may not see must not touch it: K and V of keys that no row of the
+// tile sees are zeros, and a group that is no number becomes zeros too and is
+// noted, so that the rows that do see it, and no others, come out as NaN.
+// ---------------------------------------------------------------------------
+Q3T_DEV void mbar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// whether the barrier's phase `parity` is complete, after some time of waiting for it
+Q3T_DEV bool mbar_try(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// 32 TMEM lanes x 32 consecutive columns; call tmem_wait_ld() before reading r
+Q3T_DEV void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+Q3T_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+Q3T_DEV uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// Eight digits of a word as four f16 pairs n s + z: 0x6400 | n is 1024 + n,
+// 0x6400 | 16 n is 1024 + 16 n.  Taken as the subnormals they are, digits cost
+// half the instructions but leave s only 2^-24 of f16's range: a key far below
+// the largest of its page would lose its bits.
+Q3T_DEV void unpack8(uint32_t w, const uint32_t s[2], const uint32_t z[2], uint32_t out[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const uint32_t x = i ? w >> 8 : w;
+    const uint32_t lo = h2_fma((x & 0x000f000fu) | 0x64006400u, 0x3c003c00u, 0xe400e400u);  // - 1024
+    const uint32_t hi = h2_fma((x & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u);  // / 16 - 64
+    out[2 * i] = h2_fma(lo, s[i], z[i]);
+    out[2 * i + 1] = h2_fma(hi, s[i], z[i]);
+  }
+}
+Q3T_DEV uint32_t lows(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
+Q3T_DEV uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+// pairs of f32
+Q3T_DEV uint64_t f2_pack(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+Q3T_DEV void f2_split(uint64_t d, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+Q3T_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+Q3T_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+template <int D>
+struct PromptCfg {
+  static constexpr int G = D / 32, BLK = kv4_block_bytes(D), ROWS = 256, KEYS = 64, PAGES = KEYS / kKv4Page;
+  static constexpr int THREADS = 20 * 32;
+  static constexpr int QB = 128 * D * 2, KB = KEYS * D * 2, VB = D * KEYS * 2, PB = 128 * KEYS * 2;
+  static constexpr int SC = PAGES * 2 * D;  // a tile's scales and zeros of K, or of V
+  static constexpr int ST = 3, RING = 12 * D;  // blocks on their way to an unpacking warp: digits, scale entries
+  static constexpr size_t kSmem =
+      2 * QB + 2 * KB + 2 * VB + 2 * PB + 2 * SC + 2 * PAGES * ST * RING + 1024;  // from a 1024-byte boundary
+};
+
+template <int D>
+__global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const __grid_constant__ Kv4AttendArgs a, int thr) {
+  using Cfg = PromptCfg<D>;
+  constexpr int G = Cfg::G, BLK = Cfg::BLK, ROWS = Cfg::ROWS, KEYS = Cfg::KEYS, PAGES = Cfg::PAGES;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t k_full[2], v_full[2], k_freed[2], v_freed[2], s_full[2][2], s_freed[2][2], p_full[2], pv_done[2], q_full;
+  __shared__ uint32_t tmem_slot;
+  __shared__ __align__(16) float k_fac[8][PAGES];
+  __shared__ __align__(16) int v_exp[2][PAGES];
+  __shared__ uint8_t k_bad[8][KEYS], v_bad[2][KEYS];  // a key's groups that are no numbers: any of K's; of V's, by bit
+  __shared__ __align__(4) uint8_t k_says[8][PAGES], v_says[2][PAGES];  // of a page: bit 0 it is there, bit 1 such groups
+  __shared__ int dead;  // a wait gave up
+  uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t *sq = base, *sk = sq + 2 * Cfg::QB, *sv = sk + 2 * Cfg::KB, *sp = sv + 2 * Cfg::VB, *scales = sp + 2 * Cfg::PB,
+          *rings = scales + 2 * Cfg::SC;
+  pdl_wait();
+  const int n_kv = a.c.n_kv, gq = a.n_heads / n_kv, kvh = blockIdx.x % n_kv;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int s, i_rev;
+  if (!find_item(
+          a.b.num_seqs, blockIdx.x / n_kv,
+          [&](int q) {
+            int t0, n, pos0;
+            seq_rows(a.b, q, t0, n, pos0);
+            return n * gq > thr ? (n * gq + ROWS - 1) / ROWS : 0;
+          },
+          s, i_rev))
+    return;
+  int t0, n, pos0;
+  seq_rows(a.b, s, t0, n, pos0);
+  const int total = n * gq, row0 = ((total + ROWS - 1) / ROWS - 1 - i_rev) * ROWS;  // the longest tiles first
+  const int nrow = min(ROWS, total - row0);
+  const int pos_lo = pos0 + row0 / gq, pos_hi = pos0 + (row0 + nrow - 1) / gq;
+  const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0, pg_lo = key_lo >> 4;
+  // tiles of keys that the first 128 rows see, and the others; both begin at page pg_lo
+  auto tiles_to = [&](int pos) { return pos < 0 ? 0 : max(0, ((pos >> 4) + 1 - pg_lo + PAGES - 1) / PAGES); };
+  const int nt0 = tiles_to(pos0 + (row0 + min(nrow, 128) - 1) / gq), nt1 = nrow > 128 ? tiles_to(pos_hi) : 0;
+  const int n_tiles = max(nt0, nt1), n_pages = pos_hi < 0 ? 0 : max(0, (pos_hi >> 4) + 1 - pg_lo);
+
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < 2; b++) {
+      mbar_init(&k_full[b], PAGES);
+      mbar_init(&v_full[b], PAGES);
+      mbar_init(&k_freed[b], 2);
+      mbar_init(&v_freed[b], 2);
+      for (int h = 0; h < 2; h++) {
+        mbar_init(&s_full[h][b], 2);  // the scores, and what K's warps say of the tile
+        mbar_init(&s_freed[h][b], 128);
+      }
+      mbar_init(&p_full[b], 128);
+      mbar_init(&pv_done[b], 1);
+    }
+    mbar_init(&q_full, 256);
+    fence_mbar_init();
+    dead = 0;
+  }
+  if (warp == 16) tmem_alloc(&tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // only now may the next kernel start: one that took tensor memory and then
+  // waited for this grid would keep a later CTA of it waiting for its own
+  pdl_launch();
+  const uint32_t tmem = tmem_slot;  // S of half h, buffer b: 128 h + 64 b; O of half h: 256 + 128 h
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    int n = 0;
+#pragma unroll 1
+    while (!mbar_try(bar, parity))
+      if (++n > kMbarPolls || *(volatile int *)&dead) {
+        *(volatile int *)&dead = 1;
+        break;
+      }
+  };
+
+  float q_back = 0.f;  // softmax: what the scores' scale makes up for
+  if (warp < 8) {
+    // this thread's row of Q: f16 times a power of two, swizzled
+    const int r = threadIdx.x & 127, flat = row0 + min((int)threadIdx.x, nrow - 1), tok = flat / gq;
+    const uint16_t *qp = a.q + (size_t)(t0 + tok) * a.ldq + (size_t)(kvh * gq + flat - tok * gq) * D;
+    uint8_t *to = sq + (threadIdx.x >> 7) * Cfg::QB;
+    uint32_t x[D / 2];
+    if (a.vec) {
+#pragma unroll
+      for (int c = 0; c < D / 8; c++) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(qp + 8 * c);
+        x[4 * c] = u.x, x[4 * c + 1] = u.y, x[4 * c + 2] = u.z, x[4 * c + 3] = u.w;
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < D / 2; c++) x[c] = qp[2 * c] | (uint32_t)qp[2 * c + 1] << 16;
+    }
+    uint32_t most = 0u;  // of both halves of a word at once: without signs, bf16 are ordered as their bits
+#pragma unroll
+    for (int c = 0; c < D / 2; c++) most = __vmaxu2(most, x[c] & 0x7fff7fffu);
+    const float top = bf2f((uint16_t)max(most & 0xffffu, most >> 16));
+    const float f = a.scale == 0.f ? 0.f : a.scale < 0.f ? -to_2p14(top) : to_2p14(top);
+    q_back = a.scale == 0.f ? 1.f : a.scale / f;  // positive
+#pragma unroll
+    for (int c = 0; c < D / 8; c++) {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        w[k] = pack_f16x2(bf2f(x[4 * c + k] & 0xffffu) * f, __uint_as_float(x[4 * c + k] & 0xffff0000u) * f);
+      *reinterpret_cast<uint4 *>(to + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+          make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    fence_proxy_async();
+    mbar_arrive(&q_full);
+  }
+
+  if (warp >= 8 && warp < 16) {
+    // ---- unpack: page w of every tile ----
+    constexpr int EPL = 16 * G / 32, ST = Cfg::ST;  // scale entries of a lane; blocks on their way
+    const bool is_v = warp & 2;  // each scheduler has warps of one kind, and with them less code
+    const int w = (warp & 1) + 2 * (warp >= 12), g = lane >> 2, t = lane & 3;
+    uint8_t *sc = scales + (is_v ? Cfg::SC : 0) + w * 2 * D;
+    uint8_t *ring = rings + (warp - 8) * ST * Cfg::RING;
+    uint64_t *freed = is_v ? v_freed : k_freed;
+    int ids = -1;
+    uint32_t there = 0;  // bit 0: the last page asked for is there; bit 1: the one before
+    auto fetch = [&](int tile, uint8_t *to) {
+      if (tile % 32 == 0) {  // this warp's page of the next 32 tiles, by lane
+        const int p = (tile + lane) * PAGES + w;
+        ids = p < n_pages ? page_of(a.c, a.b, s, pg_lo + p) : -1;
+      }
+      const int id = __shfl_sync(0xffffffffu, ids, tile % 32);
+      there = there << 1 | (id >= 0);
+      if (id >= 0) {
+        const uint8_t *blk = a.c.pool + ((size_t)id * n_kv + kvh) * BLK;
+#pragma unroll
+        for (int x = 0; x < 8 * D; x += 512) cp_async16(to + x + 16 * lane, blk + (is_v ? 8 * D : 0) + x + 16 * lane, 16);
+        if (lane < D / 4) cp_async16(to + 8 * D + 16 * lane, blk + 16 * D + 16 * lane, 16);
+      }
+      cp_async_commit();
+    };
+    fetch(0, ring);
+    fetch(1, ring + Cfg::RING);
+    int slot = 0;
+#pragma unroll 1
+    for (int i = 0; i < n_tiles; i++) {
+      const int b = i & 1, key0 = (pg_lo + i * PAGES + w) * 16;
+      const bool here = there & 2u;
+      uint8_t *from = ring + slot * Cfg::RING;
+      cp_async_wait<ST - 2>();
+      __syncwarp();  // all lanes' copies are here, and all lanes are done with the block before
+      slot = slot == ST - 1 ? 0 : slot + 1;
+      fetch(i + 2, ring + (slot == ST - 1 ? 0 : slot + 1) * Cfg::RING);
+      // what no row sees, and what is no number, becomes zeros
+      uint32_t en[EPL];
+      float top = 0.f;
+      uint32_t bad = 0;
+#pragma unroll
+      for (int x = 0; x < EPL; x++) {
+        const int e = lane + 32 * x, c = 2 * (e >> 2 & 3) + (e & 1) + 8 * (e >> 1 & 1), key = key0 + c;  // group e / 16
+        en[x] = *reinterpret_cast<const uint32_t *>(from + 8 * D + 8 * e + (is_v ? 4 : 0));
+        if (!(here && key <= pos_hi && key >= key_lo)) en[x] = 0u;
+        if ((en[x] & 0x7f80u) == 0x7f80u || (en[x] & 0x7f800000u) == 0x7f800000u) en[x] = 0u, bad |= 1u << (e >> 4);
+        const float z = __uint_as_float(en[x] & 0xffff0000u);
+        top = fmaxf(top, fmaxf(fabsf(z), fabsf(fmaf(15.f, bf2f(en[x] & 0xffffu), z))));
+      }
+      // (of values >= 0 the largest bits are the largest value's)
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fminf(top, FLT_MAX))));
+      bad |= __shfl_xor_sync(0xffffffffu, bad, 16);  // lanes l and l + 16 hold a token's groups
+      const int some = __any_sync(0xffffffffu, bad != 0u), token = 16 * w + 2 * (lane >> 2 & 3) + (lane & 1) + 8 * (lane >> 1 & 1);
+      // {s, z} in f16, where every lane finds them
+      const float f = to_2p14(top);
+#pragma unroll
+      for (int x = 0; x < EPL; x++)
+        *reinterpret_cast<uint32_t *>(sc + 4 * (lane + 32 * x)) =
+            pack_f16x2(bf2f(en[x] & 0xffffu) * f, __uint_as_float(en[x] & 0xffff0000u) * f);
+      __syncwarp();
+      if (i >= 2) wait(&freed[b], ((i >> 1) - 1) & 1);
+      if (is_v) {
+        // rows are dims, one atom of 64 keys; digits of dims g and g + 8 of every 16
+        uint8_t *to = sv + b * Cfg::VB + g * 128 + 4 * t;
+        const int c0 = ((2 * w) ^ g) << 4, c1 = ((2 * w + 1) ^ g) << 4;
+#pragma unroll 1
+        for (int j = 0; j < G; j++, to += 32 * 128) {
+          const uint4 u = *reinterpret_cast<const uint4 *>(sc + 64 * j + 16 * t);  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+          const uint2 d = *reinterpret_cast<const uint2 *>(from + 512 * (j >> 1) + 16 * lane + 8 * (j & 1));
+          const uint32_t sx[2] = {lows(u.x, u.y), lows(u.z, u.w)}, zx[2] = {highs(u.x, u.y), highs(u.z, u.w)};
+#pragma unroll
+          for (int m = 0; m < 2; m++) {
+            uint32_t o[4];
+            unpack8(m ? d.y : d.x, sx, zx, o);  // (dim g, dim g + 8) x (keys 2t .., keys 2t + 8 ..)
+            *reinterpret_cast<uint32_t *>(to + 16 * m * 128 + c0) = o[0];
+            *reinterpret_cast<uint32_t *>(to + (16 * m + 8) * 128 + c0) = o[1];
+            *reinterpret_cast<uint32_t *>(to + 16 * m * 128 + c1) = o[2];
+            *reinterpret_cast<uint32_t *>(to + (16 * m + 8) * 128 + c1) = o[3];
+          }
+        }
+        if (lane < 16) v_bad[b][token] = (uint8_t)bad;
+        if (lane == 0) {
+          v_says[b][w] = (uint8_t)(2 * some);
+          v_exp[b][w] = -exponent(f);
+        }
+      } else {
+        // rows are keys, D / 64 atoms of 64 dims; digits of keys g and g + 8
+        uint8_t *to = sk + b * Cfg::KB + (16 * w + g) * 128;
+#pragma unroll 1
+        for (int j = 0; j < G; j++) {
+          const int c = 4 * j + t, at = (c >> 3) * (KEYS * 128) + (((c & 7) ^ g) << 4);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const uint32_t sz = *reinterpret_cast<const uint32_t *>(sc + 64 * j + 16 * (g >> 1) + 8 * h + 4 * (g & 1));
+            const uint32_t d = *reinterpret_cast<const uint32_t *>(from + 4 * D * h + 4 * G * lane + 4 * j);
+            const uint32_t s1 = lows(sz, sz), z1 = highs(sz, sz), sx[2] = {s1, s1}, zx[2] = {z1, z1};
+            uint32_t o[4];
+            unpack8(d, sx, zx, o);
+            *reinterpret_cast<uint4 *>(to + 8 * 128 * h + at) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+        // Eight deep: a softmax reads these of tile i after its scores have freed K.
+        // K of tile i + 7 waits for a score of tile i + 5, that for a softmax to be
+        // done with tile i + 2, that for V, which waits for every P V of tile i.
+        if (lane < 16) k_bad[i & 7][token] = bad != 0u;
+        if (lane == 0) {
+          k_fac[i & 7][w] = 1.f / f;
+          k_says[i & 7][w] = (uint8_t)(here + 2 * some);
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(is_v ? &v_full[b] : &k_full[b]);
+    }
+    cp_async_wait<0>();
+  } else if (warp >= 16) {
+    // ---- products: a warp to each half's S and to its P V, one lane of it ----
+    const int h = warp & 1, nt = h ? nt1 : nt0, other = h ? nt0 : nt1;
+    if (lane == 0 && warp < 18) {
+      constexpr uint32_t id_s = umma_idesc_f16(128, KEYS);
+      const uint64_t dq = sw128_desc(sq + h * Cfg::QB), dk = sw128_desc(sk);
+      if (nt > 0) wait(&q_full, 0);
+      for (int i = 0; i < nt; i++) {
+        const int b = i & 1;
+        wait(&k_full[b], (i >> 1) & 1);
+        if (i >= 2) wait(&s_freed[h][b], ((i >> 1) - 1) & 1);
+        if (*(volatile int *)&dead) break;
+        mbar_arrive(&s_full[h][b]);
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; k++)
+          umma_kf16(tmem + 128 * h + KEYS * b, dq + (((k >> 2) * (128 * 128) + 32 * (k & 3)) >> 4),
+                    dk + ((b * Cfg::KB + (k >> 2) * (KEYS * 128) + 32 * (k & 3)) >> 4), id_s, k > 0);
+        umma_commit(&s_full[h][b]);
+        umma_commit(&k_freed[b]);
+        if (i >= other) umma_commit(&k_freed[b]);  // the other half has no use for this tile
+      }
+    } else if (lane == 0) {
+      constexpr uint32_t id_o = umma_idesc_f16(128, D);
+      const uint64_t dp = sw128_desc(sp + h * Cfg::PB), dv = sw128_desc(sv);
+      for (int i = 0; i < nt; i++) {
+        const int b = i & 1;
+        wait(&v_full[b], (i >> 1) & 1);
+        wait(&p_full[h], i & 1);
+        if (*(volatile int *)&dead) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < KEYS / 16; k++)
+          umma_kf16(tmem + 256 + 128 * h, dp + ((32 * k) >> 4), dv + ((b * Cfg::VB + 32 * k) >> 4), id_o, i > 0 || k > 0);
+        umma_commit(&pv_done[h]);
+        umma_commit(&v_freed[b]);
+        if (i >= other) umma_commit(&v_freed[b]);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: a thread holds row r of half h ----
+    const int h = threadIdx.x >> 7, r = threadIdx.x & 127, nt = h ? nt1 : nt0;
+    const int flat = row0 + min((int)threadIdx.x, nrow - 1), tok = flat / gq, head = kvh * gq + flat - tok * gq;
+    const int lim = pos0 + tok, low = a.window > 0 ? lim - a.window + 1 : 0;
+    // keys that all rows of this half see
+    const int all_to = pos0 + (row0 + min(128 * h, nrow - 1)) / gq;
+    const int all_from = a.window > 0 ? pos0 + (row0 + min(128 * h + 127, nrow - 1)) / gq - a.window + 1 : 0;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, t_s = tmem + lanes + 128 * h, t_o = tmem + lanes + 256 + 128 * h;
+    uint8_t *my_p = sp + h * Cfg::PB + r * 128;
+    float m = -INFINITY, l = 0.f;  // m: what the exponents are taken from
+    int e_ref = -1000;             // power of two of O
+    uint32_t nan = 0;              // of the keys this row has seen: bit j, V of group j; bit 7, K
+#pragma unroll 1
+    for (int i = 0; i < nt; i++) {
+      const int b = i & 1, q = i & 7, key0 = (pg_lo + i * PAGES) * 16;
+      wait(&s_full[h][b], (i >> 1) & 1);
+      tc_fence_after();
+      uint32_t x[2][32];
+      tmem_ld32_async(t_s + KEYS * b, x[0]);
+      tmem_ld32_async(t_s + KEYS * b + 32, x[1]);
+      const uint32_t k_say = *reinterpret_cast<const uint32_t *>(k_says[q]);
+      const float4 k4 = *reinterpret_cast<const float4 *>(k_fac[q]);
+      const bool edge = key0 + KEYS - 1 > all_to || key0 < all_from || (k_say & 0x01010101u) != 0x01010101u;
+      // a score of page p is its column times f[p]; zero rows and pages keep it off 0 and infinity
+      float f[PAGES] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+      for (int p = 0; p < PAGES; p++) f[p] = fminf(fmaxf(q_back * f[p], 0x1p-100f), 0x1p100f);
+      tmem_wait_ld();
+      tc_fence_before();
+      mbar_arrive(&s_freed[h][b]);
+      uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+      if (edge) {
+        // bits of the keys that this row sees
+        const int last = lim - key0, first = low - key0;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          const int l1 = last - 32 * c, f1 = first - 32 * c;
+          uint32_t y = l1 < 0 ? 0u : 0xffffffffu >> (31 - min(l1, 31));
+          y = f1 > 31 ? 0u : y & 0xffffffffu << max(f1, 0);
+          if (!(k_say >> 16 * c & 1)) y &= 0xffff0000u;
+          if (!(k_say >> (16 * c + 8) & 1)) y &= 0xffffu;
+          see[c] = y;
+#pragma unroll
+          for (int k = 0; k < 32; k++)
+            if (!(y >> k & 1)) x[c][k] = 0xff800000u;
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int p = 0; p < PAGES; p++) {
+        float y = __uint_as_float(x[p >> 1][16 * (p & 1)]);
+#pragma unroll
+        for (int k = 1; k < 16; k++) y = fmaxf(y, __uint_as_float(x[p >> 1][16 * (p & 1) + k]));
+        top = fmaxf(top, y * f[p]);
+      }
+      wait(&v_full[b], (i >> 1) & 1);
+      const uint32_t v_say = *reinterpret_cast<const uint32_t *>(v_says[b]);
+      const int4 v4 = *reinterpret_cast<const int4 *>(v_exp[b]);
+      const int ve[PAGES] = {v4.x, v4.y, v4.z, v4.w};
+      if ((k_say | v_say) & 0x02020202u)
+#pragma unroll 1
+        for (int k = 0; k < KEYS; k++)
+          if (see[k >> 5] >> (k & 31) & 1) nan |= v_bad[b][k] | (uint32_t)k_bad[q][k] << 7;
+      int e_new = e_ref;  // pages that this row sees nothing of do not count
+#pragma unroll
+      for (int p = 0; p < PAGES; p++)
+        if (see[p >> 1] >> 16 * (p & 1) & 0xffffu) e_new = max(e_new, ve[p]);
+      float scale_o = 1.f;
+      bool move = false;
+      if (top > m + 8.f) {  // the first time, or past what p in f16 holds
+        scale_o = m == -INFINITY ? 0.f : ex2(m - top);
+        m = top;
+        l *= scale_o;
+        move = true;
+      }
+      if (e_new > e_ref) {
+        scale_o *= ex2((float)(e_ref - e_new));  // (0 the first time)
+        e_ref = e_new;
+        move = true;
+      }
+      if (i > 0) wait(&pv_done[h], (i - 1) & 1);  // O is whole, and P may be written
+      const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int p = 0; p < PAGES; p++) {
+        // p with V's power in it, and the sum without; far below the largest V it does not matter how far
+        const int dv = min(max(ve[p] - e_ref, -100), 0);
+        const float c0 = (float)dv - mu;
+        const uint64_t ff = f2_pack(f[p], f[p]), cc = f2_pack(c0, c0);
+        uint64_t part = 0;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const int at = 16 * (p & 1) + 8 * c + 2 * k;
+            float y0, y1;
+            f2_split(f2_fma(f2_pack(__uint_as_float(x[p >> 1][at]), __uint_as_float(x[p >> 1][at + 1])), ff, cc), y0, y1);
+            y0 = ex2(y0), y1 = ex2(y1);
+            part = f2_add(part, f2_pack(y0, y1));
+            w[k] = pack_f16x2(y0, y1);
+          }
+          *reinterpret_cast<uint4 *>(my_p + (((2 * p + c) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        float s0, s1;
+        f2_split(part, s0, s1);
+        l = fmaf(s0 + s1, __uint_as_float((uint32_t)(127 - dv) << 23), l);
+      }
+      if (i > 0 && __any_sync(0xffffffffu, move)) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D / 32; c++) {
+          tmem_ld32_async(t_o + 32 * c, x[0]);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 32; k++) x[0][k] = __float_as_uint(__uint_as_float(x[0][k]) * scale_o);
+          tmem_st32(t_o + 32 * c, x[0]);
+        }
+      }
+      tc_fence_before();
+      fence_proxy_async();
+      mbar_arrive(&p_full[h]);
+    }
+    if (nt > 0) wait(&pv_done[h], (nt - 1) & 1);
+    tc_fence_after();
+    const bool gone = *(volatile int *)&dead;
+    const float up = exp2f((float)max(e_ref, -126)), inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t *op = a.out + (size_t)(t0 + tok) * a.ldo + (size_t)head * D;
+#pragma unroll 1
+    for (int c = 0; c < D / 32; c++) {
+      uint32_t x[32];
+      if (nt > 0) {
+        tmem_ld32_async(t_o + 32 * c, x);
+        tmem_wait_ld();
+      }
+      const bool is_nan = gone || (nan >> 7 & 1) || (nan >> c & 1);
+#pragma unroll
+      for (int k = 0; k < 32; k++)
+        x[k] = is_nan ? 0x7fc00000u : l == 0.f ? 0u : __float_as_uint(__uint_as_float(x[k]) * inv * up);
+      if ((int)threadIdx.x < nrow) {
+        if (a.vec) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            uint32_t y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              y[e] = pack_bf16x2(__uint_as_float(x[8 * k + 2 * e]), __uint_as_float(x[8 * k + 2 * e + 1]));
+            *reinterpret_cast<uint4 *>(op + 32 * c + 8 * k) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; k++) op[32 * c + k] = f2bf(__uint_as_float(x[k]));
+        }
+      }
+    }
+    if (gone && threadIdx.x == 0 && a.err) atomicOr(a.err, 0x400);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 16) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -1229,11 +1771,38 @@ cudaError_t kv4_read(const Kv4ReadArgs &a0, cudaStream_t st, bool pdl) {
   return a.c.head_dim == 128 ? read_launch<128>(a, windows, st, pdl) : read_launch<64>(a, windows, st, pdl);
 }
 
+template <int D>
+static cudaError_t prompt_launch(const Kv4AttendArgs &a, int thr, cudaStream_t st, bool pdl) {
+  using Cfg = PromptCfg<D>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = once_per_device(done, [] {
+    return cudaFuncSetAttribute(k_kv4_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  // tiles, at most: whole ones, and one more for every sequence that has over thr rows
+  const int64_t rows = (int64_t)a.b.num_tokens * (a.n_heads / a.c.n_kv);
+  const int64_t tiles = rows / Cfg::ROWS + std::min<int64_t>(a.b.num_seqs, rows / (thr + 1));
+  const int64_t grid = std::min<int64_t>(tiles, rows) * a.c.n_kv;
+  if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  return launch(k_kv4_prompt<D>, dim3((unsigned)grid), Cfg::THREADS, Cfg::kSmem, 1, pdl, st, a, thr);
+}
+
 cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st,
                        bool pdl) {
   if (a0.b.num_tokens <= 0 || a0.b.num_seqs <= 0) return cudaSuccess;
-  const int rows = (max_q > 0 ? max_q : 2) * (a0.n_heads / a0.c.n_kv);  // rows of a kv head: one column tile, or two
   Kv4AttendArgs a = a0;
+  const int gq = a.n_heads / a.c.n_kv;
+  // sequences of more rows than this go by tiles of 128 rows on k_kv4_prompt
+  constexpr int kBig = 16;
+  const bool some_big = max_q <= 0 || (int64_t)max_q * gq > kBig;
+  const bool mostly_big = some_big && (int64_t)a.b.num_tokens * gq > (int64_t)kBig * a.b.num_seqs;
+  if (some_big) {
+    const int thr = mostly_big ? 0 : kBig;
+    const cudaError_t e = a.c.head_dim == 128 ? prompt_launch<128>(a, thr, st, pdl) : prompt_launch<64>(a, thr, st, pdl);
+    if (e != cudaSuccess || mostly_big) return e;
+    a.big = kBig;
+  }
+  const int rows = (some_big ? 1 : max_q) * gq;  // rows of a kv head: one column tile, or two
   constexpr int kSeqs = AttendCfg<128, 1>::MAXSEQ;
   for (int s0 = 0; s0 < a0.b.num_seqs; s0 += kSeqs) {  // sequences of one launch
     a.b.num_seqs = std::min(kSeqs, a0.b.num_seqs - s0);

@@ -65,6 +65,8 @@ struct Kv4AttendArgs {
   float scale;        // of the scores, times log2(e)
   int window;         // keys a query sees at most (0: all before it)
   int vec;            // q and out rows start on 16-byte boundaries
+  int *err;           // set (bitwise or) when a bounded wait gave up; nullable
+  int big;            // launcher: sequences of more rows are another kernel's (0: none)
 };
 
 struct Kv4ReadArgs {
