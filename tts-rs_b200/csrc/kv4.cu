@@ -60,6 +60,19 @@ template <class F>
 Q3T_DEV bool find_item(int num_seqs, int item, F count, int &s, int &i) {
   __shared__ int warp_tot[32], hit[2];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  if (num_seqs <= 32) {  // every warp for itself
+    const int mine = lane < num_seqs ? count(lane) : 0;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const uint32_t found = __ballot_sync(0xffffffffu, item < incl);
+    s = __ffs(found) - 1;
+    i = item - __shfl_sync(0xffffffffu, incl - mine, max(s, 0));
+    return s >= 0;
+  }
   if (threadIdx.x == 0) hit[0] = -1;
   for (int base = 0; base < num_seqs; base += blockDim.x) {
     const int mine = base + (int)threadIdx.x < num_seqs ? count(base + threadIdx.x) : 0;
@@ -1218,7 +1231,10 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   using Cfg = PromptCfg<D>;
   constexpr int G = Cfg::G, BLK = Cfg::BLK, ROWS = Cfg::ROWS, KEYS = Cfg::KEYS, PAGES = Cfg::PAGES;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t k_full[2], v_full[2], k_freed[2], v_freed[2], s_full[2][2], s_freed[2][2], p_full[2], pv_done[2], q_full;
+  __shared__ uint64_t bars[21];
+  uint64_t *k_full = bars, *v_full = bars + 2, *k_freed = bars + 4, *v_freed = bars + 6;  // by buffer
+  uint64_t *s_full = bars + 8, *s_freed = bars + 12;                                     // by half and buffer
+  uint64_t *p_full = bars + 16, *pv_done = bars + 18, *q_full = bars + 20;               // by half
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) float k_fac[8][PAGES];
   __shared__ __align__(16) int v_exp[2][PAGES];
@@ -1231,6 +1247,14 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   pdl_wait();
   const int n_kv = a.c.n_kv, gq = a.n_heads / n_kv, kvh = blockIdx.x % n_kv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 17 && lane < 21) {
+    // arrivals: the unpacking warps; both halves' products; the scores, and what K's warps say of the tile;
+    // the softmax threads of a half; P V; all softmax threads
+    const int n = lane < 4 ? PAGES : lane < 12 ? 2 : lane < 18 ? 128 : lane < 20 ? 1 : 256;
+    mbar_init(&bars[lane], n);
+    fence_mbar_init();
+    if (lane == 0) dead = 0;
+  }
   int s, i_rev;
   if (!find_item(
           a.b.num_seqs, blockIdx.x / n_kv,
@@ -1252,23 +1276,6 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   const int nt0 = tiles_to(pos0 + (row0 + min(nrow, 128) - 1) / gq), nt1 = nrow > 128 ? tiles_to(pos_hi) : 0;
   const int n_tiles = max(nt0, nt1), n_pages = pos_hi < 0 ? 0 : max(0, (pos_hi >> 4) + 1 - pg_lo);
 
-  if (threadIdx.x == 0) {
-    for (int b = 0; b < 2; b++) {
-      mbar_init(&k_full[b], PAGES);
-      mbar_init(&v_full[b], PAGES);
-      mbar_init(&k_freed[b], 2);
-      mbar_init(&v_freed[b], 2);
-      for (int h = 0; h < 2; h++) {
-        mbar_init(&s_full[h][b], 2);  // the scores, and what K's warps say of the tile
-        mbar_init(&s_freed[h][b], 128);
-      }
-      mbar_init(&p_full[b], 128);
-      mbar_init(&pv_done[b], 1);
-    }
-    mbar_init(&q_full, 256);
-    fence_mbar_init();
-    dead = 0;
-  }
   if (warp == 16) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -1287,40 +1294,70 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       }
   };
 
+  // row o of the tile is head hd of token tok of the sequence; o + rem0 is small, so 2^32 / gq, rounded up, divides it
+  const int tok0 = row0 / gq, rem0 = row0 - tok0 * gq;
+  const uint32_t inv_gq = gq == 1 ? 0u : 0xffffffffu / (uint32_t)gq + 1u;
+  auto row_at = [&](int o, int &tok, int &hd) {
+    const int x = rem0 + min(o, nrow - 1), y = gq == 1 ? x : (int)__umulhi((uint32_t)x, inv_gq);
+    tok = tok0 + y;
+    hd = kvh * gq + x - y * gq;
+  };
+  // Q's way in and O's way out: LPR lanes to a row, so that a warp's accesses are whole lines
+  constexpr int LPR = D / 8, RPS = 32 / LPR;
+  auto q_at = [&](int o, int c) {  // 16 bytes: dims 8 c .. of row o
+    return reinterpret_cast<uint4 *>(sq + (o >> 7) * Cfg::QB + (c >> 3) * (128 * 128) + (o & 127) * 128 +
+                                     (((c & 7) ^ (o & 7)) << 4));
+  };
   float q_back = 0.f;  // softmax: what the scores' scale makes up for
   if (warp < 8) {
-    // this thread's row of Q: f16 times a power of two, swizzled
-    const int r = threadIdx.x & 127, flat = row0 + min((int)threadIdx.x, nrow - 1), tok = flat / gq;
-    const uint16_t *qp = a.q + (size_t)(t0 + tok) * a.ldq + (size_t)(kvh * gq + flat - tok * gq) * D;
-    uint8_t *to = sq + (threadIdx.x >> 7) * Cfg::QB;
-    uint32_t x[D / 2];
+    // Q: f16 times a power of two per row, swizzled; a warp has the rows of its own threads
+    const int c = lane % LPR, k0 = lane / LPR;
+    int tok, hd;
+    row_at(threadIdx.x, tok, hd);
+    const long long mine = (long long)((size_t)(t0 + tok) * a.ldq + (size_t)hd * D);
     if (a.vec) {
-#pragma unroll
-      for (int c = 0; c < D / 8; c++) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(qp + 8 * c);
-        x[4 * c] = u.x, x[4 * c + 1] = u.y, x[4 * c + 2] = u.z, x[4 * c + 3] = u.w;
-      }
+#pragma unroll 8
+      for (int k = 0; k < 32; k += RPS)
+        cp_async16(q_at(32 * warp + k0 + k, c), a.q + __shfl_sync(0xffffffffu, mine, k0 + k) + 8 * c, 16);
     } else {
+#pragma unroll 1
+      for (int k = 0; k < 32; k += RPS) {
+        const uint16_t *from = a.q + __shfl_sync(0xffffffffu, mine, k0 + k) + 8 * c;
+        uint32_t x[4];
 #pragma unroll
-      for (int c = 0; c < D / 2; c++) x[c] = qp[2 * c] | (uint32_t)qp[2 * c + 1] << 16;
+        for (int e = 0; e < 4; e++) x[e] = from[2 * e] | (uint32_t)from[2 * e + 1] << 16;
+        *q_at(32 * warp + k0 + k, c) = make_uint4(x[0], x[1], x[2], x[3]);
+      }
     }
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncwarp();
     uint32_t most = 0u;  // of both halves of a word at once: without signs, bf16 are ordered as their bits
+#pragma unroll 8
+    for (int c8 = 0; c8 < D / 8; c8++) {
+      const uint4 u = *q_at(threadIdx.x, c8);
+      most = __vmaxu2(most, __vmaxu2(__vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu),
+                                     __vmaxu2(u.z & 0x7fff7fffu, u.w & 0x7fff7fffu)));
+    }
+    const float up = to_2p14(bf2f((uint16_t)max(most & 0xffffu, most >> 16)));
+    const float f = a.scale == 0.f ? 0.f : a.scale < 0.f ? -up : up;
+    q_back = a.scale == 0.f ? 1.f : fabsf(a.scale) * __uint_as_float((254u << 23) - __float_as_uint(up));  // / up
+#pragma unroll 1
+    for (int c8 = 0; c8 < D / 8; c8 += 4) {
+      uint4 u[4];
 #pragma unroll
-    for (int c = 0; c < D / 2; c++) most = __vmaxu2(most, x[c] & 0x7fff7fffu);
-    const float top = bf2f((uint16_t)max(most & 0xffffu, most >> 16));
-    const float f = a.scale == 0.f ? 0.f : a.scale < 0.f ? -to_2p14(top) : to_2p14(top);
-    q_back = a.scale == 0.f ? 1.f : a.scale / f;  // positive
+      for (int k = 0; k < 4; k++) u[k] = *q_at(threadIdx.x, c8 + k);
 #pragma unroll
-    for (int c = 0; c < D / 8; c++) {
-      uint32_t w[4];
+      for (int k = 0; k < 4; k++) {
+        const uint32_t x[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+        uint32_t w[4];
 #pragma unroll
-      for (int k = 0; k < 4; k++)
-        w[k] = pack_f16x2(bf2f(x[4 * c + k] & 0xffffu) * f, __uint_as_float(x[4 * c + k] & 0xffff0000u) * f);
-      *reinterpret_cast<uint4 *>(to + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
-          make_uint4(w[0], w[1], w[2], w[3]);
+        for (int e = 0; e < 4; e++) w[e] = pack_f16x2(bf2f(x[e] & 0xffffu) * f, __uint_as_float(x[e] & 0xffff0000u) * f);
+        *q_at(threadIdx.x, c8 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
     fence_proxy_async();
-    mbar_arrive(&q_full);
+    mbar_arrive(q_full);
   }
 
   if (warp >= 8 && warp < 16) {
@@ -1445,19 +1482,19 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     if (lane == 0 && warp < 18) {
       constexpr uint32_t id_s = umma_idesc_f16(128, KEYS);
       const uint64_t dq = sw128_desc(sq + h * Cfg::QB), dk = sw128_desc(sk);
-      if (nt > 0) wait(&q_full, 0);
+      if (nt > 0) wait(q_full, 0);
       for (int i = 0; i < nt; i++) {
         const int b = i & 1;
         wait(&k_full[b], (i >> 1) & 1);
-        if (i >= 2) wait(&s_freed[h][b], ((i >> 1) - 1) & 1);
+        if (i >= 2) wait(&s_freed[2 * h + b], ((i >> 1) - 1) & 1);
         if (*(volatile int *)&dead) break;
-        mbar_arrive(&s_full[h][b]);
+        mbar_arrive(&s_full[2 * h + b]);
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; k++)
           umma_kf16(tmem + 128 * h + KEYS * b, dq + (((k >> 2) * (128 * 128) + 32 * (k & 3)) >> 4),
                     dk + ((b * Cfg::KB + (k >> 2) * (KEYS * 128) + 32 * (k & 3)) >> 4), id_s, k > 0);
-        umma_commit(&s_full[h][b]);
+        umma_commit(&s_full[2 * h + b]);
         umma_commit(&k_freed[b]);
         if (i >= other) umma_commit(&k_freed[b]);  // the other half has no use for this tile
       }
@@ -1482,7 +1519,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   } else {
     // ---- softmax: a thread holds row r of half h ----
     const int h = threadIdx.x >> 7, r = threadIdx.x & 127, nt = h ? nt1 : nt0;
-    const int flat = row0 + min((int)threadIdx.x, nrow - 1), tok = flat / gq, head = kvh * gq + flat - tok * gq;
+    int tok, hd;
+    row_at(threadIdx.x, tok, hd);
     const int lim = pos0 + tok, low = a.window > 0 ? lim - a.window + 1 : 0;
     // keys that all rows of this half see
     const int all_to = pos0 + (row0 + min(128 * h, nrow - 1)) / gq;
@@ -1495,7 +1533,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
 #pragma unroll 1
     for (int i = 0; i < nt; i++) {
       const int b = i & 1, q = i & 7, key0 = (pg_lo + i * PAGES) * 16;
-      wait(&s_full[h][b], (i >> 1) & 1);
+      wait(&s_full[2 * h + b], (i >> 1) & 1);
       tc_fence_after();
       uint32_t x[2][32];
       tmem_ld32_async(t_s + KEYS * b, x[0]);
@@ -1509,7 +1547,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       for (int p = 0; p < PAGES; p++) f[p] = fminf(fmaxf(q_back * f[p], 0x1p-100f), 0x1p100f);
       tmem_wait_ld();
       tc_fence_before();
-      mbar_arrive(&s_freed[h][b]);
+      mbar_arrive(&s_freed[2 * h + b]);
       uint32_t see[2] = {0xffffffffu, 0xffffffffu};
       if (edge) {
         // bits of the keys that this row sees
@@ -1606,7 +1644,6 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     tc_fence_after();
     const bool gone = *(volatile int *)&dead;
     const float up = exp2f((float)max(e_ref, -126)), inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t *op = a.out + (size_t)(t0 + tok) * a.ldo + (size_t)head * D;
 #pragma unroll 1
     for (int c = 0; c < D / 32; c++) {
       uint32_t x[32];
@@ -1614,24 +1651,40 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         tmem_ld32_async(t_o + 32 * c, x);
         tmem_wait_ld();
       }
+      else {
+#pragma unroll
+        for (int k = 0; k < 32; k++) x[k] = 0u;
+      }
       const bool is_nan = gone || (nan >> 7 & 1) || (nan >> c & 1);
+      const float f1 = is_nan ? __uint_as_float(0x7fc00000u) : inv;
 #pragma unroll
-      for (int k = 0; k < 32; k++)
-        x[k] = is_nan ? 0x7fc00000u : l == 0.f ? 0u : __float_as_uint(__uint_as_float(x[k]) * inv * up);
-      if ((int)threadIdx.x < nrow) {
-        if (a.vec) {
+      for (int k = 0; k < 4; k++) {
+        uint32_t y[4];
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            uint32_t y[4];
+        for (int e = 0; e < 4; e++)
+          y[e] = pack_bf16x2(__uint_as_float(x[8 * k + 2 * e]) * f1 * up, __uint_as_float(x[8 * k + 2 * e + 1]) * f1 * up);
+        *q_at(threadIdx.x, 4 * c + k) = make_uint4(y[0], y[1], y[2], y[3]);  // (this half's S are done with Q)
+      }
+    }
+    __syncwarp();
+    const int c = lane % LPR, k0 = lane / LPR;
+    const long long mine = (long long)((size_t)(t0 + tok) * a.ldo + (size_t)hd * D);
+    if (a.vec) {
+#pragma unroll 8
+      for (int k = 0; k < 32; k += RPS) {
+        const uint4 u = *q_at(32 * warp + k0 + k, c);
+        uint16_t *to = a.out + __shfl_sync(0xffffffffu, mine, k0 + k) + 8 * c;
+        if (32 * warp + k0 + k < nrow) *reinterpret_cast<uint4 *>(to) = u;
+      }
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < 32; k += RPS) {
+        const uint4 u = *q_at(32 * warp + k0 + k, c);
+        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+        uint16_t *to = a.out + __shfl_sync(0xffffffffu, mine, k0 + k) + 8 * c;
+        if (32 * warp + k0 + k < nrow)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              y[e] = pack_bf16x2(__uint_as_float(x[8 * k + 2 * e]), __uint_as_float(x[8 * k + 2 * e + 1]));
-            *reinterpret_cast<uint4 *>(op + 32 * c + 8 * k) = make_uint4(y[0], y[1], y[2], y[3]);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; k++) op[32 * c + k] = f2bf(__uint_as_float(x[k]));
-        }
+          for (int e = 0; e < 8; e++) to[e] = (uint16_t)(x[e >> 1] >> 16 * (e & 1));
       }
     }
     if (gone && threadIdx.x == 0 && a.err) atomicOr(a.err, 0x400);
