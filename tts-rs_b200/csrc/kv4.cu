@@ -60,18 +60,27 @@ template <class F>
 Q3T_DEV bool find_item(int num_seqs, int item, F count, int &s, int &i) {
   __shared__ int warp_tot[32], hit[2];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  if (num_seqs <= 32) {  // every warp for itself
-    const int mine = lane < num_seqs ? count(lane) : 0;
-    int incl = mine;
+  if (num_seqs <= 128) {  // every warp for itself, four sequences to a lane
+    int mine[4], sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) mine[j] = 4 * lane + j < num_seqs ? count(4 * lane + j) : 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) sum += mine[j];
+    int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
     const uint32_t found = __ballot_sync(0xffffffffu, item < incl);
-    s = __ffs(found) - 1;
-    i = item - __shfl_sync(0xffffffffu, incl - mine, max(s, 0));
-    return s >= 0;
+    const int at = max(__ffs(found) - 1, 0);
+    int j = 0, left = item - (incl - sum);  // of that lane's four: which, and where in it
+#pragma unroll
+    for (int x = 0; x < 3; x++)
+      if (j == x && left >= mine[x]) left -= mine[x], j = x + 1;
+    s = found ? 4 * at + __shfl_sync(0xffffffffu, j, at) : -1;
+    i = __shfl_sync(0xffffffffu, left, at);
+    return found != 0;
   }
   if (threadIdx.x == 0) hit[0] = -1;
   for (int base = 0; base < num_seqs; base += blockDim.x) {
@@ -138,91 +147,129 @@ int max_windows(const Kv4Batch &b) {
 // ---------------------------------------------------------------------------
 // Rows
 // ---------------------------------------------------------------------------
-Q3T_DEV void load4(const float *p, bool vec, float v[4]) {
-  if (vec) {
-    const float4 u = *reinterpret_cast<const float4 *>(p);
-    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = p[i];
-  }
+// Pairs of f32: one instruction for two of the same.
+Q3T_DEV uint64_t f2_pack(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
 }
-Q3T_DEV void load4(const uint16_t *p, bool vec, float v[4]) {
-  if (vec) {
-    const uint2 u = *reinterpret_cast<const uint2 *>(p);
-    v[0] = bf2f(u.x & 0xffffu), v[1] = bf2f(u.x >> 16), v[2] = bf2f(u.y & 0xffffu), v[3] = bf2f(u.y >> 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = bf2f(p[i]);
-  }
+Q3T_DEV void f2_split(uint64_t d, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+Q3T_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
 }
-Q3T_DEV void store4(uint16_t *p, bool vec, const float v[4]) {
-  if (vec) {
-    *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) p[i] = f2bf(v[i]);
-  }
+Q3T_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
+Q3T_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+Q3T_DEV uint64_t f2_sub(uint64_t a, uint64_t b) { return f2_fma(b, 0xbf800000bf800000ull, a); }
 
-// RMSNorm of a row spread over LPR lanes, four dims each.  The sum of squares
-// runs in 64 bits, so its order leaves no trace in the 32-bit factor.
-template <int LPR>
-Q3T_DEV void norm_row(float v[4], const float *gamma, float eps, int l) {
-  double ss = 0.0;
+// Eight elements of a row, as they are and as floats.
+template <typename T>
+struct Raw8 {
+  uint32_t w[2 * sizeof(T)];
+};
+template <typename T>
+Q3T_DEV void load8(const T *p, bool vec, Raw8<T> &x) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) ss += (double)v[i] * v[i];
+  for (int i = 0; i < (int)(2 * sizeof(T)); i += 4) {
+    if (vec) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
+      x.w[i] = u.x, x.w[i + 1] = u.y, x.w[i + 2] = u.z, x.w[i + 3] = u.w;
+    } else {
 #pragma unroll
-  for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const float r = (float)(1.0 / sqrt(ss / (4 * LPR) + (double)eps));
-#pragma unroll
-  for (int i = 0; i < 4; i++) v[i] = __fmul_rn(__fmul_rn(v[i], r), gamma[4 * l + i]);
-}
-
-// Rotation of a row by (cos, sin) per pair; every product and sum is rounded
-// by itself, so a value does not depend on which of them a compiler fuses.
-template <int LPR>
-Q3T_DEV void rotate_row(float v[4], const float2 *cs, int rot, int interleaved, int l) {
-  if (interleaved) {
-    if (4 * l < rot) {
-#pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        const float2 f = cs[2 * l + (i >> 1)];
-        const float a = v[i], b = v[i + 1];
-        v[i] = __fsub_rn(__fmul_rn(a, f.x), __fmul_rn(b, f.y));
-        v[i + 1] = __fadd_rn(__fmul_rn(b, f.x), __fmul_rn(a, f.y));
+      for (int k = i; k < i + 4; k++) {
+        if constexpr (sizeof(T) == 4)
+          x.w[k] = __float_as_uint(p[k]);
+        else
+          x.w[k] = p[2 * k] | (uint32_t)p[2 * k + 1] << 16;
       }
     }
-    return;
-  }
-  const int q = rot >> 3;  // lanes of the first half (rot % 8 == 0)
-  const bool first = l < q, in = l < 2 * q;
-  const int src = first ? l + q : in ? l - q : l;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const float p = __shfl_sync(0xffffffffu, v[i], src, LPR);
-    if (in) {
-      const float2 f = cs[4 * (first ? l : l - q) + i];
-      const float a = __fmul_rn(v[i], f.x), b = __fmul_rn(p, f.y);
-      v[i] = first ? __fsub_rn(a, b) : __fadd_rn(a, b);
-    }
   }
 }
-
-// Digits, scale and zero of the group of 32 that this lane's 8 lanes hold.  A
-// group with a value that is not finite gets a NaN scale and zero: it reads
-// back as NaN, as such a value does from a cache that is not quantised.
-Q3T_DEV void quantise(const float v[4], uint32_t n[4], uint16_t &scale, uint16_t &zero) {
-  float lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), hi = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-  int bad = 0;
+Q3T_DEV void floats(const Raw8<float> &x, float v[8]) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) bad |= !(fabsf(v[i]) <= FLT_MAX);
+  for (int i = 0; i < 8; i++) v[i] = __uint_as_float(x.w[i]);
+}
+Q3T_DEV void floats(const Raw8<uint16_t> &x, float v[8]) {
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+  for (int i = 0; i < 4; i++) v[2 * i] = bf2f(x.w[i] & 0xffffu), v[2 * i + 1] = __uint_as_float(x.w[i] & 0xffff0000u);
+}
+Q3T_DEV void store8(uint16_t *p, bool vec, const float v[8]) {
+  if (vec) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                               pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) p[i] = f2bf(v[i]);
   }
+}
+// the smaller and the larger, NaN if one is
+Q3T_DEV float min_nan(float a, float b) {
+  float d;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+Q3T_DEV float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// Sum of squares to about 2^-45 of itself: every addition's error (Knuth's
+// two-sum), and every square's, goes into a second sum.  In 32 bits, two at a
+// time: a conversion to 64 costs as much as eight of these.  For sums in
+// 2^-90 .. 2^100; another has squares that 32 bits do not hold.
+Q3T_DEV double square_sum(const float v[8]) {
+  uint64_t sum = 0, rest = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t x = f2_pack(v[i], v[i + 1]), sq = f2_mul(x, x);
+    rest = f2_sub(rest, f2_fma(x, f2_mul(x, 0xbf800000bf800000ull), sq));
+    if (i == 0) {
+      sum = sq;
+      continue;
+    }
+    const uint64_t t = f2_add(sum, sq), b = f2_sub(t, sum);
+    rest = f2_add(rest, f2_add(f2_sub(sum, f2_sub(t, b)), f2_sub(sq, b)));
+    sum = t;
+  }
+  float s0, s1, r0, r1;
+  f2_split(sum, s0, s1);
+  f2_split(rest, r0, r1);
+  return (double)s0 + (double)s1 + (double)(r0 + r1);
+}
+// 1 / sqrt(x) rounded to 32 bits: the 32-bit one and a Newton step in 64 bits
+Q3T_DEV float rsqrt64(double x) {
+  const float f = (float)x;
+  if (!(f > 0x1p-100f && f < 0x1p100f)) return (float)(1.0 / sqrt(x));
+  const double y = rsqrtf(f), e = fma(-x * y, y, 1.0);
+  return (float)fma(0.5 * e, y, y);
+}
+
+// Digits, scale and zero of a group of 32 that four lanes hold; a digit lies
+// in the low bits of n[i], whose others are kDigit's.  A group with a value
+// that is not finite gets a NaN scale and zero: it reads back as NaN, as such
+// a value does from a cache that is not quantised.  Without a scale (false)
+// the digits are to be zeros.
+constexpr uint32_t kDigit = 0x4b400000u;  // 1.5 2^23
+Q3T_DEV bool quantise(const float v[8], uint32_t n[8], uint32_t &scale_zero) {
+  float lo = v[0], hi = v[0];
+#pragma unroll
+  for (int i = 1; i < 8; i++) lo = min_nan(lo, v[i]), hi = max_nan(hi, v[i]);
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  const bool bad = !(fabsf(lo) <= FLT_MAX && fabsf(hi) <= FLT_MAX);
   // towards minus infinity: more magnitude below zero, less above
   uint32_t zb = __float_as_uint(lo);
   zb = ((zb >> 31 && (zb << 1)) ? zb + 0xffffu : zb) & 0xffff0000u;
@@ -231,28 +278,45 @@ Q3T_DEV void quantise(const float v[4], uint32_t n[4], uint16_t &scale, uint16_t
   // halves first: the range of two finite values need not be finite
   const uint16_t sb = f2bf(__fmul_rn(__fsub_rn(__fmul_rn(hi, 0.5f), __fmul_rn(z, 0.5f)), (float)(2.0 / 15.0)));
   const float s = bf2f(sb);
-  scale = bad ? 0x7fc0 : sb;
-  zero = bad ? 0x7fc0 : (uint16_t)(zb >> 16);
+  scale_zero = bad ? 0x7fc07fc0u : sb | zb;
+  // The quotient correctly rounded (Markstein 1990): y is 1 / s rounded, q the
+  // product rounded, q + y (t - q s) then rounds as t / s does.  A scale that
+  // is small enough for its reciprocal to overflow is first raised, with t.
+  const float up = s < 0x1p-80f ? 0x1p100f : 1.f, su = s * up, y = __frcp_rn(su);
+  const uint64_t z2 = f2_pack(-z, -z), up2 = f2_pack(up, up), s2 = f2_pack(-su, -su), y2 = f2_pack(y, y);
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const float d = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v[i], z), s)), 0.f), 15.f);
-    n[i] = !bad && s > 0.f ? (uint32_t)d : 0u;
+  for (int i = 0; i < 8; i += 2) {
+    const uint64_t t = f2_mul(f2_add(f2_pack(v[i], v[i + 1]), z2), up2), q = f2_mul(t, y2);
+    float d0, d1;
+    f2_split(f2_fma(f2_fma(q, s2, t), y2, q), d0, d1);
+    d0 = fmaxf(fminf(d0, 15.f), 0.f), d1 = fmaxf(fminf(d1, 15.f), 0.f);  // (t infinite: 15)
+    f2_split(f2_add(f2_pack(d0, d1), f2_pack(0x1.8p23f, 0x1.8p23f)), d0, d1);  // to the nearest, ties to even
+    n[i] = __float_as_uint(d0), n[i + 1] = __float_as_uint(d1);
   }
+  return !bad && s > 0.f;
 }
 
 // ---------------------------------------------------------------------------
-// Append: one CTA per (window, head split).  Rows go through a warp (D = 128)
-// or half a warp (D = 64), four dims to a lane; blocks are put together in
-// shared memory, and a window that fills its page is written in 16-byte
-// pieces, any other in the bytes that its tokens own.
+// Append: one CTA per (window, head split).  A lane has eight dims of a row,
+// four lanes a group of 32, and a warp two rows (D = 128) or four of one kind.
+// Blocks are put together in shared memory, and a window that fills its page
+// is written in 16-byte pieces, any other in the bytes that its tokens own.
+// (With 32 dims to a lane the sums and shuffles per element are fewer, but the
+// code is four times as long, and a decoding step, which goes through it once,
+// spends its time fetching it: 64 rows took 11.2 us, like this 5.4.)
 // ---------------------------------------------------------------------------
 constexpr int kAppendThreads = 256;
 
+// {cos, cos, sin, sin} of the pairs f = 32 i + 8 l + e and f + 1, f even, lie in the
+// order [i][e / 2][l]: neighbouring lanes read neighbouring banks
+Q3T_DEV int cs_at(int f) { return (((f >> 5) << 2) + ((f >> 1) & 3)) * 4 + ((f >> 3) & 3); }
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
-  constexpr int LPR = D / 4, RPW = 32 / LPR, G = D / 32, BLK = kv4_block_bytes(D);
+__global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
+  constexpr int LPR = D / 8, RPW = 32 / LPR, G = D / 32, BLK = kv4_block_bytes(D), CS = D / 4 + 4;
   extern __shared__ __align__(16) uint8_t img[];  // [kv heads of this split][BLK]
-  __shared__ float2 cs[kKv4Page][D / 2];
+  __shared__ float4 cs[kKv4Page * CS];
+  __shared__ __align__(16) float gam[2][D];
   pdl_wait();
   pdl_launch();
   Window w;
@@ -261,61 +325,146 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv4_append(const __grid_cons
   const int qh0 = (int)((int64_t)a.n_heads * y / sp), qh1 = (int)((int64_t)a.n_heads * (y + 1) / sp);
   const int kh0 = (int)((int64_t)a.c.n_kv * y / sp), kh1 = (int)((int64_t)a.c.n_kv * (y + 1) / sp);
   const int nq = qh1 - qh0, nk = kh1 - kh0;
-  const int half = a.rope.rot / 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, C = lane % LPR, l = C & 3;
+  const int q_items = (w.n * nq + RPW - 1) / RPW, k_items = (w.n * nk + RPW - 1) / RPW, items = q_items + 2 * k_items;
+  const uint32_t inv_n = w.n == 1 ? 0u : 0xffffffffu / (uint32_t)w.n + 1u;  // divides a row's number, which is small
+  // kind 0 q, 1 k, 2 v: of a warp at a time
+  int kind, h, tok, item = warp, left = 0;
+  int64_t ld = 0;
+  const T *base = nullptr;
+  auto set_kind = [&] {
+    kind = item < q_items ? 0 : item < q_items + k_items ? 1 : 2;
+    left = item - (kind == 0 ? 0 : kind == 1 ? q_items : q_items + k_items);
+    ld = kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv;
+    base = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + w.t0 * ld + (kind ? kh0 : qh0) * D + 8 * C;
+  };
+  auto fetch = [&](Raw8<T> &x) {
+    const int r = min(RPW * left + lane / LPR, w.n * (kind ? nk : nq) - 1);  // a row past the end repeats the last one
+    h = w.n == 1 ? r : (int)__umulhi((uint32_t)r, inv_n);
+    tok = r - h * w.n;
+    load8(base + tok * ld + h * D, a.vec, x);
+  };
+  Raw8<T> raw = {};
+  set_kind();
+  if (item < items) fetch(raw);
+  const int page = page_of(a.c, a.b, w.s, w.p), half = a.rope.rot / 2;
   for (int i = threadIdx.x; i < w.n * half; i += kAppendThreads) {
     const int c = i / half, f = i - c * half;
     double s, co;  // angles in 64 bits: a 32-bit product is off by its position's last bits
     sincospi((double)(w.p * 16 + w.c0 + c) * a.rope.freq_pi[f], &s, &co);
-    cs[c][f] = make_float2((float)(co * a.rope.amplitude), (float)(s * a.rope.amplitude));
+    float *to = reinterpret_cast<float *>(cs + c * CS + cs_at(f)) + (f & 1);
+    to[0] = (float)(co * a.rope.amplitude);
+    to[2] = (float)(s * a.rope.amplitude);
   }
-  const int page = page_of(a.c, a.b, w.s, w.p);
+  for (int i = threadIdx.x; i < 2 * D; i += kAppendThreads) {
+    const float *g = i < D ? a.q_gamma : a.k_gamma;
+    if (g) gam[i / D][i % D] = g[i % D];
+  }
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LPR, per = nq + 2 * nk, rows = w.n * per;
-  for (int r0 = warp * RPW; r0 < rows; r0 += (kAppendThreads / 32) * RPW) {
-    const int r = min(r0 + lane / LPR, rows - 1);  // a row past the end repeats the last one
-    const int tok = r / per, hs = r - tok * per;
-    const size_t row = (size_t)(w.t0 + tok);
-    const int kind = hs < nq ? 0 : hs < nq + nk ? 1 : 2;
-    const int head = kind == 0 ? qh0 + hs : kind == 1 ? kh0 + hs - nq : kh0 + hs - nq - nk;
-    const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
-                   row * (kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv) + (size_t)head * D + 4 * l;
-    float v[4];
-    load4(src, a.vec, v);
-    const float *gamma = kind == 0 ? a.q_gamma : kind == 1 ? a.k_gamma : nullptr;
-    if (a.q_gamma || a.k_gamma) {  // the shuffles are for the whole warp
-      float n[4] = {v[0], v[1], v[2], v[3]};
-      norm_row<LPR>(n, gamma ? gamma : (a.q_gamma ? a.q_gamma : a.k_gamma), a.eps, l);
-      if (gamma)
+  // of the rotation by halves, for dims 8 C .. + 3 and + 4 .. + 7: where the others of their pairs are (rot % 8 ==
+  // 0, so the same element of a lane or the one four away), their sign, and the angles
+  int from[2], angle[2];
+  uint64_t sign[2];
+  bool turns[2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = n[i];
+  for (int e = 0; e < 2; e++) {
+    const int d = 8 * C + 4 * e, o = d < half ? d + half : d < 2 * half ? d - half : d;
+    from[e] = o >> 3;
+    turns[e] = d < 2 * half;
+    angle[e] = turns[e] ? cs_at(min(d, o)) : 0;
+    sign[e] = d < half ? f2_pack(-1.f, -1.f) : f2_pack(1.f, 1.f);
+  }
+#pragma unroll 1
+  while (item < items) {
+    const int my_h = h, my_tok = tok, my_kind = kind;
+    float x[8];
+    floats(raw, x);
+    item += kAppendThreads / 32;
+    left += kAppendThreads / 32;
+    if (item < items) {
+      if (RPW * left >= w.n * (kind ? nk : nq)) set_kind();
+      fetch(raw);
     }
-    if (half) {
-      float n[4] = {v[0], v[1], v[2], v[3]};
-      rotate_row<LPR>(n, cs[tok], a.rope.rot, a.rope.interleaved, l);
-      if (kind != 2)
+    if (my_kind == 0 ? a.q_gamma : my_kind == 1 ? a.k_gamma : nullptr) {
+      // RMSNorm.  The order of the sum leaves no trace in the 32-bit factor.
+      double ss = square_sum(x);
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = n[i];
-    }
-    uint32_t n[4];
-    uint16_t scale, zero;
-    quantise(v, n, scale, zero);
-    if (kind == 0) store4(a.q_out + row * a.ldqo + (size_t)head * D + 4 * l, a.vec, v);
-    // key bytes: b1 = 0, 1 of this lane's b0, the other b0 from the next lane;
-    // value bytes: nibble h = 0 here, h = 1 two lanes on
-    const uint32_t kb = n[0] | n[2] << 4 | n[1] << 16 | n[3] << 20, ko = __shfl_xor_sync(0xffffffffu, kb, 1);
-    const uint32_t vn = n[0] | n[1] << 8 | n[2] << 16 | n[3] << 24, vo = __shfl_xor_sync(0xffffffffu, vn, 2);
-    const int c = w.c0 + tok, t = (c >> 1) & 3;
-    uint8_t *blk = img + (size_t)(head - kh0) * BLK;
-    if (kind == 1 && !(l & 1))
-      *reinterpret_cast<uint32_t *>(blk + c * (D / 2) + 4 * (G * ((l >> 1) & 3) + (l >> 3))) = kb | ko << 8;
-    if (kind == 2 && !(l & 2)) {
-      uint8_t *p = blk + 8 * D + 512 * (l >> 4) + 64 * (4 * (l & 1)) + 16 * t + 4 * ((l >> 2) & 3) + 2 * (c & 1) + (c >> 3);
+      for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+      const bool odd_one = !(ss > 0x1p-90 && ss < 0x1p100);  // squares outside what 32 bits hold
+      if (__any_sync(0xffffffffu, odd_one)) {
+        double wide = 0.0;
 #pragma unroll
-      for (int i = 0; i < 4; i++) p[64 * i] = (uint8_t)((vn | vo << 4) >> 8 * i);
+        for (int e = 0; e < 8; e++) wide += (double)x[e] * x[e];
+#pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) wide += __shfl_xor_sync(0xffffffffu, wide, d);
+        ss = odd_one ? wide : ss;
+      }
+      const float rs = rsqrt64(ss * (1.0 / D) + (double)a.eps);
+      const float4 *g = reinterpret_cast<const float4 *>(&gam[my_kind][8 * C]);
+      const uint64_t r2 = f2_pack(rs, rs);
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 u = g[e >> 2];
+        f2_split(f2_mul(f2_mul(f2_pack(x[e], x[e + 1]), r2), f2_pack(u.x, u.y)), x[e], x[e + 1]);
+        f2_split(f2_mul(f2_mul(f2_pack(x[e + 2], x[e + 3]), r2), f2_pack(u.z, u.w)), x[e + 2], x[e + 3]);
+      }
     }
-    if (kind && !(l & 7)) {
-      uint16_t *p = reinterpret_cast<uint16_t *>(blk + 16 * D + 8 * (4 * (4 * (l >> 3) + t) + 2 * (c >> 3) + (c & 1)));
-      *reinterpret_cast<uint32_t *>(p + 2 * (kind - 1)) = scale | (uint32_t)zero << 16;
+    if (my_kind < 2 && half) {
+      // (x0 c - x1 s, x1 c + x0 s), every product and sum rounded by itself, so that a value does
+      // not depend on which of them a compiler fuses
+      const float4 *f = cs + my_tok * CS;
+      if (a.rope.interleaved) {
+        if (8 * C < a.rope.rot)
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            const float4 u = f[cs_at(4 * C + (e >> 1))];
+            const uint64_t c0 = f2_pack(u.x, u.x), s0 = f2_pack(-u.z, u.z), c1 = f2_pack(u.y, u.y), s1 = f2_pack(-u.w, u.w);
+            f2_split(f2_add(f2_mul(f2_pack(x[e], x[e + 1]), c0), f2_mul(f2_pack(x[e + 1], x[e]), s0)), x[e], x[e + 1]);
+            f2_split(f2_add(f2_mul(f2_pack(x[e + 2], x[e + 3]), c1), f2_mul(f2_pack(x[e + 3], x[e + 2]), s1)), x[e + 2],
+                     x[e + 3]);
+          }
+      } else {
+        float z[8];
+        if (half & 4) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) z[e] = __shfl_sync(0xffffffffu, x[e ^ 4], from[e >> 2], LPR);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) z[e] = __shfl_sync(0xffffffffu, x[e], from[0], LPR);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float4 u = f[angle[e >> 2] + 4 * (e >> 1 & 1)];
+          const uint64_t y = f2_add(f2_mul(f2_pack(x[e], x[e + 1]), f2_pack(u.x, u.y)),
+                                    f2_mul(f2_pack(z[e], z[e + 1]), f2_mul(f2_pack(u.z, u.w), sign[e >> 2])));
+          if (turns[e >> 2]) f2_split(y, x[e], x[e + 1]);
+        }
+      }
+    }
+    if (my_kind == 0) {
+      __syncwarp();  // out may be q
+      store8(a.q_out + (size_t)(w.t0 + my_tok) * a.ldqo + (size_t)(qh0 + my_h) * D + 8 * C, a.vec, x);
+      continue;
+    }
+    uint32_t n[8], sz;
+    const uint32_t some = quantise(x, n, sz) ? 0xffffffffu : 0u;
+    const int c = w.c0 + my_tok, t = (c >> 1) & 3, i = C >> 2, odd = l & 1;
+    uint8_t *blk = img + (size_t)my_h * BLK;
+    if (l == 0)
+      *reinterpret_cast<uint32_t *>(blk + 16 * D + 8 * (4 * (4 * i + t) + 2 * (c >> 3) + (c & 1)) + 4 * (my_kind - 1)) = sz;
+    if (my_kind == 1) {
+      const uint32_t word = n[0] + (n[2] << 4) + (n[4] << 8) + (n[6] << 12) + (n[1] << 16) + (n[3] << 20) +
+                            (n[5] << 24) + (n[7] << 28) - kDigit * 0x11111111u;
+      *reinterpret_cast<uint32_t *>(blk + c * (D / 2) + 4 * (G * l + i)) = word & some;
+    } else {
+      // a byte has dims d and d + 8, which are this lane's and its neighbour's: each writes four
+      const uint32_t first = (n[0] + (n[1] << 8) + (n[2] << 16) + (n[3] << 24) - kDigit * 0x01010101u) & some;
+      const uint32_t last = (n[4] + (n[5] << 8) + (n[6] << 16) + (n[7] << 24) - kDigit * 0x01010101u) & some;
+      const uint32_t theirs = __shfl_xor_sync(0xffffffffu, odd ? first : last, 1);
+      const uint32_t bytes = odd ? theirs | last << 4 : first | theirs << 4;
+      uint8_t *p = blk + 8 * D + 512 * (C >> 3) + 256 * odd + 16 * t + 4 * ((C >> 1) & 3) + 2 * (c & 1) + (c >> 3);
+#pragma unroll
+      for (int k = 0; k < 4; k++) p[64 * k] = (uint8_t)(bytes >> 8 * k);
     }
   }
   __syncthreads();
@@ -352,7 +501,7 @@ constexpr int kReadThreads = 256;
 
 template <int D>
 __global__ void __launch_bounds__(kReadThreads) k_kv4_read(const __grid_constant__ Kv4ReadArgs a) {
-  constexpr int LPR = D / 4, RPC = kReadThreads / LPR, G = D / 32, BLK = kv4_block_bytes(D);
+  constexpr int G = D / 32, BLK = kv4_block_bytes(D);
   extern __shared__ __align__(16) uint8_t img[];
   pdl_wait();
   pdl_launch();
@@ -361,38 +510,61 @@ __global__ void __launch_bounds__(kReadThreads) k_kv4_read(const __grid_constant
   const int kh0 = (int)((int64_t)a.c.n_kv * blockIdx.y / a.splits);
   const int nk = (int)((int64_t)a.c.n_kv * (blockIdx.y + 1) / a.splits) - kh0;
   const int page = page_of(a.c, a.b, w.s, w.p);
-  if (page >= 0) {
-    const uint4 *src = reinterpret_cast<const uint4 *>(a.c.pool + ((size_t)page * a.c.n_kv + kh0) * BLK);
-    for (int i = threadIdx.x; i < nk * (BLK / 16); i += kReadThreads) cp_async16(img + 16 * i, src + i, 16);
-    cp_async_commit();
-    cp_async_wait<0>();
-  }
+  const uint4 *src = reinterpret_cast<const uint4 *>(a.c.pool + ((size_t)max(page, 0) * a.c.n_kv + kh0) * BLK);
+  for (int i = threadIdx.x; i < nk * (BLK / 16); i += kReadThreads)
+    cp_async16(img + 16 * i, src + i, page < 0 ? 0 : 16);  // a position that has no page reads as zeros
+  cp_async_commit();
+  cp_async_wait<0>();
   __syncthreads();
-  const int l = threadIdx.x % LPR;
-  for (int r = threadIdx.x / LPR; r < 2 * nk * w.n; r += RPC) {
-    const int is_v = r & 1, hc = r >> 1, tok = hc / nk, h = hc - tok * nk, c = w.c0 + tok, t = (c >> 1) & 3;
-    uint16_t *out = is_v ? a.v : a.k;
-    if (!out) continue;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};  // a position that has no page reads as zeros
-    if (page >= 0) {
+  auto value = [](uint32_t n, uint32_t sz) {
+    return __fadd_rn(__fmul_rn(__uint_as_float(0x4b000000u | n) - 0x1p23f, bf2f(sz & 0xffffu)), __uint_as_float(sz & 0xffff0000u));
+  };
+  if (a.k)  // four threads to a row, the dims as in append
+    for (int x = threadIdx.x; x < 4 * nk * w.n; x += kReadThreads) {
+      const int l = x & 3, r = x >> 2, h = r / w.n, tok = r - h * w.n, c = w.c0 + tok, t = (c >> 1) & 3;
       const uint8_t *blk = img + (size_t)h * BLK;
-      uint32_t n[4];
-      if (!is_v) {
-        const uint8_t *p = blk + c * (D / 2) + 4 * (G * ((l >> 1) & 3) + (l >> 3)) + (l & 1);
-        n[0] = p[0] & 15, n[2] = p[0] >> 4, n[1] = p[2] & 15, n[3] = p[2] >> 4;
+      uint16_t *out = a.k + (size_t)(w.t0 + tok) * a.ldk + (size_t)(kh0 + h) * D + 8 * l;
+      uint32_t keys[G];
+      if constexpr (G == 4) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(blk + c * (D / 2) + 4 * G * l);
+        keys[0] = u.x, keys[1] = u.y, keys[2] = u.z, keys[3] = u.w;
       } else {
-        const uint8_t *p = blk + 8 * D + 512 * (l >> 4) + 64 * (4 * (l & 1)) + 16 * t + 4 * ((l >> 2) & 3) +
-                           2 * (c & 1) + (c >> 3);
-#pragma unroll
-        for (int i = 0; i < 4; i++) n[i] = (p[64 * i] >> 2 * (l & 2)) & 15;
+        const uint2 u = *reinterpret_cast<const uint2 *>(blk + c * (D / 2) + 4 * G * l);
+        keys[0] = u.x, keys[1] = u.y;
       }
-      const uint32_t sz = *reinterpret_cast<const uint32_t *>(
-          blk + 16 * D + 8 * (4 * (4 * (l >> 3) + t) + 2 * (c >> 3) + (c & 1)) + 4 * is_v);
 #pragma unroll
-      for (int i = 0; i < 4; i++) x[i] = __fadd_rn(__fmul_rn((float)n[i], bf2f(sz & 0xffffu)), bf2f(sz >> 16));
+      for (int i = 0; i < G; i++) {
+        const uint32_t sz =
+            *reinterpret_cast<const uint32_t *>(blk + 16 * D + 8 * (4 * (4 * i + t) + 2 * (c >> 3) + (c & 1)));
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = value(keys[i] >> (16 * (e & 1) + 8 * (e >> 2) + 4 * (e >> 1 & 1)) & 15u, sz);
+        store8(out + 32 * i, a.vec, v);
+      }
     }
-    store4(out + (size_t)(w.t0 + tok) * (is_v ? a.ldv : a.ldk) + (size_t)(kh0 + h) * D + 4 * l, a.vec, x);
-  }
+  if (a.v)  // a thread has 16 dims of the four tokens that share its bytes' words
+    for (int x = threadIdx.x; x < nk * (D / 4); x += kReadThreads) {
+      const int m = x % (D / 16), t = x / (D / 16) & 3, h = x / (D / 4);
+      const uint8_t *blk = img + (size_t)h * BLK;
+      uint32_t word[8];
+#pragma unroll
+      for (int g = 0; g < 8; g++)
+        word[g] = *reinterpret_cast<const uint32_t *>(blk + 8 * D + 512 * (m >> 2) + 64 * g + 16 * t + 4 * (m & 3));
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int c = 2 * t + (j & 1) + 8 * (j >> 1), tok = c - w.c0, bit = 8 * (2 * (j & 1) + (j >> 1));
+        if (tok < 0 || tok >= w.n) continue;
+        const uint32_t sz = *reinterpret_cast<const uint32_t *>(blk + 16 * D + 8 * (4 * (4 * (m >> 1) + t) + j) + 4);
+        uint16_t *out = a.v + (size_t)(w.t0 + tok) * a.ldv + (size_t)(kh0 + h) * D + 16 * m;
+        float v[8];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+#pragma unroll
+          for (int g = 0; g < 8; g++) v[g] = value(word[g] >> (bit + 4 * n) & 15u, sz);
+          store8(out + 8 * n, a.vec, v);
+        }
+      }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1197,24 +1369,6 @@ Q3T_DEV void unpack8(uint32_t w, const uint32_t s[2], const uint32_t z[2], uint3
 }
 Q3T_DEV uint32_t lows(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 Q3T_DEV uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
-// pairs of f32
-Q3T_DEV uint64_t f2_pack(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-Q3T_DEV void f2_split(uint64_t d, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
-Q3T_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-Q3T_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 template <int D>
 struct PromptCfg {
   static constexpr int G = D / 32, BLK = kv4_block_bytes(D), ROWS = 256, KEYS = 64, PAGES = KEYS / kKv4Page;
@@ -2020,11 +2174,11 @@ extern "C" q3t_status q3t_kv4_append(const q3t_kv4_cache *cache, const q3t_kv4_b
     const int D = a.c.head_dim, size = rows->dtype == Q3T_F32 ? 4 : 2;
     check_rows(what, "k", rows->k, rows->k_stride, a.c.n_kv, D, size);
     check_rows(what, "v", rows->v, rows->v_stride, a.c.n_kv, D, size);
-    a.vec = wide(rows->k, rows->k_stride, size, 4) && wide(rows->v, rows->v_stride, size, 4);
+    a.vec = wide(rows->k, rows->k_stride, size, 16 / size) && wide(rows->v, rows->v_stride, size, 16 / size);
     if (rows->num_heads) {
       check_rows(what, "q", rows->q, rows->q_stride, rows->num_heads, D, size);
       check_rows(what, "q_out", rows->q_out, rows->q_out_stride, rows->num_heads, D, 2);
-      a.vec = a.vec && wide(rows->q, rows->q_stride, size, 4) && wide(rows->q_out, rows->q_out_stride, 2, 4);
+      a.vec = a.vec && wide(rows->q, rows->q_stride, size, 16 / size) && wide(rows->q_out, rows->q_out_stride, 2, 8);
     }
     a.n_heads = rows->num_heads;
     a.q = rows->q, a.k = rows->k, a.v = rows->v;
@@ -2083,7 +2237,7 @@ extern "C" q3t_status q3t_kv4_read(const q3t_kv4_cache *cache, const q3t_kv4_bat
     if (v) check_rows(what, "v", v, v_stride, a.c.n_kv, a.c.head_dim, 2);
     a.k = k, a.v = v;
     a.ldk = k_stride, a.ldv = v_stride;
-    a.vec = wide(k, k_stride, 2, 4) && wide(v, v_stride, 2, 4);
+    a.vec = wide(k, k_stride, 2, 8) && wide(v, v_stride, 2, 8);
     DeviceScope dev(cache->device);
     CK(kv4_read(a, (cudaStream_t)stream, true));
   });

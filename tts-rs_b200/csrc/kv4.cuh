@@ -50,7 +50,7 @@ struct Kv4AppendArgs {
   float eps;
   uint16_t *q_out;        // bf16 rows
   int64_t ldqo;
-  int vec;                // every row starts on a 4-element boundary
+  int vec;                // every row starts on a 16-byte boundary
   int splits;             // head splits (gridDim.y)
 };
 
@@ -74,7 +74,7 @@ struct Kv4ReadArgs {
   Kv4Batch b;
   uint16_t *k, *v;    // bf16 rows, nullable
   int64_t ldk, ldv;
-  int vec;
+  int vec;            // every row starts on a 16-byte boundary
   int splits;
 };
 
