@@ -227,11 +227,12 @@ Q3T_DEV float max_nan(float a, float b) {
 // two-sum), and every square's, goes into a second sum.  In 32 bits, two at a
 // time: a conversion to 64 costs as much as eight of these.  For sums in
 // 2^-90 .. 2^100; another has squares that 32 bits do not hold.
-Q3T_DEV double square_sum(const float v[8]) {
+template <int E>
+Q3T_DEV double square_sum(const float (&v)[E][8]) {
   uint64_t sum = 0, rest = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const uint64_t x = f2_pack(v[i], v[i + 1]), sq = f2_mul(x, x);
+  for (int i = 0; i < 8 * E; i += 2) {
+    const uint64_t x = f2_pack(v[i >> 3][i & 7], v[i >> 3][(i & 7) + 1]), sq = f2_mul(x, x);
     rest = f2_sub(rest, f2_fma(x, f2_mul(x, 0xbf800000bf800000ull), sq));
     if (i == 0) {
       sum = sq;
@@ -305,15 +306,16 @@ Q3T_DEV bool quantise(const float v[8], uint32_t n[8], uint32_t &scale_zero) {
 // code is four times as long, and a decoding step, which goes through it once,
 // spends its time fetching it: 64 rows took 11.2 us, like this 5.4.)
 // ---------------------------------------------------------------------------
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 256, kAppendDeep = 32;
 
 // {cos, cos, sin, sin} of the pairs f = 32 i + 8 l + e and f + 1, f even, lie in the
 // order [i][e / 2][l]: neighbouring lanes read neighbouring banks
 Q3T_DEV int cs_at(int f) { return (((f >> 5) << 2) + ((f >> 1) & 3)) * 4 + ((f >> 3) & 3); }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
-  constexpr int LPR = D / 8, RPW = 32 / LPR, G = D / 32, BLK = kv4_block_bytes(D), CS = D / 4 + 4;
+template <typename T, int D, int E>
+__global__ void __launch_bounds__(kAppendThreads, E == 1 ? 4 : E == 2 ? 3 : 2) k_kv4_append(const __grid_constant__ Kv4AppendArgs a) {
+  constexpr int LPR = D / 8 / E, RPW = 32 / LPR, G = D / 32, BLK = kv4_block_bytes(D), CS = D / 4 + 4;
+  static_assert(E == 1 || E == G);
   extern __shared__ __align__(16) uint8_t img[];  // [kv heads of this split][BLK]
   __shared__ float4 cs[kKv4Page * CS];
   __shared__ __align__(16) float gam[2][D];
@@ -336,15 +338,16 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
     kind = item < q_items ? 0 : item < q_items + k_items ? 1 : 2;
     left = item - (kind == 0 ? 0 : kind == 1 ? q_items : q_items + k_items);
     ld = kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv;
-    base = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + w.t0 * ld + (kind ? kh0 : qh0) * D + 8 * C;
+    base = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + w.t0 * ld + (kind ? kh0 : qh0) * D + 8 * C;  // its first eight
   };
-  auto fetch = [&](Raw8<T> &x) {
+  auto fetch = [&](Raw8<T> (&x)[E]) {
     const int r = min(RPW * left + lane / LPR, w.n * (kind ? nk : nq) - 1);  // a row past the end repeats the last one
     h = w.n == 1 ? r : (int)__umulhi((uint32_t)r, inv_n);
     tok = r - h * w.n;
-    load8(base + tok * ld + h * D, a.vec, x);
+#pragma unroll
+    for (int i = 0; i < E; i++) load8(base + tok * ld + h * D + 32 * i, a.vec, x[i]);
   };
-  Raw8<T> raw = {};
+  Raw8<T> raw[E] = {};
   set_kind();
   if (item < items) fetch(raw);
   const int page = page_of(a.c, a.b, w.s, w.p), half = a.rope.rot / 2;
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
     if (g) gam[i / D][i % D] = g[i % D];
   }
   __syncthreads();
-  // of the rotation by halves, for dims 8 C .. + 3 and + 4 .. + 7: where the others of their pairs are (rot % 8 ==
+  // of the rotation by halves (E == 1), for dims 8 C .. + 3 and + 4 .. + 7: where the others of their pairs are (rot % 8 ==
   // 0, so the same element of a lane or the one four away), their sign, and the angles
   int from[2], angle[2];
   uint64_t sign[2];
@@ -377,8 +380,9 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
 #pragma unroll 1
   while (item < items) {
     const int my_h = h, my_tok = tok, my_kind = kind;
-    float x[8];
-    floats(raw, x);
+    float x[E][8];
+#pragma unroll
+    for (int i = 0; i < E; i++) floats(raw[i], x[i]);
     item += kAppendThreads / 32;
     left += kAppendThreads / 32;
     if (item < items) {
@@ -394,19 +398,19 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
       if (__any_sync(0xffffffffu, odd_one)) {
         double wide = 0.0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) wide += (double)x[e] * x[e];
+        for (int e = 0; e < 8 * E; e++) wide += (double)x[e >> 3][e & 7] * x[e >> 3][e & 7];
 #pragma unroll
         for (int d = 1; d < LPR; d <<= 1) wide += __shfl_xor_sync(0xffffffffu, wide, d);
         ss = odd_one ? wide : ss;
       }
       const float rs = rsqrt64(ss * (1.0 / D) + (double)a.eps);
-      const float4 *g = reinterpret_cast<const float4 *>(&gam[my_kind][8 * C]);
       const uint64_t r2 = f2_pack(rs, rs);
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const float4 u = g[e >> 2];
-        f2_split(f2_mul(f2_mul(f2_pack(x[e], x[e + 1]), r2), f2_pack(u.x, u.y)), x[e], x[e + 1]);
-        f2_split(f2_mul(f2_mul(f2_pack(x[e + 2], x[e + 3]), r2), f2_pack(u.z, u.w)), x[e + 2], x[e + 3]);
+      for (int e = 0; e < 8 * E; e += 4) {
+        const float4 u = *reinterpret_cast<const float4 *>(&gam[my_kind][8 * C + 32 * (e >> 3) + (e & 7)]);
+        float *y = &x[e >> 3][e & 7];
+        f2_split(f2_mul(f2_mul(f2_pack(y[0], y[1]), r2), f2_pack(u.x, u.y)), y[0], y[1]);
+        f2_split(f2_mul(f2_mul(f2_pack(y[2], y[3]), r2), f2_pack(u.z, u.w)), y[2], y[3]);
       }
     }
     if (my_kind < 2 && half) {
@@ -414,57 +418,80 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_kv4_append(const __grid_c
       // not depend on which of them a compiler fuses
       const float4 *f = cs + my_tok * CS;
       if (a.rope.interleaved) {
-        if (8 * C < a.rope.rot)
 #pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            const float4 u = f[cs_at(4 * C + (e >> 1))];
-            const uint64_t c0 = f2_pack(u.x, u.x), s0 = f2_pack(-u.z, u.z), c1 = f2_pack(u.y, u.y), s1 = f2_pack(-u.w, u.w);
-            f2_split(f2_add(f2_mul(f2_pack(x[e], x[e + 1]), c0), f2_mul(f2_pack(x[e + 1], x[e]), s0)), x[e], x[e + 1]);
-            f2_split(f2_add(f2_mul(f2_pack(x[e + 2], x[e + 3]), c1), f2_mul(f2_pack(x[e + 3], x[e + 2]), s1)), x[e + 2],
-                     x[e + 3]);
-          }
-      } else {
+        for (int i = 0; i < E; i++)
+          if (8 * C + 32 * i < a.rope.rot)
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+              const float4 u = f[cs_at(4 * C + 16 * i + (e >> 1))];
+              float *y = &x[i][e];
+              const uint64_t c0 = f2_pack(u.x, u.x), s0 = f2_pack(-u.z, u.z), c1 = f2_pack(u.y, u.y), s1 = f2_pack(-u.w, u.w);
+              f2_split(f2_add(f2_mul(f2_pack(y[0], y[1]), c0), f2_mul(f2_pack(y[1], y[0]), s0)), y[0], y[1]);
+              f2_split(f2_add(f2_mul(f2_pack(y[2], y[3]), c1), f2_mul(f2_pack(y[3], y[2]), s1)), y[2], y[3]);
+            }
+      } else if constexpr (E == 1) {
         float z[8];
         if (half & 4) {
 #pragma unroll
-          for (int e = 0; e < 8; e++) z[e] = __shfl_sync(0xffffffffu, x[e ^ 4], from[e >> 2], LPR);
+          for (int e = 0; e < 8; e++) z[e] = __shfl_sync(0xffffffffu, x[0][e ^ 4], from[e >> 2], LPR);
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; e++) z[e] = __shfl_sync(0xffffffffu, x[e], from[0], LPR);
+          for (int e = 0; e < 8; e++) z[e] = __shfl_sync(0xffffffffu, x[0][e], from[0], LPR);
         }
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const float4 u = f[angle[e >> 2] + 4 * (e >> 1 & 1)];
-          const uint64_t y = f2_add(f2_mul(f2_pack(x[e], x[e + 1]), f2_pack(u.x, u.y)),
+          const uint64_t y = f2_add(f2_mul(f2_pack(x[0][e], x[0][e + 1]), f2_pack(u.x, u.y)),
                                     f2_mul(f2_pack(z[e], z[e + 1]), f2_mul(f2_pack(u.z, u.w), sign[e >> 2])));
-          if (turns[e >> 2]) f2_split(y, x[e], x[e + 1]);
+          if (turns[e >> 2]) f2_split(y, x[0][e], x[0][e + 1]);
+        }
+      } else {  // of a whole row: both of a pair are this lane's
+#pragma unroll
+        for (int e = 0; e < 4 * E; e += 2) {
+          float *lo = &x[e >> 3][e & 7], *hi = &x[(e >> 3) + E / 2][e & 7];
+          const float4 u = f[(4 * (e >> 3) + ((e & 7) >> 1)) * 4 + l];
+          const uint64_t x0 = f2_pack(lo[0], lo[1]), x1 = f2_pack(hi[0], hi[1]), cc = f2_pack(u.x, u.y), ss = f2_pack(u.z, u.w);
+          f2_split(f2_sub(f2_mul(x0, cc), f2_mul(x1, ss)), lo[0], lo[1]);
+          f2_split(f2_add(f2_mul(x1, cc), f2_mul(x0, ss)), hi[0], hi[1]);
         }
       }
     }
     if (my_kind == 0) {
       __syncwarp();  // out may be q
-      store8(a.q_out + (size_t)(w.t0 + my_tok) * a.ldqo + (size_t)(qh0 + my_h) * D + 8 * C, a.vec, x);
+      uint16_t *out = a.q_out + (size_t)(w.t0 + my_tok) * a.ldqo + (size_t)(qh0 + my_h) * D + 8 * C;
+#pragma unroll
+      for (int i = 0; i < E; i++) store8(out + 32 * i, a.vec, x[i]);
       continue;
     }
-    uint32_t n[8], sz;
-    const uint32_t some = quantise(x, n, sz) ? 0xffffffffu : 0u;
-    const int c = w.c0 + my_tok, t = (c >> 1) & 3, i = C >> 2, odd = l & 1;
+    const int c = w.c0 + my_tok, t = (c >> 1) & 3, odd = l & 1;
     uint8_t *blk = img + (size_t)my_h * BLK;
-    if (l == 0)
-      *reinterpret_cast<uint32_t *>(blk + 16 * D + 8 * (4 * (4 * i + t) + 2 * (c >> 3) + (c & 1)) + 4 * (my_kind - 1)) = sz;
-    if (my_kind == 1) {
-      const uint32_t word = n[0] + (n[2] << 4) + (n[4] << 8) + (n[6] << 12) + (n[1] << 16) + (n[3] << 20) +
-                            (n[5] << 24) + (n[7] << 28) - kDigit * 0x11111111u;
-      *reinterpret_cast<uint32_t *>(blk + c * (D / 2) + 4 * (G * l + i)) = word & some;
-    } else {
-      // a byte has dims d and d + 8, which are this lane's and its neighbour's: each writes four
-      const uint32_t first = (n[0] + (n[1] << 8) + (n[2] << 16) + (n[3] << 24) - kDigit * 0x01010101u) & some;
-      const uint32_t last = (n[4] + (n[5] << 8) + (n[6] << 16) + (n[7] << 24) - kDigit * 0x01010101u) & some;
-      const uint32_t theirs = __shfl_xor_sync(0xffffffffu, odd ? first : last, 1);
-      const uint32_t bytes = odd ? theirs | last << 4 : first | theirs << 4;
-      uint8_t *p = blk + 8 * D + 512 * (C >> 3) + 256 * odd + 16 * t + 4 * ((C >> 1) & 3) + 2 * (c & 1) + (c >> 3);
+    uint32_t keys[E];
 #pragma unroll
-      for (int k = 0; k < 4; k++) p[64 * k] = (uint8_t)(bytes >> 8 * k);
+    for (int j = 0; j < E; j++) {
+      const int i = E == 1 ? C >> 2 : j, ch = E == 1 ? C : 4 * j + l;  // group of 32, eight dims
+      uint32_t n[8], sz;
+      const uint32_t some = quantise(x[j], n, sz) ? 0xffffffffu : 0u;
+      if (l == 0)
+        *reinterpret_cast<uint32_t *>(blk + 16 * D + 8 * (4 * (4 * i + t) + 2 * (c >> 3) + (c & 1)) + 4 * (my_kind - 1)) = sz;
+      if (my_kind == 1) {
+        keys[j] = (n[0] + (n[2] << 4) + (n[4] << 8) + (n[6] << 12) + (n[1] << 16) + (n[3] << 20) + (n[5] << 24) +
+                   (n[7] << 28) - kDigit * 0x11111111u) & some;
+        if (E == 1) *reinterpret_cast<uint32_t *>(blk + c * (D / 2) + 4 * (G * l + i)) = keys[j];
+      } else {
+        // a byte has dims d and d + 8, which are this lane's and its neighbour's: each writes four
+        const uint32_t first = (n[0] + (n[1] << 8) + (n[2] << 16) + (n[3] << 24) - kDigit * 0x01010101u) & some;
+        const uint32_t last = (n[4] + (n[5] << 8) + (n[6] << 16) + (n[7] << 24) - kDigit * 0x01010101u) & some;
+        const uint32_t theirs = __shfl_xor_sync(0xffffffffu, odd ? first : last, 1);
+        const uint32_t bytes = odd ? theirs | last << 4 : first | theirs << 4;
+        uint8_t *p = blk + 8 * D + 512 * (ch >> 3) + 256 * odd + 16 * t + 4 * ((ch >> 1) & 3) + 2 * (c & 1) + (c >> 3);
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[64 * k] = (uint8_t)(bytes >> 8 * k);
+      }
+    }
+    if (E > 1 && my_kind == 1) {
+      uint8_t *p = blk + c * (D / 2) + 4 * G * l;
+      if constexpr (E == 4) *reinterpret_cast<uint4 *>(p) = make_uint4(keys[0], keys[1], keys[2], keys[3]);
+      if constexpr (E == 2) *reinterpret_cast<uint2 *>(p) = make_uint2(keys[0], keys[1]);
     }
   }
   __syncthreads();
@@ -1902,16 +1929,16 @@ int head_splits(int windows, int n_kv) {
   return s < n_kv ? s : n_kv;
 }
 
-template <typename T, int D>
+template <typename T, int D, int E>
 cudaError_t append_launch(const Kv4AppendArgs &a, int windows, cudaStream_t st, bool pdl) {
   static std::atomic<uint64_t> done{0};
   const int per = (a.c.n_kv + a.splits - 1) / a.splits;
   const size_t smem = (size_t)per * kv4_block_bytes(D);
   cudaError_t e = once_per_device(done, [] {
-    return cudaFuncSetAttribute(k_kv4_append<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 << 10);
+    return cudaFuncSetAttribute(k_kv4_append<T, D, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 << 10);
   });
   if (e != cudaSuccess) return e;
-  return launch(k_kv4_append<T, D>, dim3(windows, a.splits), kAppendThreads, smem, 1, pdl, st, a);
+  return launch(k_kv4_append<T, D, E>, dim3(windows, a.splits), kAppendThreads, smem, 1, pdl, st, a);
 }
 
 template <int D>
@@ -1964,9 +1991,17 @@ cudaError_t kv4_append(const Kv4AppendArgs &a0, bool f32_rows, cudaStream_t st, 
   a.splits = head_splits(windows, a.c.n_kv);
   // a split's blocks have to fit shared memory
   while ((size_t)((a.c.n_kv + a.splits - 1) / a.splits) * kv4_block_bytes(a.c.head_dim) > (40 << 10)) a.splits++;
+  // a whole group to a lane where prompts fill their pages
+  const bool deep = a.b.num_tokens >= kAppendDeep * a.b.num_seqs &&
+                    (a.rope.rot == 0 || a.rope.interleaved || a.rope.rot == a.c.head_dim);
+  auto go = [&](auto t, auto d) {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value;
+    return deep ? append_launch<T, D, D / 32>(a, windows, st, pdl) : append_launch<T, D, 1>(a, windows, st, pdl);
+  };
   if (a.c.head_dim == 128)
-    return f32_rows ? append_launch<float, 128>(a, windows, st, pdl) : append_launch<uint16_t, 128>(a, windows, st, pdl);
-  return f32_rows ? append_launch<float, 64>(a, windows, st, pdl) : append_launch<uint16_t, 64>(a, windows, st, pdl);
+    return f32_rows ? go(0.f, std::integral_constant<int, 128>{}) : go((uint16_t)0, std::integral_constant<int, 128>{});
+  return f32_rows ? go(0.f, std::integral_constant<int, 64>{}) : go((uint16_t)0, std::integral_constant<int, 64>{});
 }
 
 cudaError_t kv4_read(const Kv4ReadArgs &a0, cudaStream_t st, bool pdl) {
