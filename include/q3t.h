@@ -635,7 +635,7 @@ q3t_status q3t_kv4_append(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch
  * alone uses while it runs (calls that may overlap, and graphs that may replay
  * at once, need one each); it needs no initialisation and holds nothing
  * between calls.  64 KiB at least; Q3T_KV4_WORKSPACE serves the widest launch. */
-#define Q3T_KV4_WORKSPACE (4 << 20)
+#define Q3T_KV4_WORKSPACE (20 << 20)
 q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, int num_heads, const uint16_t *q,
                           int64_t q_stride, float scale, int window, uint16_t *out, int64_t out_stride,
                           void *workspace, int64_t workspace_bytes, void *stream);

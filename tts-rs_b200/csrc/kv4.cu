@@ -1396,10 +1396,27 @@ Q3T_DEV void unpack8(uint32_t w, const uint32_t s[2], const uint32_t z[2], uint3
 }
 Q3T_DEV uint32_t lows(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
 Q3T_DEV uint32_t highs(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+// How the key axis is divided: by `most` in all, as many CTAs to each of the
+// call's `tiles` (of all kv heads) as the grid and the workspace have.
+struct PromptSplit {
+  int thr;    // sequences of more rows than this
+  int most;   // 1: not divided
+  float *parts;  // [CTA] m[256], l[256], o[D / 4][256][4]
+};
+template <typename F>
+Q3T_DEV int split_count(const PromptSplit &sp, int num_seqs, int n_kv, F count) {
+  if (sp.most <= 1) return 1;
+  int tiles = 0;
+  for (int q = threadIdx.x & 31; q < num_seqs; q += 32) tiles += count(q);
+  tiles = max(__reduce_add_sync(0xffffffffu, tiles), 1);
+  return max(1, min(32, sp.most / (tiles * n_kv)));
+}
+
 template <int D>
 struct PromptCfg {
   static constexpr int G = D / 32, BLK = kv4_block_bytes(D), ROWS = 256, KEYS = 64, PAGES = KEYS / kKv4Page;
   static constexpr int THREADS = 20 * 32;
+  static constexpr int PART = ROWS * (D + 2);  // floats
   static constexpr int QB = 128 * D * 2, KB = KEYS * D * 2, VB = D * KEYS * 2, PB = 128 * KEYS * 2;
   static constexpr int SC = PAGES * 2 * D;  // a tile's scales and zeros of K, or of V
   static constexpr int ST = 3, RING = 12 * D;  // blocks on their way to an unpacking warp: digits, scale entries
@@ -1408,7 +1425,7 @@ struct PromptCfg {
 };
 
 template <int D>
-__global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const __grid_constant__ Kv4AttendArgs a, int thr) {
+__global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const __grid_constant__ Kv4AttendArgs a, PromptSplit ks) {
   using Cfg = PromptCfg<D>;
   constexpr int G = Cfg::G, BLK = Cfg::BLK, ROWS = Cfg::ROWS, KEYS = Cfg::KEYS, PAGES = Cfg::PAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -1436,26 +1453,32 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     fence_mbar_init();
     if (lane == 0) dead = 0;
   }
+  auto tiles_of = [&](int q) {
+    int t0, n, pos0;
+    seq_rows(a.b, q, t0, n, pos0);
+    return n * gq > ks.thr ? (n * gq + ROWS - 1) / ROWS : 0;
+  };
+  const int splits = split_count(ks, a.b.num_seqs, n_kv, tiles_of), split = blockIdx.x / n_kv % splits;
   int s, i_rev;
-  if (!find_item(
-          a.b.num_seqs, blockIdx.x / n_kv,
-          [&](int q) {
-            int t0, n, pos0;
-            seq_rows(a.b, q, t0, n, pos0);
-            return n * gq > thr ? (n * gq + ROWS - 1) / ROWS : 0;
-          },
-          s, i_rev))
-    return;
+  if (!find_item(a.b.num_seqs, blockIdx.x / n_kv / splits, tiles_of, s, i_rev)) return;
   int t0, n, pos0;
   seq_rows(a.b, s, t0, n, pos0);
   const int total = n * gq, row0 = ((total + ROWS - 1) / ROWS - 1 - i_rev) * ROWS;  // the longest tiles first
   const int nrow = min(ROWS, total - row0);
   const int pos_lo = pos0 + row0 / gq, pos_hi = pos0 + (row0 + nrow - 1) / gq;
-  const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0, pg_lo = key_lo >> 4;
+  const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+  int pg_lo = key_lo >> 4;
   // tiles of keys that the first 128 rows see, and the others; both begin at page pg_lo
   auto tiles_to = [&](int pos) { return pos < 0 ? 0 : max(0, ((pos >> 4) + 1 - pg_lo + PAGES - 1) / PAGES); };
-  const int nt0 = tiles_to(pos0 + (row0 + min(nrow, 128) - 1) / gq), nt1 = nrow > 128 ? tiles_to(pos_hi) : 0;
-  const int n_tiles = max(nt0, nt1), n_pages = pos_hi < 0 ? 0 : max(0, (pos_hi >> 4) + 1 - pg_lo);
+  int nt0 = tiles_to(pos0 + (row0 + min(nrow, 128) - 1) / gq), nt1 = nrow > 128 ? tiles_to(pos_hi) : 0;
+  int n_tiles = max(nt0, nt1), n_pages = pos_hi < 0 ? 0 : max(0, (pos_hi >> 4) + 1 - pg_lo);
+  if (splits > 1) {  // this CTA's tiles of keys, four at least
+    const int per = max(4, (n_tiles + splits - 1) / splits), skip = split * per;
+    nt0 = max(0, min(nt0 - skip, per)), nt1 = max(0, min(nt1 - skip, per));
+    n_tiles = max(nt0, nt1);
+    pg_lo += skip * PAGES;
+    n_pages = max(0, min(n_pages - skip * PAGES, per * PAGES));
+  }
 
   if (warp == 16) tmem_alloc(&tmem_slot, 512);
   tc_fence_before();
@@ -1825,6 +1848,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     tc_fence_after();
     const bool gone = *(volatile int *)&dead;
     const float up = exp2f((float)max(e_ref, -126)), inv = l == 0.f ? 0.f : 1.f / l;
+    float *part = splits > 1 ? ks.parts + (size_t)blockIdx.x * Cfg::PART + threadIdx.x : nullptr;
+    if (part) part[0] = m, part[ROWS] = l;
 #pragma unroll 1
     for (int c = 0; c < D / 32; c++) {
       uint32_t x[32];
@@ -1838,6 +1863,14 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       }
       const bool is_nan = gone || (nan >> 7 & 1) || (nan >> c & 1);
       const float f1 = is_nan ? __uint_as_float(0x7fc00000u) : inv;
+      if (part) {
+        float4 *to = reinterpret_cast<float4 *>(part - threadIdx.x + 2 * ROWS) + threadIdx.x;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+          to[(8 * c + k) * ROWS] = make_float4(__uint_as_float(x[4 * k]) * f1 * up, __uint_as_float(x[4 * k + 1]) * f1 * up,
+                                               __uint_as_float(x[4 * k + 2]) * f1 * up, __uint_as_float(x[4 * k + 3]) * f1 * up);
+        continue;
+      }
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         uint32_t y[4];
@@ -1850,7 +1883,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     __syncwarp();
     const int c = lane % LPR, k0 = lane / LPR;
     const long long mine = (long long)((size_t)(t0 + tok) * a.ldo + (size_t)hd * D);
-    if (a.vec) {
+    if (part) {
+      // k_kv4_join has the rest
+    } else if (a.vec) {
 #pragma unroll 8
       for (int k = 0; k < 32; k += RPS) {
         const uint4 u = *q_at(32 * warp + k0 + k, c);
@@ -1875,6 +1910,59 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of k_kv4_prompt's tiles, where it divided the keys: a thread
+// has a row, 32 dims of it.  A part's o is divided by its l already, so a part
+// weighs l 2^m; parts come in order, and the result does not depend on timing.
+template <int D>
+__global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4AttendArgs a, PromptSplit sp) {
+  using Cfg = PromptCfg<D>;
+  constexpr int ROWS = Cfg::ROWS;
+  pdl_wait();
+  pdl_launch();
+  const int n_kv = a.c.n_kv, gq = a.n_heads / n_kv, kvh = blockIdx.x % n_kv, r = threadIdx.x, d0 = 32 * blockIdx.y;
+  auto tiles_of = [&](int q) {
+    int t0, n, pos0;
+    seq_rows(a.b, q, t0, n, pos0);
+    return n * gq > sp.thr ? (n * gq + ROWS - 1) / ROWS : 0;
+  };
+  const int splits = split_count(sp, a.b.num_seqs, n_kv, tiles_of);
+  if (splits == 1) return;
+  int s, i_rev;
+  if (!find_item(a.b.num_seqs, blockIdx.x / n_kv, tiles_of, s, i_rev)) return;
+  int t0, n, pos0;
+  seq_rows(a.b, s, t0, n, pos0);
+  const int total = n * gq, row0 = ((total + ROWS - 1) / ROWS - 1 - i_rev) * ROWS, flat = row0 + r, tok = flat / gq;
+  if (flat >= total) return;
+  const float *part = sp.parts + (size_t)(blockIdx.x / n_kv * splits * n_kv + kvh) * Cfg::PART + r;
+  const size_t step = (size_t)n_kv * Cfg::PART;
+  float M = -INFINITY, L = 0.f;
+  for (int k = 0; k < splits; k++) M = fmaxf(M, part[k * step]);
+  float o[32] = {};
+  for (int k = 0; k < splits; k++) {
+    const float *p = part + k * step;
+    const float l = p[ROWS], w = l == 0.f ? 0.f : l * ex2(p[0] - M);
+    const float4 *from = reinterpret_cast<const float4 *>(p - r + 2 * ROWS) + r + (size_t)(d0 / 4) * ROWS;
+    L += w;
+    float4 u[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) u[i] = from[i * ROWS];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      o[4 * i] = fmaf(w, u[i].x, o[4 * i]), o[4 * i + 1] = fmaf(w, u[i].y, o[4 * i + 1]);
+      o[4 * i + 2] = fmaf(w, u[i].z, o[4 * i + 2]), o[4 * i + 3] = fmaf(w, u[i].w, o[4 * i + 3]);
+    }
+  }
+  const float inv = L == 0.f ? 1.f : 1.f / L;  // (a row that sees no key: 0, or NaN where a wait gave up)
+  uint16_t *out = a.out + (size_t)(t0 + tok) * a.ldo + (size_t)(kvh * gq + flat - tok * gq) * D + d0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = o[i + e] * inv;
+    store8(out + i, a.vec, v);
   }
 }
 
@@ -2014,19 +2102,30 @@ cudaError_t kv4_read(const Kv4ReadArgs &a0, cudaStream_t st, bool pdl) {
 }
 
 template <int D>
-static cudaError_t prompt_launch(const Kv4AttendArgs &a, int thr, cudaStream_t st, bool pdl) {
+static cudaError_t prompt_launch(const Kv4AttendArgs &a, int thr, void *ws, int64_t ws_bytes, cudaStream_t st, bool pdl) {
   using Cfg = PromptCfg<D>;
   static std::atomic<uint64_t> done{0};
+  static std::atomic<int> sms{0};
   cudaError_t e = once_per_device(done, [] {
-    return cudaFuncSetAttribute(k_kv4_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::kSmem);
+    int dev = 0, n = 0;
+    cudaError_t r = cudaFuncSetAttribute(k_kv4_prompt<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::kSmem);
+    if (r == cudaSuccess) r = cudaGetDevice(&dev);
+    if (r == cudaSuccess) r = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (r == cudaSuccess) sms.store(n);
+    return r;
   });
   if (e != cudaSuccess) return e;
   // tiles, at most: whole ones, and one more for every sequence that has over thr rows
   const int64_t rows = (int64_t)a.b.num_tokens * (a.n_heads / a.c.n_kv);
-  const int64_t tiles = rows / Cfg::ROWS + std::min<int64_t>(a.b.num_seqs, rows / (thr + 1));
-  const int64_t grid = std::min<int64_t>(tiles, rows) * a.c.n_kv;
+  const int64_t tiles = std::min<int64_t>(rows / Cfg::ROWS + std::min<int64_t>(a.b.num_seqs, rows / (thr + 1)), rows);
+  // where these cannot fill the GPU, CTAs share the keys of each
+  const int64_t fit = std::min<int64_t>(sms.load(), ws_bytes / (4 * Cfg::PART));
+  const int64_t grid = std::max<int64_t>(tiles * a.c.n_kv, fit);
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  return launch(k_kv4_prompt<D>, dim3((unsigned)grid), Cfg::THREADS, Cfg::kSmem, 1, pdl, st, a, thr);
+  const PromptSplit sp = {thr, tiles * a.c.n_kv < fit ? (int)fit : 1, (float *)ws};
+  e = launch(k_kv4_prompt<D>, dim3((unsigned)grid), Cfg::THREADS, Cfg::kSmem, 1, pdl, st, a, sp);
+  if (e != cudaSuccess || sp.most == 1) return e;
+  return launch(k_kv4_join<D>, dim3((unsigned)(tiles * a.c.n_kv), D / 32), 256, 0, 1, false, st, a, sp);
 }
 
 cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st,
@@ -2040,7 +2139,8 @@ cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws,
   const bool mostly_big = some_big && (int64_t)a.b.num_tokens * gq > (int64_t)kBig * a.b.num_seqs;
   if (some_big) {
     const int thr = mostly_big ? 0 : kBig;
-    const cudaError_t e = a.c.head_dim == 128 ? prompt_launch<128>(a, thr, st, pdl) : prompt_launch<64>(a, thr, st, pdl);
+    const cudaError_t e = a.c.head_dim == 128 ? prompt_launch<128>(a, thr, ws, ws_bytes, st, pdl)
+                                                   : prompt_launch<64>(a, thr, ws, ws_bytes, st, pdl);
     if (e != cudaSuccess || mostly_big) return e;
     a.big = kBig;
   }

@@ -91,7 +91,7 @@ struct Kv4Step {
 // returned; `pdl` lets the launch overlap the tail of the one before it.
 cudaError_t kv4_append(const Kv4AppendArgs &a, bool f32_rows, cudaStream_t st, bool pdl);
 // attend needs a workspace: 64 KiB at least, kKv4Workspace for the widest launch.
-constexpr int64_t kKv4Workspace = 4 << 20;
+constexpr int64_t kKv4Workspace = 20 << 20;
 cudaError_t kv4_attend(const Kv4AttendArgs &a, int max_q, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st,
                        bool pdl);
 cudaError_t kv4_read(const Kv4ReadArgs &a, cudaStream_t st, bool pdl);

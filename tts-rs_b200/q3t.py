@@ -867,7 +867,7 @@ class Batch:
 # 4-bit paged key/value cache on torch CUDA tensors (q3t_kv4_*).  Calls run on
 # torch's current stream of the cache's device and return without waiting.
 # ---------------------------------------------------------------------------
-KV4_WORKSPACE = 4 << 20  # Q3T_KV4_WORKSPACE
+KV4_WORKSPACE = 20 << 20  # Q3T_KV4_WORKSPACE
 
 
 def _bad(message):
