@@ -1478,6 +1478,13 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     n_tiles = max(nt0, nt1);
     pg_lo += skip * PAGES;
     n_pages = max(0, min(n_pages - skip * PAGES, per * PAGES));
+    if (n_tiles == 0) {  // nothing left for it
+      if ((int)threadIdx.x < nrow) {
+        float *part = ks.parts + (size_t)blockIdx.x * Cfg::PART + threadIdx.x;
+        part[0] = -INFINITY, part[ROWS] = 0.f;
+      }
+      return;
+    }
   }
 
   if (warp == 16) tmem_alloc(&tmem_slot, 512);
@@ -1849,7 +1856,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     const bool gone = *(volatile int *)&dead;
     const float up = exp2f((float)max(e_ref, -126)), inv = l == 0.f ? 0.f : 1.f / l;
     float *part = splits > 1 ? ks.parts + (size_t)blockIdx.x * Cfg::PART + threadIdx.x : nullptr;
-    if (part) part[0] = m, part[ROWS] = l;
+    const bool in_tile = (int)threadIdx.x < nrow;
+    if (part && in_tile) part[0] = m, part[ROWS] = gone ? __uint_as_float(0x7fc00000u) : l;
 #pragma unroll 1
     for (int c = 0; c < D / 32; c++) {
       uint32_t x[32];
@@ -1867,7 +1875,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         float4 *to = reinterpret_cast<float4 *>(part - threadIdx.x + 2 * ROWS) + threadIdx.x;
 #pragma unroll
         for (int k = 0; k < 8; k++)
-          to[(8 * c + k) * ROWS] = make_float4(__uint_as_float(x[4 * k]) * f1 * up, __uint_as_float(x[4 * k + 1]) * f1 * up,
+          if (in_tile) to[(8 * c + k) * ROWS] = make_float4(__uint_as_float(x[4 * k]) * f1 * up, __uint_as_float(x[4 * k + 1]) * f1 * up,
                                                __uint_as_float(x[4 * k + 2]) * f1 * up, __uint_as_float(x[4 * k + 3]) * f1 * up);
         continue;
       }
@@ -1943,7 +1951,8 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
   float o[32] = {};
   for (int k = 0; k < splits; k++) {
     const float *p = part + k * step;
-    const float l = p[ROWS], w = l == 0.f ? 0.f : l * ex2(p[0] - M);
+    const float l = p[ROWS], w = l * ex2(p[0] - M);
+    if (l == 0.f) continue;  // no key of it
     const float4 *from = reinterpret_cast<const float4 *>(p - r + 2 * ROWS) + r + (size_t)(d0 / 4) * ROWS;
     L += w;
     float4 u[8];
@@ -1955,7 +1964,7 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
       o[4 * i + 2] = fmaf(w, u[i].z, o[4 * i + 2]), o[4 * i + 3] = fmaf(w, u[i].w, o[4 * i + 3]);
     }
   }
-  const float inv = L == 0.f ? 1.f : 1.f / L;  // (a row that sees no key: 0, or NaN where a wait gave up)
+  const float inv = L == 0.f ? 0.f : 1.f / L;
   uint16_t *out = a.out + (size_t)(t0 + tok) * a.ldo + (size_t)(kvh * gq + flat - tok * gq) * D + d0;
 #pragma unroll
   for (int i = 0; i < 32; i += 8) {
