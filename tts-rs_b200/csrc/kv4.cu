@@ -2280,8 +2280,11 @@ void rope_freqs(const char *what, const q3t_rope *r, double *freqs) {
   if (r->scaling == Q3T_ROPE_BANDS && (!(r->low < r->high) || !std::isfinite(r->low) || !std::isfinite(r->high) ||
                                        r->original < 1))
     FAIL(Q3T_INVALID_INPUT, "%s: band scaling needs low < high and original > 0", what);
-  for (int i = 0; i < rot / 2; i++) {
-    double f = std::pow((double)r->theta, -2.0 * i / rot);
+  // theta^(-2 i / rot) step by step in 80 bits: 64 steps are off by 2^-57, and 64 powers would be 2 us of every append
+  const long double step = rot ? std::pow((long double)r->theta, -2.0L / rot) : 1.0L;
+  long double power = 1.0L;
+  for (int i = 0; i < rot / 2; i++, power *= step) {
+    double f = (double)power;
     if (r->scaling == Q3T_ROPE_LINEAR) f /= r->factor;
     if (r->scaling == Q3T_ROPE_BANDS) {
       const double turns = r->original * f / (2.0 * M_PI);

@@ -917,7 +917,7 @@ class KV4Batch:
             _bad("KV4Batch: kv_len must be on a CUDA device")
         if q_start.shape[0] != n + 1 or (table_row is not None and table_row.shape[0] != n):
             _bad(f"KV4Batch: q_start needs {n + 1} entries, and table_row {n}, for {n} sequences")
-        self.device, self.tokens = dev, int(num_tokens)
+        self.device, self.index, self.tokens = dev, dev.index, int(num_tokens)
         self.view = KV4BatchView(n, self.tokens, int(max_q), int(max_kv), _int32(q_start, "q_start", dev, 1),
                                  _int32(kv_len, "kv_len", dev, 1),
                                  None if table_row is None else _int32(table_row, "table_row", dev, 1))
@@ -935,6 +935,7 @@ class KV4Cache:
                 tuple(pool.shape[1:]) != (num_kv_heads, 20 * head_dim):
             _bad(f"KV4Cache: the pool is a contiguous uint8 CUDA tensor [pages, {num_kv_heads}, {20 * head_dim}]")
         self.device, self.kv_heads, self.head_dim = pool.device, num_kv_heads, head_dim
+        self.index = pool.device.index
         self.view = KV4CacheView(pool.device.index, num_kv_heads, head_dim, page_table.shape[0], page_table.shape[-1],
                                  pool.shape[0], pool.data_ptr(), _int32(page_table, "page_table", pool.device, 2))
         self.ref = C.byref(self.view)
@@ -948,23 +949,25 @@ class KV4Cache:
 
     def _torch(self):
         import torch
-        self._bf16, self._empty, self._stream = torch.bfloat16, torch.empty, torch.cuda.current_stream
-        self._f32, self._u8 = torch.float32, torch.uint8
+        self._bf16, self._empty, self._f32, self._u8 = torch.bfloat16, torch.empty, torch.float32, torch.uint8
+        self._stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream(device).cuda_stream, in 0.1 us
 
     def _rows(self, t, name, batch, heads, dtype):
         D = self.head_dim
-        if t.dtype != dtype or t.device != self.device or t.shape != (batch.tokens, heads, D):
+        if t.dtype is not dtype or t.get_device() != self.index or t.shape != (batch.tokens, heads, D):
             _bad(f"{name}: {dtype} rows [{batch.tokens}, {heads}, {D}] on {self.device} are needed, got {t.dtype} "
                  f"{list(t.shape)} on {t.device}")
-        st = t.stride()
-        if t.shape[0] and (st[2] != 1 or (st[1] != D and heads > 1)):
+        if t.is_contiguous():
+            return t.data_ptr(), heads * D
+        row, head, dim = t.stride()
+        if t.shape[0] and (dim != 1 or (head != D and heads > 1)):
             _bad(f"{name}: a token's heads must be contiguous")
-        return t.data_ptr(), st[0] if t.shape[0] > 1 else heads * D
+        return t.data_ptr(), row if t.shape[0] > 1 else heads * D
 
     def _gamma(self, g, name):
         if g is None:
             return None
-        if g.dtype != self._f32 or g.device != self.device or g.shape != (self.head_dim,) or not g.is_contiguous():
+        if g.dtype is not self._f32 or g.get_device() != self.index or g.shape != (self.head_dim,) or not g.is_contiguous():
             _bad(f"{name}: a contiguous float32 tensor [{self.head_dim}] on {self.device} is needed")
         return g.data_ptr()
 
@@ -974,24 +977,25 @@ class KV4Cache:
         heads, D] normed and rotated in bf16 (None without q)."""
         if self._bf16 is None:
             self._torch()
-        if batch.device != self.device:
+        if batch.index != self.index:
             _bad(f"append: the batch is on {batch.device}, the cache on {self.device}")
         dt = k.dtype
-        if dt != self._bf16 and dt != self._f32:
+        if dt is not self._bf16 and dt is not self._f32:
             _bad(f"append: rows are float32 or bfloat16, got {dt}")
-        r = KV4Rows(0 if dt == self._f32 else 1)
-        r.k, r.k_stride = self._rows(k, "k", batch, self.kv_heads, dt)
-        r.v, r.v_stride = self._rows(v, "v", batch, self.kv_heads, dt)
+        kp, ks = self._rows(k, "k", batch, self.kv_heads, dt)
+        vp, vs = self._rows(v, "v", batch, self.kv_heads, dt)
+        heads = qs = os_ = 0
+        qp = op = None
         if q is not None:
             heads = q.shape[1]
-            r.num_heads = heads
-            r.q, r.q_stride = self._rows(q, "q", batch, heads, dt)
+            qp, qs = self._rows(q, "q", batch, heads, dt)
             if q_out is None:
                 q_out = self._empty(q.shape, dtype=self._bf16, device=self.device)
-            r.q_out, r.q_out_stride = self._rows(q_out, "q_out", batch, heads, self._bf16)
-        r.q_gamma, r.k_gamma, r.eps = self._gamma(q_gamma, "q_gamma"), self._gamma(k_gamma, "k_gamma"), eps
+            op, os_ = self._rows(q_out, "q_out", batch, heads, self._bf16)
+        r = KV4Rows(0 if dt is self._f32 else 1, heads, qp, kp, vp, qs, ks, vs, self._gamma(q_gamma, "q_gamma"),
+                    self._gamma(k_gamma, "k_gamma"), eps, op, os_)
         check(lib().q3t_kv4_append(self.ref, batch.ref, C.byref(r), None if rope is None else rope.ref,
-                                   self._stream(self.device).cuda_stream))
+                                   self._stream(self.index)))
         return q_out if q is not None else None
 
     def attend(self, batch, q, scale=None, window=0, out=None):
@@ -999,7 +1003,7 @@ class KV4Cache:
         [tokens, heads, D]); scale defaults to head_dim ** -0.5."""
         if self._bf16 is None:
             self._torch()
-        if batch.device != self.device:
+        if batch.index != self.index:
             _bad(f"attend: the batch is on {batch.device}, the cache on {self.device}")
         if out is None:
             out = self._empty(q.shape, dtype=self._bf16, device=self.device)
@@ -1009,21 +1013,21 @@ class KV4Cache:
         ws = self._empty(KV4_WORKSPACE, dtype=self._u8, device=self.device)  # this call's own, from torch's allocator
         check(lib().q3t_kv4_attend(self.ref, batch.ref, heads, qp, qs,
                                    self.head_dim ** -0.5 if scale is None else scale, window, op, os_, ws.data_ptr(),
-                                   KV4_WORKSPACE, self._stream(self.device).cuda_stream))
+                                   KV4_WORKSPACE, self._stream(self.index)))
         return out
 
     def read(self, batch, k=None, v=None):
         """(keys, values) the cache holds for the batch's rows, bf16 [tokens, kv heads, D]."""
         if self._bf16 is None:
             self._torch()
-        if batch.device != self.device:
+        if batch.index != self.index:
             _bad(f"read: the batch is on {batch.device}, the cache on {self.device}")
         shape = (batch.tokens, self.kv_heads, self.head_dim)
         k = self._empty(shape, dtype=self._bf16, device=self.device) if k is None else k
         v = self._empty(shape, dtype=self._bf16, device=self.device) if v is None else v
         kp, ks = self._rows(k, "k", batch, self.kv_heads, self._bf16)
         vp, vs = self._rows(v, "v", batch, self.kv_heads, self._bf16)
-        check(lib().q3t_kv4_read(self.ref, batch.ref, kp, ks, vp, vs, self._stream(self.device).cuda_stream))
+        check(lib().q3t_kv4_read(self.ref, batch.ref, kp, ks, vp, vs, self._stream(self.index)))
         return k, v
 
 
