@@ -97,6 +97,12 @@ APPEND = [  # D, kvh, group, new, past, dtype, norm, rope kwargs, row padding
     (64, 2, 4, [9, 8], [70_000, 8], torch.float32, False, dict(scaling="linear", factor=3.0), 2),
     (128, 2, 0, [20], [12], torch.bfloat16, False, None, 0),
     (128, 20, 1, [5], [3], torch.bfloat16, False, dict(rotary_dim=0), 0),
+    (128, 2, 2, [70, 40], [3, 100], torch.bfloat16, True, dict(theta=1e6), 0),
+    (64, 3, 2, [64], [7], torch.float32, True, dict(layout="interleaved", rotary_dim=48), 0),
+    (128, 1, 3, [45], [0], torch.float32, False, None, 1),
+    (64, 2, 1, [35, 100], [60, 0], torch.bfloat16, False, dict(), 2),
+    (128, 2, 1, [50, 33], [0, 1], torch.bfloat16, True, dict(rotary_dim=72), 0),
+    (64, 1, 2, [3, 0, 18], [2, 0, 40], torch.float32, True, dict(rotary_dim=8), 0),
 ]
 
 
@@ -159,9 +165,9 @@ def test_append_matches_definition(D, kvh, group, new, past, dtype, norm, rp, pa
 
 
 @pytest.mark.parametrize("D", [64, 128])
-def test_append_without_rotation_stores_exact_digits(D):
+@pytest.mark.parametrize("new, past", [([16, 5, 37], [0, 11, 16]), ([64, 33], [0, 5])])
+def test_append_without_rotation_stores_exact_digits(D, new, past):
     """Nothing precedes the quantisation, so every digit, scale and zero equals the definition's in 32 bits."""
-    new, past = [16, 5, 37], [0, 11, 16]
     S = Setup(D, 3, new, past)
     cache, batch = S.on_gpu()
     g = S.rng
@@ -185,6 +191,58 @@ def test_append_without_rotation_stores_exact_digits(D):
             np.testing.assert_array_equal(pool[pg][:, byte[c]] >> shift[c] & 15, n[row])
             np.testing.assert_array_equal(half[pg][:, sc[c, ::32] + o], R.bf16_bits(scale[row]))
             np.testing.assert_array_equal(half[pg][:, sc[c, ::32] + o + 1], R.bf16_bits(zero[row]))
+
+
+@pytest.mark.parametrize("new", [[9], [48]])
+def test_append_norm_of_extreme_rows(new):
+    """Rows whose squares 32 bits do not hold, rows of zeros, and q_out = q."""
+    S = Setup(128, 2, new, [0])
+    cache, batch = S.on_gpu()
+    x = S.rng.standard_normal((S.T, 6, 128)) * 10.0 ** S.rng.choice([-35, -25, -12, 0, 12, 25, 35], (S.T, 6, 1))
+    x[1] = 0
+    x[2, :, 5] = 1e30  # one element far above the rest
+    rows = torch.from_numpy(x).cuda().bfloat16()
+    x = rows.double().cpu().numpy()
+    gamma = (1 + 0.3 * S.rng.standard_normal(128)).astype(np.float32)
+    g = torch.from_numpy(gamma).cuda()
+    q, k, v = rows[:, :2].clone(), rows[:, 2:4], rows[:, 4:]
+    for eps in (0.0, 1e-6):
+        ref = R.rms_norm(x, gamma.astype(np.float64), eps) if eps else R.rms_norm(
+            np.where(x == 0, np.nan, x), gamma.astype(np.float64), eps)  # 0 / 0 is no number
+        ref = np.where(np.isnan(x * ref), np.nan, ref) if eps else ref
+        mine = q.clone()
+        out = cache.append(batch, k, v, q=mine, q_gamma=g, k_gamma=g, eps=eps, q_out=mine)
+        assert out.data_ptr() == mine.data_ptr()
+        got, want = mine.double().cpu().numpy(), ref[:, :2]
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        # norm and gamma: two 32-bit roundings, the factor's own, and the bf16's; below 2^-126 steps are 2^-133
+        err = np.abs(got - want) - (HALF + 2.0 ** -21) * np.abs(want) - 2.0 ** -133
+        assert np.nanmax(err) <= 0
+
+
+@pytest.mark.parametrize("B", [33, 129, 600])
+def test_many_sequences(B):
+    """More sequences than a warp, a CTA and one launch of attend look through at a time, some without rows."""
+    g = np.random.default_rng(B)
+    new = [int(x) for x in g.choice([0, 1, 1, 1, 2, 20], B)]
+    past = [int(x) for x in g.integers(0, 40, B)]
+    S = Setup(64, 2, new, past)
+    q = attend_case(S, 2)
+    cache, batch = S.on_gpu()
+    check_attend(cache.attend(batch, q), q, S, 0)
+    cache, batch = S.on_gpu(0, 0)
+    check_attend(cache.attend(batch, q, window=9), q, S, 9)
+    k, v = (torch.from_numpy(S.rng.standard_normal((S.T, 2, 64)).astype(np.float32)).cuda() for _ in range(2))
+    cache.append(batch, k, v)
+    kc, vc, _, _ = R.unpack(S.d_pool.cpu().numpy(), 64)
+    got = [t.double().cpu().numpy() for t in cache.read(batch)]
+    for x, y, stored, src in zip(got, range(2), (kc, vc), (k, v)):
+        ref = np.stack([stored[S.slot(s, p)[0], :, S.slot(s, p)[1]] for _, s, p in S.places()])
+        assert (np.abs(x - ref) <= HALF * np.abs(ref) + 2.0 ** -22 * np.abs(ref).max()).all()
+        # and what is stored are the rows: within half a scale, which is at most (range + 2^-7 of the smallest) / 15
+        src = src.double().cpu().numpy()
+        step = (np.ptp(src.reshape(S.T, 2, 2, 32), axis=-1) * 1.02 + 0.04) / 15
+        assert (np.abs(ref - src) <= 0.5 * step.repeat(32, -1) * (1 + 2.0 ** -6)).all()
 
 
 def test_values_that_are_not_finite_read_back_as_nan():
@@ -277,11 +335,20 @@ def attend_case(S, group, scale_up=1.0):
     return q
 
 
-def check_attend(out, q, S, window, scale=None, pool=None):
+def check_attend(out, q, S, window, scale=None, pool=None, key_bits=None):
     kc, vc, _, _ = R.unpack(S.pool if pool is None else pool, S.D)
     scale = S.D ** -0.5 if scale is None else scale
     ref, big = R.attend(q.double().cpu().numpy(), kc, vc, S.table, S.q_start, S.kv, scale, window, S.table_row)
     got = out.double().cpu().numpy()
+    if key_bits:
+        # keys in key_bits: a score is off by half a step of every product, its weight by e to that, and the weights'
+        # sum too
+        rows, k = np.abs(q.double().cpu().numpy()), np.abs(kc)
+        pg = sorted({S.slot(s, p)[0] for s, n in enumerate(S.kv) for p in range(n)} & set(range(S.P)))
+        most = np.nan_to_num(k[pg], nan=0).transpose(0, 2, 1, 3).reshape(-1, S.kvh, S.D)
+        group = rows.shape[1] // S.kvh
+        sums = np.stack([(most[:, h // group] @ rows[:, h].T).max(0) for h in range(rows.shape[1])], 1)
+        big = big * (1 + 2 * abs(scale) * sums[..., None] * 2.0 ** -key_bits / (3 * 2.0 ** -11))
     # the output's own rounding, and weights and values in 11 bits: three half steps of 2^-11 on what they weigh
     # (a weight p s of the value, or the value and the weight; and the scores' 32-bit steps far below that)
     bound = HALF * np.abs(ref) + 3 * 2.0 ** -11 * big + 1e-30
@@ -295,6 +362,87 @@ def test_attend_matches_definition(D, kvh, group, new, past, window, hints):
     q = attend_case(S, group)
     cache, batch = S.on_gpu(*(() if hints else (0, 0)))
     check_attend(cache.attend(batch, q, window=window), q, S, window)
+
+
+PROMPTS = [  # D, kvh, group, new, past, window, spread of the values
+    (128, 1, 2, [600], [0], 0, 1.0),           # rows of several tiles, each with its own number of keys
+    (128, 2, 2, [140], [700], 0, 1.0),         # both halves of a tile, its keys divided
+    (128, 2, 2, [20], [1500], 0, 1.0),         # few rows on many keys
+    (128, 1, 3, [100, 9, 60], [300, 900, 0], 150, 1.0),
+    (64, 2, 4, [70, 1, 33], [450, 17, 5], 0, 1.0),
+    (64, 1, 8, [40], [1100], 333, 1.0),
+    (128, 1, 2, [200], [100], 0, 1e5),         # values and keys that later rows see are far larger
+    (64, 1, 2, [18, 30], [900, 2], 0, 1e5),
+]
+
+
+@pytest.mark.parametrize("D, kvh, group, new, past, window, spread", PROMPTS)
+@pytest.mark.parametrize("workspace", [64 << 10, q3t.KV4_WORKSPACE])
+def test_attend_of_prompts(D, kvh, group, new, past, window, spread, workspace, monkeypatch):
+    """Tiles of 256 rows on the tensor cores, whole (no room for parts) and with their keys divided."""
+    monkeypatch.setattr(q3t, "KV4_WORKSPACE", workspace)
+    S = Setup(D, kvh, new, past)
+    q = attend_case(S, group)
+    if spread > 1:
+        g = S.rng
+        grow = [spread ** np.linspace(-1, 0, n)[None, :, None] for n in S.kv]
+        ks, vs = ([(g.standard_normal((kvh, n, D)) * w).astype(np.float32) for n, w in zip(S.kv, grow)] for _ in range(2))
+        for v, n, p in zip(vs, new, past):
+            v[:, (p + n // 2) | 15] *= 1e5  # the last key of a page, which the rows before it share
+        S.fill(ks, vs)
+    cache, batch = S.on_gpu()
+    check_attend(cache.attend(batch, q, window=window), q, S, window, key_bits=11)
+    a = cache.attend(batch, q, window=window)
+    assert torch.equal(a, cache.attend(batch, q, window=window))
+
+
+def test_attend_of_a_prompt_with_keys_that_are_no_numbers():
+    """Rows behind such a key are NaN (of a value: its group), rows before it and outside their window are not."""
+    S = Setup(128, 1, [300], [40])
+    q = attend_case(S, 2)
+    _, _, _, _, sc = R.block_tables(128)
+    half = S.pool.view(np.uint16)
+    for pos, what in ((200, 0), (250, 2)):  # K's scale of group 1, V's of group 2
+        pg, c = S.slot(0, pos)
+        half[pg, 0, sc[c, 32 * (1 + (what > 0))] + what] = 0x7fc0
+    cache, batch = S.on_gpu()
+    nan = np.isnan(cache.attend(batch, q).float().cpu().numpy())
+    assert not nan[:160].any() and nan[160:].all()
+    nan = np.isnan(cache.attend(batch, q, window=30).float().cpu().numpy())
+    assert not nan[:160].any() and nan[160:190].all() and not nan[190:210].any() and not nan[240:].any()
+    assert nan[210:240, :, 64:96].all() and not nan[210:240, :, :64].any() and not nan[210:240, :, 96:].any()
+
+
+def test_attend_of_a_prompt_with_missing_pages():
+    S = Setup(128, 2, [90, 40], [200, 1000])
+    q = attend_case(S, 2)
+    S.table[0, [0, 3, 15]] = -1
+    S.table[1, 4:60] = S.P + 7
+    cache, batch = S.on_gpu()
+    check_attend(cache.attend(batch, q), q, S, 0, key_bits=11)
+    S.table[:] = -5
+    cache, batch = S.on_gpu()
+    assert (cache.attend(batch, q) == 0).all()
+
+
+def test_attend_of_a_prompt_in_a_graph_next_to_eager_calls():
+    """A captured prompt keeps its own parts: eager calls between replays do not disturb it."""
+    S = Setup(128, 2, [30], [1200])
+    q = attend_case(S, 2)
+    cache, batch = S.on_gpu()
+    ref = cache.attend(batch, q)
+    once, twice = torch.empty_like(q), torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(batch, q, out=once)
+        cache.attend(batch, once, out=twice)  # on the parts' memory again
+    ref2 = cache.attend(batch, ref)
+    for _ in range(3):
+        once.zero_()
+        graph.replay()
+        assert torch.equal(cache.attend(batch, q), ref)
+        torch.cuda.synchronize()
+        assert torch.equal(once, ref) and torch.equal(twice, ref2)
 
 
 def test_attend_hints_do_not_change_what_is_computed():
