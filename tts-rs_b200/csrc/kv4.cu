@@ -1201,7 +1201,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) k_kv4_attend(const __gri
   pdl_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int carry = 0, more = 0;
-  for (int base = 0; base < B; base += 128) {
+  for (int base = 0; notes && base < B; base += 128) {
     const int s = base + (int)threadIdx.x;
     int incl = 0;
     if (s < B) {
@@ -1231,23 +1231,41 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) k_kv4_attend(const __gri
     if (s < B) pre[s + 1] = before + incl;
     __syncthreads();
   }
-  if (threadIdx.x == 0) pre[0] = 0;
+  if (notes && threadIdx.x == 0) pre[0] = 0;
   more = __syncthreads_or(more);
-  attend_list<D, NT>(a, StepList{pre, seq, B, 0}, blockIdx.x % n_kv, blockIdx.x / n_kv, gridDim.x / n_kv, ring_all, s_part,
-                     slot, notes + blockIdx.x, parts + (size_t)blockIdx.x * 2 * PART);
-  // rows beyond the first R of a sequence (more than the caller announced): a CTA to each unit
-  for (int item = blockIdx.x; more; item += gridDim.x) {
-    int s, i;
-    __syncthreads();
-    if (!find_item(B, item, [&](int q) { return max(0, (seq[q].total + R - 1) / R - 1) * n_kv; }, s, i)) break;
-    const int row0 = (i / n_kv + 1) * R;
-    if (threadIdx.x == 0) {
-      one_seq = seq[s];
-      one_pre[0] = 0;
-      one_pre[1] = unit_steps(unit_of<R>(one_seq, row0, gq, a.window));
+  // attend_list is here once: its code, twice or three times, would be fetched more than run
+  for (int turn = 0;; turn++) {
+    StepList list{pre, seq, B, 0};
+    int kvh = blockIdx.x % n_kv, ci = blockIdx.x / n_kv, ctas = gridDim.x / n_kv;
+    if (!notes || turn > 0) {
+      int s, i;
+      if (!notes) {  // a CTA to each sequence of a kv head, its units in turn
+        s = ci, i = turn;
+        if (threadIdx.x == 0) {
+          int n;
+          seq_rows(a.b, s, one_seq.t0, n, one_seq.pos0);
+          one_seq.total = a.big > 0 && n * gq > a.big ? 0 : n * gq;
+          one_seq.table_row = a.b.table_row ? a.b.table_row[s] : a.b.first + s;
+        }
+      } else {  // rows beyond the first R of a sequence (more than the caller announced): a CTA to each unit
+        if (!more || !find_item(B, blockIdx.x + (turn - 1) * gridDim.x,
+                                [&](int q) { return max(0, (seq[q].total + R - 1) / R - 1) * n_kv; }, s, i))
+          break;
+        kvh = i % n_kv, i = i / n_kv + 1;
+        if (threadIdx.x == 0) one_seq = seq[s];
+      }
+      if (threadIdx.x == 0) {
+        one_pre[0] = 0;
+        one_pre[1] = unit_steps(unit_of<R>(one_seq, i * R, gq, a.window));
+      }
+      __syncthreads();
+      if (i * R >= one_seq.total) break;
+      list = StepList{one_pre, &one_seq, 1, i * R};
+      ci = 0, ctas = 1;
     }
+    attend_list<D, NT>(a, list, kvh, ci, ctas, ring_all, s_part, slot, notes ? notes + blockIdx.x : nullptr,
+                       parts + (size_t)blockIdx.x * 2 * PART);
     __syncthreads();
-    attend_list<D, NT>(a, StepList{one_pre, &one_seq, 1, row0}, i % n_kv, 0, 1, ring_all, s_part, slot, nullptr, nullptr);
   }
 }
 
@@ -2080,6 +2098,14 @@ cudaError_t attend_launch(const Kv4AttendArgs &a, int max_kv, void *ws, int64_t 
   // one grid that fills the GPU once, fewer where a warp would have less than one step
   const int64_t pages = (a.window > 0 && (max_kv <= 0 || a.window < max_kv) ? a.window + 31 : max_kv > 0 ? max_kv : 1 << 20) / 16 + 1;
   const int64_t steps = (pages + 1) / 2 * a.b.num_seqs;
+  // A CTA to each sequence and kv head where they all fit the GPU at once and a warp's share is short: no second
+  // launch to join parts.  The more CTAs, the less an equal division gains (us, whole against divided, D = 128): 8 CTAs
+  // of 200 keys 6.7 and 8.0, of 1000 12.4 and 8.4; 32 of 500 9.1 and 8.9; 128 of 500 9.3 and 12.3, of 1000 12.8 and
+  // 15.5, of 2500 23.9 and 20.9; 512, which do not fit, of 500 21.6 and 20.5.
+  const int64_t per_warp = ((pages + 1) / 2 + Cfg::W - 1) / Cfg::W, whole = (int64_t)a.b.num_seqs * a.c.n_kv;
+  if (whole <= resident.load() && per_warp <= 2 + whole / 9)
+    return launch(k_kv4_attend<D, NT>, dim3((unsigned)whole), Cfg::W * 32, Cfg::smem(1), 1, pdl, st, a, (PartNote *)nullptr,
+                  (float *)nullptr);
   const int64_t fit = ws_bytes / (int64_t)(sizeof(PartNote) + 2 * Cfg::PART * 4);
   const int64_t most = std::min<int64_t>(std::min<int64_t>(resident.load(), fit) / a.c.n_kv, (steps + Cfg::W - 1) / Cfg::W);
   const int ctas = (int)std::max<int64_t>(most, 1), grid = ctas * a.c.n_kv;  // of a kv head, of all
