@@ -302,9 +302,13 @@ Q3T_DEV bool quantise(const float v[8], uint32_t n[8], uint32_t &scale_zero) {
 // four lanes a group of 32, and a warp two rows (D = 128) or four of one kind.
 // Blocks are put together in shared memory, and a window that fills its page
 // is written in 16-byte pieces, any other in the bytes that its tokens own.
-// (With 32 dims to a lane the sums and shuffles per element are fewer, but the
-// code is four times as long, and a decoding step, which goes through it once,
-// spends its time fetching it: 64 rows took 11.2 us, like this 5.4.)
+// Bound by issuing instructions, not by bytes: 8100 rows of 32 heads take
+// 52 us, 2.1 TB/s.  With 32 dims to a lane (E = D / 32) the sums and shuffles
+// per element are fewer, but the code is longer, and a decoding step, which
+// goes through it once, spends its time fetching it.  Eight dims to a lane and
+// 32 (D = 128): 64 rows 6.3 and 11.2 us, 8100 rows 65 and 52 us; so prompts,
+// of 32 rows and more to a sequence, take the second, unless only a part of
+// their rows turns by halves (the others of its pairs are other lanes').
 // ---------------------------------------------------------------------------
 constexpr int kAppendThreads = 256, kAppendDeep = 32;
 
@@ -522,7 +526,10 @@ __global__ void __launch_bounds__(kAppendThreads, E == 1 ? 4 : E == 2 ? 3 : 2) k
 
 // ---------------------------------------------------------------------------
 // Read: one CTA per (window, head split) brings its blocks to shared memory
-// and writes the rows n s + z, rounded once to bf16.
+// and writes the rows n s + z, rounded once to bf16.  A thread takes whole
+// words of digits: eight of a key, or the 64 of 16 dims of four tokens' values.
+// Bound by HBM: 64 sequences of 100 to 1500 tokens, 314 MB, in 60 us, 0.80 of
+// the measured copy rate (a byte at a time: 109 us).
 // ---------------------------------------------------------------------------
 constexpr int kReadThreads = 256;
 
@@ -616,6 +623,11 @@ __global__ void __launch_bounds__(kReadThreads) k_kv4_read(const __grid_constant
 // lies inside a warp's run is finished there; the (m, l, o) parts of one that
 // does not are joined in order, by the CTA where it has them all, otherwise
 // by k_kv4_combine from the workspace.  Nothing is kept between calls.
+//
+// Long caches are bound by HBM: 64 requests of 4096 keys on 8 kv heads, 336
+// MB, take 67 us, 0.76 of the measured copy rate, and the loads alone take as
+// long; one of 131071 keys 39 us (in units of CTAs that end with a sequence
+// 94).  Short ones are bound by both ends: 64 of 100 to 1500 keys 27 us.
 //
 // f16 holds q times a power of two per row (its 11 bits keep a bf16 q whole
 // down to 2^-25 of the row's largest) and p s, where p carries a power of two
@@ -1341,14 +1353,27 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
 //   S = Q K^T     M 128 rows, N 64 keys, K D        (TMEM, two buffers)
 //   O += P V      M 128 rows, N D, K 64 keys        (TMEM)
 // Two such halves share every unpacked tile of keys.  Warps 0-7 are the
-// softmax (a thread to a row), 8-11 unpack K and 12-15 V (a warp to a page of
+// softmax (a thread to a row), 8-15 unpack (a warp to a page of K or of V of
 // the tile), 16-19 issue the products, one lane to each half's S and P V (one
-// lane for all four spent its time issuing: 540 cycles for an S).  K, V and S have two buffers each, so the unpacking of a
-// tile, its S, the softmax of the one before and its P V run at once.
+// lane for all four spent its time issuing: 540 cycles for an S).  K, V and S
+// have two buffers each, so the unpacking of a tile, its S, the softmax of the
+// one before and its P V run at once.
 //
-// f16 holds q times a power of two per row, K and V times one per page and per
-// tile (from the largest value there, 11 bits of each), and p, with V's power
-// relative to the largest so far.  A page's power of K enters with the score's
+// What bounds it is issuing instructions: a tile of 256 rows x 64 keys takes
+// 3100 cycles and 7900 warp instructions, 64 % of the four schedulers' slots;
+// the tensor pipe is busy 27 %, HBM does not matter.  Unpacking is 40 % of
+// them, which 4-bit keys cost and bf16 ones would not.  A prompt of 4096
+// tokens on 8 kv heads (68.7 GFLOP) takes 122 us, 0.34 of the floor of the
+// products alone.  With loops unrolled throughout, 102 KB of code instead of
+// 62, warps waited for instructions most of the time: 178 us.
+//
+// Where tiles of rows cannot fill the GPU, CTAs share the keys of each and
+// k_kv4_join joins their parts: 16 rows of one request on 8000 keys 30 us, and
+// 85 as units of k_kv4_attend.
+//
+// f16 holds q times a power of two per row, K and V times one per page (from
+// the largest value there, 11 bits of each), and p, with V's power relative to
+// the largest a row has seen.  A page's power of K enters with the score's
 // scale.  m, l, S and O are in 32 bits; m is moved, and O with it, only when a
 // score passes it by 2^8, which p in f16 can hold.
 //
