@@ -558,7 +558,7 @@ typedef struct {
   int num_kv_heads;          /* 1..1024 */
   int head_dim;              /* 64 or 128 */
   int table_rows;
-  int table_stride;          /* page-table entries of a row */
+  int table_stride;          /* page-table entries of a row, up to 2^20 */
   int64_t num_pages;         /* pages of the pool */
   void *pool;                /* device, on a 16-byte boundary */
   const int32_t *page_table; /* device [table_rows][table_stride]: entry i of a row is the page of

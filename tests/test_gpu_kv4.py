@@ -317,6 +317,8 @@ ATTEND = [  # D, kvh, group, new, past, window, hints
     (64, 4, 4, [1, 1, 1], [0, 64, 129], 33, True),
     (64, 2, 8, [4, 1], [100, 17], 0, True),
     (64, 1, 5, [50], [0], 0, False),
+    (128, 2, 2, [1, 2], [9, 40], 0, False),
+    (64, 2, 1, [1], [3], 0, False),
     (128, 2, 2, [150], [0], 0, True),
     (128, 2, 2, [129, 64], [37, 500], 48, True),
     (64, 2, 2, [200], [33], 0, True),
@@ -423,6 +425,32 @@ def test_attend_of_a_prompt_with_missing_pages():
     S.table[:] = -5
     cache, batch = S.on_gpu()
     assert (cache.attend(batch, q) == 0).all()
+
+
+@pytest.mark.parametrize("new, group", [([2, 1], 2), ([20, 3], 2), ([1, 1], 16)])
+def test_attend_of_lengths_far_past_the_table(new, group):
+    """Positions that no table entry stands for hold no keys, up to the largest lengths there are."""
+    # every table entry is a page of written keys: stale bytes are numbers up to 3e38, whose scores 32 bits do not hold
+    S = Setup(128, 2, new, [96 - n for n in new], stride_extra=0)
+    q = attend_case(S, group)
+    S.kv = [100_000 + n for n in new]
+    cache, batch = S.on_gpu(0, 0)
+    out = cache.attend(batch, q)
+    keys = S.table.shape[1] * 16
+    kc, vc, _, _ = R.unpack(S.pool, 128)
+    end = np.array([keys + n for n in new])  # every row sees the whole table
+    ref, big = R.attend(q.double().cpu().numpy(), kc, vc, S.table, S.q_start, end, 128 ** -0.5)
+    assert (np.abs(out.double().cpu().numpy() - ref) <= HALF * np.abs(ref) + 2.0 ** -9 * big).all()
+    S.kv = [2 ** 31 - 1, 2 ** 31 - 17]
+    cache, batch = S.on_gpu(0, 0)
+    assert torch.equal(cache.attend(batch, q), out)
+    assert torch.equal(cache.attend(batch, q, window=2 ** 31 - 1), out)
+    assert (cache.attend(batch, q, window=1000) == 0).all()
+    k, v = (torch.zeros(S.T, 2, 128, device="cuda") for _ in range(2))
+    before = S.d_pool.clone()
+    assert torch.equal(cache.append(batch, k, v, q=q.float()), q)  # the queries come all the same
+    assert torch.equal(S.d_pool, before)
+    assert all((t == 0).all() for t in cache.read(batch))
 
 
 def test_attend_of_a_prompt_in_a_graph_next_to_eager_calls():

@@ -47,7 +47,7 @@ def call_append(c=None, b=None, r=None, p=None):
 
 BAD_CACHE = [dict(head_dim=96), dict(head_dim=0), dict(num_kv_heads=0), dict(num_kv_heads=1025), dict(num_pages=0),
              dict(num_pages=1 << 31), dict(table_rows=0), dict(table_stride=-1), dict(pool=None), dict(page_table=None),
-             dict(pool=(1 << 20) + 8)]
+             dict(pool=(1 << 20) + 8), dict(table_stride=(1 << 20) + 1)]
 BAD_BATCH = [dict(num_seqs=-1), dict(num_seqs=(1 << 20) + 1), dict(num_tokens=-1), dict(num_tokens=(1 << 28) + 1),
              dict(max_q_len=-1), dict(max_kv_len=-5), dict(q_start=None), dict(kv_len=None)]
 BAD_ROWS = [dict(dtype=2), dict(num_heads=-1), dict(k=None), dict(v=None), dict(q=None), dict(q_out=None),

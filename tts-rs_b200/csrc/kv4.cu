@@ -132,10 +132,10 @@ Q3T_DEV bool find_window(const Kv4Batch &b, int item, Window &w) {
   int t0, n, pos0;
   seq_rows(b, w.s, t0, n, pos0);
   w.p = (pos0 >> 4) + i;  // negative for padding in front of position 0
-  const int first = max(pos0, w.p * 16), last = min(pos0 + n, w.p * 16 + 16);
-  w.t0 = t0 + first - pos0;
-  w.n = last - first;
-  w.c0 = first - w.p * 16;
+  const int base = w.p * 16;
+  w.c0 = max(pos0 - base, 0);
+  w.t0 = t0 + base + w.c0 - pos0;
+  w.n = min(pos0 + n - base, 16) - w.c0;
   return true;
 }
 // windows of a call, at most: a sequence's n rows touch (n + 14) / 16 + 1 pages, and n
@@ -683,14 +683,14 @@ struct Unit {
 // token of a query row: a decode step has one, and no division then
 Q3T_DEV int token_of(int row, int gq) { return row < gq ? 0 : row / gq; }
 template <int R>
-Q3T_DEV Unit unit_of(const SeqRows &s, int row0, int gq, int window) {
+Q3T_DEV Unit unit_of(const SeqRows &s, int row0, int gq, int window, int table_stride) {
   Unit u;
   u.row0 = row0;
   u.nrow = min(R, s.total - row0);
   u.pos_lo = s.pos0 + token_of(row0, gq);
   u.pos_hi = s.pos0 + token_of(row0 + max(u.nrow, 1) - 1, gq);
   u.pg_lo = window > 0 ? max(0, u.pos_lo - window + 1) >> 4 : 0;
-  u.pages = u.pos_hi < 0 ? 0 : max(0, (u.pos_hi >> 4) + 1 - u.pg_lo);
+  u.pages = u.pos_hi < 0 ? 0 : max(0, min((u.pos_hi >> 4) + 1, table_stride) - u.pg_lo);  // none past the table
   return u;
 }
 // steps of a unit: one at least, so that rows without keys are answered too
@@ -755,13 +755,13 @@ struct PageCursor {
       do next_seq++;
       while (L.pre[next_seq + 1] == L.pre[next_seq]);
       next_end = min(L.pre[next_seq + 1] - L.pre[next_seq], left_after);
-      const Unit u = unit_of<R>(L.seq[next_seq], L.row0, gq, a.window);
+      const Unit u = unit_of<R>(L.seq[next_seq], L.row0, gq, a.window, a.c.table_stride);
       next_lo = u.pg_lo, next_pages = u.pages;
     }
     look(a, L, next_seq, next_step, next_lo, next_pages, next_ids);
   }
   Q3T_DEV void start(const Kv4AttendArgs &a, const StepList &L, int gq, int s, int at, int to) {
-    const Unit u = unit_of<R>(L.seq[s], L.row0, gq, a.window);
+    const Unit u = unit_of<R>(L.seq[s], L.row0, gq, a.window, a.c.table_stride);
     seq = s, step = block = at - L.pre[s], left = to - at;
     end = min(L.pre[s + 1] - L.pre[s], step + left);
     pg_lo = u.pg_lo, pages = u.pages;
@@ -861,7 +861,7 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
   int get = 0, parts = 0;
   while (at < to) {
     const SeqRows sq = L.seq[seq];
-    const Unit u = unit_of<R>(sq, L.row0, gq, a.window);
+    const Unit u = unit_of<R>(sq, L.row0, gq, a.window, a.c.table_stride);
     const int steps = L.pre[seq + 1] - L.pre[seq], i0 = at - L.pre[seq], i1 = min(steps, i0 + (to - at));
     const int pos_lo = u.pos_lo, pos_hi = u.pos_hi;
 
@@ -1224,7 +1224,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) k_kv4_attend(const __gri
       q.table_row = a.b.table_row ? a.b.table_row[s] : a.b.first + s;
       if (a.big > 0 && q.total > a.big) q.total = 0;  // k_kv4_prompt has it
       seq[s] = q;
-      incl = unit_steps(unit_of<R>(q, 0, gq, a.window));
+      incl = unit_steps(unit_of<R>(q, 0, gq, a.window, a.c.table_stride));
       more |= q.total > R;
     }
 #pragma unroll
@@ -1268,7 +1268,7 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) k_kv4_attend(const __gri
       }
       if (threadIdx.x == 0) {
         one_pre[0] = 0;
-        one_pre[1] = unit_steps(unit_of<R>(one_seq, i * R, gq, a.window));
+        one_pre[1] = unit_steps(unit_of<R>(one_seq, i * R, gq, a.window, a.c.table_stride));
       }
       __syncthreads();
       if (i * R >= one_seq.total) break;
@@ -1512,9 +1512,10 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
   int pg_lo = key_lo >> 4;
   // tiles of keys that the first 128 rows see, and the others; both begin at page pg_lo
-  auto tiles_to = [&](int pos) { return pos < 0 ? 0 : max(0, ((pos >> 4) + 1 - pg_lo + PAGES - 1) / PAGES); };
+  auto pages_to = [&](int pos) { return pos < 0 ? 0 : max(0, min((pos >> 4) + 1, a.c.table_stride) - pg_lo); };
+  auto tiles_to = [&](int pos) { return (pages_to(pos) + PAGES - 1) / PAGES; };
   int nt0 = tiles_to(pos0 + (row0 + min(nrow, 128) - 1) / gq), nt1 = nrow > 128 ? tiles_to(pos_hi) : 0;
-  int n_tiles = max(nt0, nt1), n_pages = pos_hi < 0 ? 0 : max(0, (pos_hi >> 4) + 1 - pg_lo);
+  int n_tiles = max(nt0, nt1), n_pages = pages_to(pos_hi);
   if (splits > 1) {  // this CTA's tiles of keys, four at least
     const int per = max(4, (n_tiles + splits - 1) / splits), skip = split * per;
     nt0 = max(0, min(nt0 - skip, per)), nt1 = max(0, min(nt1 - skip, per));
@@ -1959,6 +1960,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   tc_fence_before();
   __syncthreads();
   if (warp == 16) {
+    if (dead) __nanosleep(50000);  // products that were issued before a wait gave up end within it
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -2121,7 +2123,9 @@ cudaError_t attend_launch(const Kv4AttendArgs &a, int max_kv, void *ws, int64_t 
   });
   if (e != cudaSuccess) return e;
   // one grid that fills the GPU once, fewer where a warp would have less than one step
-  const int64_t pages = (a.window > 0 && (max_kv <= 0 || a.window < max_kv) ? a.window + 31 : max_kv > 0 ? max_kv : 1 << 20) / 16 + 1;
+  const bool windowed = a.window > 0 && (max_kv <= 0 || a.window < max_kv);
+  const int64_t keys = windowed ? (int64_t)a.window + 31 : max_kv > 0 ? max_kv : 1 << 20;
+  const int64_t pages = std::min<int64_t>(keys / 16 + 1, a.c.table_stride);
   const int64_t steps = (pages + 1) / 2 * a.b.num_seqs;
   // A CTA to each sequence and kv head where they all fit the GPU at once and a warp's share is short: no second
   // launch to join parts.  The more CTAs, the less an equal division gains (us, whole against divided, D = 128): 8 CTAs
@@ -2189,6 +2193,7 @@ static cudaError_t prompt_launch(const Kv4AttendArgs &a, int thr, void *ws, int6
   // tiles, at most: whole ones, and one more for every sequence that has over thr rows
   const int64_t rows = (int64_t)a.b.num_tokens * (a.n_heads / a.c.n_kv);
   const int64_t tiles = std::min<int64_t>(rows / Cfg::ROWS + std::min<int64_t>(a.b.num_seqs, rows / (thr + 1)), rows);
+  if (tiles == 0) return cudaSuccess;  // too few rows for a sequence of over thr
   // where these cannot fill the GPU, CTAs share the keys of each
   const int64_t fit = std::min<int64_t>(sms.load(), ws_bytes / (4 * Cfg::PART));
   const int64_t grid = std::max<int64_t>(tiles * a.c.n_kv, fit);
@@ -2285,8 +2290,9 @@ Kv4View view_of(const char *what, const q3t_kv4_cache *c) {
     FAIL(Q3T_INVALID_INPUT, "%s: num_kv_heads %d outside 1..1024", what, c->num_kv_heads);
   if (c->num_pages < 1 || c->num_pages > 0x7fffffff)
     FAIL(Q3T_INVALID_INPUT, "%s: num_pages %lld outside 1..2^31-1", what, (long long)c->num_pages);
-  if (c->table_rows < 1 || c->table_stride < 1)
-    FAIL(Q3T_INVALID_INPUT, "%s: page table of %d x %d", what, c->table_rows, c->table_stride);
+  if (c->table_rows < 1 || c->table_stride < 1 || c->table_stride > (1 << 20))
+    FAIL(Q3T_INVALID_INPUT, "%s: page table of %d x %d (1..2^20 entries to a row)", what, c->table_rows,
+         c->table_stride);
   if (!c->pool || !c->page_table) FAIL(Q3T_INVALID_INPUT, "%s: null pool or page table", what);
   if (!aligned(c->pool, 16)) FAIL(Q3T_INVALID_INPUT, "%s: the pool must start on a 16-byte boundary", what);
   return Kv4View{(uint8_t *)c->pool, c->page_table, c->num_pages, c->num_kv_heads, c->head_dim, c->table_rows,
