@@ -2209,15 +2209,19 @@ cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws,
   if (a0.b.num_tokens <= 0 || a0.b.num_seqs <= 0) return cudaSuccess;
   Kv4AttendArgs a = a0;
   const int gq = a.n_heads / a.c.n_kv;
-  // sequences of more rows than this go by tiles of 128 rows on k_kv4_prompt
+  // Sequences of more rows than this go by tiles on k_kv4_prompt.  At 17 to 32 rows it takes, against k_kv4_attend
+  // (us), 30 and 85 (one sequence, 8000 keys), 106 and 220 (eight), 128 and 264 (64, 1000 keys); at 16 about as much.
   constexpr int kBig = 16;
   const bool some_big = max_q <= 0 || (int64_t)max_q * gq > kBig;
-  const bool mostly_big = some_big && (int64_t)a.b.num_tokens * gq > (int64_t)kBig * a.b.num_seqs;
+  // No sequence is small where all but one at their most leave more than kBig rows for the last.  Elsewhere both
+  // kernels run, each for its sequences: a tile of 256 rows for one row of a decoding request costs 7 us of an SM.
+  const bool none_small = (int64_t)a.b.num_tokens - (int64_t)(a.b.num_seqs - 1) * std::max(max_q, 0) > kBig / gq &&
+                          (max_q > 0 || a.b.num_seqs == 1);
   if (some_big) {
-    const int thr = mostly_big ? 0 : kBig;
+    const int thr = none_small ? 0 : kBig;
     const cudaError_t e = a.c.head_dim == 128 ? prompt_launch<128>(a, thr, ws, ws_bytes, st, pdl)
-                                                   : prompt_launch<64>(a, thr, ws, ws_bytes, st, pdl);
-    if (e != cudaSuccess || mostly_big) return e;
+                                              : prompt_launch<64>(a, thr, ws, ws_bytes, st, pdl);
+    if (e != cudaSuccess || none_small) return e;
     a.big = kBig;
   }
   const int rows = (some_big ? 1 : max_q) * gq;  // rows of a kv head: one column tile, or two
