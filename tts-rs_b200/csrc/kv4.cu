@@ -1968,8 +1968,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
 
 // Joins the parts of k_kv4_prompt's tiles, where it divided the keys: a thread
 // has a row, eight dims of it (32 to a thread, one part after the other, took
-// 33 us for 18 parts: all of it waiting for loads).  A part's o is divided by its l already, so a part
-// weighs l 2^m; parts come in order, and the result does not depend on timing.
+// 33 us for 18 parts: all of it waiting for loads).  A part's o is divided by
+// its l already, so a part weighs l 2^m; parts come in order, and the result
+// does not depend on timing.
 template <int D>
 __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4AttendArgs a, PromptSplit sp) {
   using Cfg = PromptCfg<D>;
@@ -1989,46 +1990,47 @@ __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4Att
   int t0, n, pos0;
   seq_rows(a.b, s, t0, n, pos0);
   const int total = n * gq, row0 = ((total + ROWS - 1) / ROWS - 1 - i_rev) * ROWS, nrow = min(ROWS, total - row0);
-  const int at = blockIdx.y * 256 + threadIdx.x, d0 = 8 * (at / nrow), r = at % nrow, flat = row0 + r, tok = flat / gq;
-  if (d0 >= D) return;
-  const float *part = sp.parts + (size_t)(blockIdx.x / n_kv * splits * n_kv + kvh) * Cfg::PART + r;
-  const size_t step = (size_t)n_kv * Cfg::PART;
-  constexpr int N = 8;  // parts whose loads are on their way together
-  float M = -INFINITY, L = 0.f;
-  for (int k0 = 0; k0 < splits; k0 += N) {
-    float m[N];
+  for (int at = blockIdx.y * 256 + threadIdx.x; at < nrow * (D / 8); at += gridDim.y * 256) {
+    const int d0 = 8 * (at / nrow), r = at % nrow, flat = row0 + r, tok = flat / gq;
+    const float *part = sp.parts + (size_t)(blockIdx.x / n_kv * splits * n_kv + kvh) * Cfg::PART + r;
+    const size_t step = (size_t)n_kv * Cfg::PART;
+    constexpr int N = 8;  // parts whose loads are on their way together
+    float M = -INFINITY, L = 0.f;
+    for (int k0 = 0; k0 < splits; k0 += N) {
+      float m[N];
 #pragma unroll
-    for (int k = 0; k < N; k++) m[k] = k0 + k < splits ? part[(k0 + k) * step] : -INFINITY;
+      for (int k = 0; k < N; k++) m[k] = k0 + k < splits ? part[(k0 + k) * step] : -INFINITY;
 #pragma unroll
-    for (int k = 0; k < N; k++) M = fmaxf(M, m[k]);
+      for (int k = 0; k < N; k++) M = fmaxf(M, m[k]);
+    }
+    float o[8] = {};
+    for (int k0 = 0; k0 < splits; k0 += N) {
+      float m[N], l[N];
+      float4 u[N], v[N];
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        const float *p = part + (k0 + k) * step;
+        m[k] = k0 + k < splits ? p[0] : 0.f, l[k] = k0 + k < splits ? p[ROWS] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        const float4 *from = reinterpret_cast<const float4 *>(part - r + (k0 + k) * step + 2 * ROWS) + r + (size_t)(d0 / 4) * ROWS;
+        u[k] = v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (l[k] != 0.f) u[k] = from[0], v[k] = from[ROWS];  // it has keys of this row
+      }
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        const float w = l[k] == 0.f ? 0.f : l[k] * ex2(m[k] - M);
+        L += w;
+        o[0] = fmaf(w, u[k].x, o[0]), o[1] = fmaf(w, u[k].y, o[1]), o[2] = fmaf(w, u[k].z, o[2]), o[3] = fmaf(w, u[k].w, o[3]);
+        o[4] = fmaf(w, v[k].x, o[4]), o[5] = fmaf(w, v[k].y, o[5]), o[6] = fmaf(w, v[k].z, o[6]), o[7] = fmaf(w, v[k].w, o[7]);
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int e = 0; e < 8; e++) o[e] *= inv;
+    store8(a.out + (size_t)(t0 + tok) * a.ldo + (size_t)(kvh * gq + flat - tok * gq) * D + d0, a.vec, o);
   }
-  float o[8] = {};
-  for (int k0 = 0; k0 < splits; k0 += N) {
-    float m[N], l[N];
-    float4 u[N], v[N];
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-      const float *p = part + (k0 + k) * step;
-      m[k] = k0 + k < splits ? p[0] : 0.f, l[k] = k0 + k < splits ? p[ROWS] : 0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-      const float4 *from = reinterpret_cast<const float4 *>(part - r + (k0 + k) * step + 2 * ROWS) + r + (size_t)(d0 / 4) * ROWS;
-      u[k] = v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (l[k] != 0.f) u[k] = from[0], v[k] = from[ROWS];  // it has keys of this row
-    }
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-      const float w = l[k] == 0.f ? 0.f : l[k] * ex2(m[k] - M);
-      L += w;
-      o[0] = fmaf(w, u[k].x, o[0]), o[1] = fmaf(w, u[k].y, o[1]), o[2] = fmaf(w, u[k].z, o[2]), o[3] = fmaf(w, u[k].w, o[3]);
-      o[4] = fmaf(w, v[k].x, o[4]), o[5] = fmaf(w, v[k].y, o[5]), o[6] = fmaf(w, v[k].z, o[6]), o[7] = fmaf(w, v[k].w, o[7]);
-    }
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-  for (int e = 0; e < 8; e++) o[e] *= inv;
-  store8(a.out + (size_t)(t0 + tok) * a.ldo + (size_t)(kvh * gq + flat - tok * gq) * D + d0, a.vec, o);
 }
 
 // ---------------------------------------------------------------------------
@@ -2201,7 +2203,10 @@ static cudaError_t prompt_launch(const Kv4AttendArgs &a, int thr, void *ws, int6
   const PromptSplit sp = {thr, tiles * a.c.n_kv < fit ? (int)fit : 1, (float *)ws};
   e = launch(k_kv4_prompt<D>, dim3((unsigned)grid), Cfg::THREADS, Cfg::kSmem, 1, pdl, st, a, sp);
   if (e != cudaSuccess || sp.most == 1) return e;
-  return launch(k_kv4_join<D>, dim3((unsigned)std::min(tiles * a.c.n_kv, fit / 2), D / 8), 256, 0, 1, false, st, a, sp);
+  // as many CTAs as the GPU holds at once: more of them cost a call with nothing to join 9 us instead of 4
+  const int64_t most = std::min(tiles * a.c.n_kv, fit / 2);
+  const unsigned along = (unsigned)std::max<int64_t>(1, std::min<int64_t>(D / 8, 2 * sms.load() / most));
+  return launch(k_kv4_join<D>, dim3((unsigned)most, along), 256, 0, 1, false, st, a, sp);
 }
 
 cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st,
