@@ -1678,9 +1678,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       __syncwarp();
       if (i >= 2) wait(&freed[b], ((i >> 1) - 1) & 1);
       if (is_v) {
-        // rows are dims, one atom of 64 keys; digits of dims g and g + 8 of every 16
-        uint8_t *to = sv + b * Cfg::VB + g * 128 + 4 * t;
-        const int c0 = ((2 * w) ^ g) << 4, c1 = ((2 * w + 1) ^ g) << 4;
+        // rows are dims, one atom of 64 keys; digits of dims g and g + 8 of every 16.  A page's keys lie in the order
+        // that a lane has them in (2t, 2t + 1, 2t + 8, 2t + 9; P's do too): half the stores
+        uint8_t *to = sv + b * Cfg::VB + g * 128 + (((2 * w + (t >> 1)) ^ g) << 4) + 8 * (t & 1);
 #pragma unroll 1
         for (int j = 0; j < G; j++, to += 32 * 128) {
           const uint4 u = *reinterpret_cast<const uint4 *>(sc + 64 * j + 16 * t);  // keys 2t, 2t + 1, 2t + 8, 2t + 9
@@ -1690,10 +1690,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
           for (int m = 0; m < 2; m++) {
             uint32_t o[4];
             unpack8(m ? d.y : d.x, sx, zx, o);  // (dim g, dim g + 8) x (keys 2t .., keys 2t + 8 ..)
-            *reinterpret_cast<uint32_t *>(to + 16 * m * 128 + c0) = o[0];
-            *reinterpret_cast<uint32_t *>(to + (16 * m + 8) * 128 + c0) = o[1];
-            *reinterpret_cast<uint32_t *>(to + 16 * m * 128 + c1) = o[2];
-            *reinterpret_cast<uint32_t *>(to + (16 * m + 8) * 128 + c1) = o[3];
+            *reinterpret_cast<uint2 *>(to + 16 * m * 128) = make_uint2(o[0], o[2]);
+            *reinterpret_cast<uint2 *>(to + (16 * m + 8) * 128) = make_uint2(o[1], o[3]);
           }
         }
         if (lane < 16) v_bad[b][token] = (uint8_t)bad;
@@ -1867,7 +1865,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; k++) {
-            const int at = 16 * (p & 1) + 8 * c + 2 * k;
+            const int at = 16 * (p & 1) + 4 * c + 8 * (k & 1) + 2 * (k >> 1);  // V's order of keys
             float y0, y1;
             f2_split(f2_fma(f2_pack(__uint_as_float(x[p >> 1][at]), __uint_as_float(x[p >> 1][at + 1])), ff, cc), y0, y1);
             y0 = ex2(y0), y1 = ex2(y1);
