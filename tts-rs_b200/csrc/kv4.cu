@@ -1462,9 +1462,9 @@ struct PromptCfg {
   static constexpr int PART = ROWS * (D + 2);  // floats
   static constexpr int QB = 128 * D * 2, KB = KEYS * D * 2, VB = D * KEYS * 2, PB = 128 * KEYS * 2;
   static constexpr int SC = PAGES * 2 * D;  // a tile's scales and zeros of K, or of V
-  static constexpr int ST = 3, RING = 12 * D;  // blocks on their way to an unpacking warp: digits, scale entries
+  static constexpr int ST = 2, RING = 12 * D;  // blocks on their way to an unpacking warp: digits, scale entries
   static constexpr size_t kSmem =
-      2 * QB + 2 * KB + 2 * VB + 2 * PB + 2 * SC + 2 * PAGES * ST * RING + 1024;  // from a 1024-byte boundary
+      2 * QB + 2 * KB + 2 * VB + 4 * PB + 2 * SC + 2 * PAGES * ST * RING + 1024;  // from a 1024-byte boundary
 };
 
 template <int D>
@@ -1483,7 +1483,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   __shared__ __align__(4) uint8_t k_says[8][PAGES], v_says[2][PAGES];  // of a page: bit 0 it is there, bit 1 such groups
   __shared__ int dead;  // a wait gave up
   uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *sq = base, *sk = sq + 2 * Cfg::QB, *sv = sk + 2 * Cfg::KB, *sp = sv + 2 * Cfg::VB, *scales = sp + 2 * Cfg::PB,
+  uint8_t *sq = base, *sk = sq + 2 * Cfg::QB, *sv = sk + 2 * Cfg::KB, *sp = sv + 2 * Cfg::VB, *scales = sp + 4 * Cfg::PB,
           *rings = scales + 2 * Cfg::SC;
   pdl_wait();
   const int n_kv = a.c.n_kv, gq = a.n_heads / n_kv, kvh = blockIdx.x % n_kv;
@@ -1617,21 +1617,21 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
 
   if (warp >= 8 && warp < 16) {
     // ---- unpack: page w of every tile ----
-    constexpr int EPL = 16 * G / 32, ST = Cfg::ST;  // scale entries of a lane; blocks on their way
+    constexpr int EPL = 16 * G / 32;  // scale entries of a lane
     const bool is_v = warp & 2;  // each scheduler has warps of one kind, and with them less code
     const int w = (warp & 1) + 2 * (warp >= 12), g = lane >> 2, t = lane & 3;
     uint8_t *sc = scales + (is_v ? Cfg::SC : 0) + w * 2 * D;
-    uint8_t *ring = rings + (warp - 8) * ST * Cfg::RING;
+    uint8_t *ring = rings + (warp - 8) * Cfg::ST * Cfg::RING;
     uint64_t *freed = is_v ? v_freed : k_freed;
     int ids = -1;
-    uint32_t there = 0;  // bit 0: the last page asked for is there; bit 1: the one before
+    bool there = false;  // the page asked for last
     auto fetch = [&](int tile, uint8_t *to) {
       if (tile % 32 == 0) {  // this warp's page of the next 32 tiles, by lane
         const int p = (tile + lane) * PAGES + w;
         ids = p < n_pages ? page_of(a.c, a.b, s, pg_lo + p) : -1;
       }
       const int id = __shfl_sync(0xffffffffu, ids, tile % 32);
-      there = there << 1 | (id >= 0);
+      there = id >= 0;
       if (id >= 0) {
         const uint8_t *blk = a.c.pool + ((size_t)id * n_kv + kvh) * BLK;
 #pragma unroll
@@ -1641,17 +1641,14 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       cp_async_commit();
     };
     fetch(0, ring);
-    fetch(1, ring + Cfg::RING);
-    int slot = 0;
 #pragma unroll 1
     for (int i = 0; i < n_tiles; i++) {
       const int b = i & 1, key0 = (pg_lo + i * PAGES + w) * 16;
-      const bool here = there & 2u;
-      uint8_t *from = ring + slot * Cfg::RING;
-      cp_async_wait<ST - 2>();
+      const bool here = there;
+      const uint8_t *from = ring + b * Cfg::RING;
+      cp_async_wait<0>();
       __syncwarp();  // all lanes' copies are here, and all lanes are done with the block before
-      slot = slot == ST - 1 ? 0 : slot + 1;
-      fetch(i + 2, ring + (slot == ST - 1 ? 0 : slot + 1) * Cfg::RING);
+      fetch(i + 1, ring + (b ^ 1) * Cfg::RING);
       // what no row sees, and what is no number, becomes zeros
       uint32_t en[EPL];
       float top = 0.f;
@@ -1753,7 +1750,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       }
     } else if (lane == 0) {
       constexpr uint32_t id_o = umma_idesc_f16(128, D);
-      const uint64_t dp = sw128_desc(sp + h * Cfg::PB), dv = sw128_desc(sv);
+      const uint64_t dp = sw128_desc(sp + 2 * h * Cfg::PB), dv = sw128_desc(sv);
       for (int i = 0; i < nt; i++) {
         const int b = i & 1;
         wait(&v_full[b], (i >> 1) & 1);
@@ -1762,7 +1759,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < KEYS / 16; k++)
-          umma_kf16(tmem + 256 + 128 * h, dp + ((32 * k) >> 4), dv + ((b * Cfg::VB + 32 * k) >> 4), id_o, i > 0 || k > 0);
+          umma_kf16(tmem + 256 + 128 * h, dp + ((b * Cfg::PB + 32 * k) >> 4), dv + ((b * Cfg::VB + 32 * k) >> 4), id_o,
+                    i > 0 || k > 0);
         umma_commit(&pv_done[h]);
         umma_commit(&v_freed[b]);
         if (i >= other) umma_commit(&v_freed[b]);
@@ -1779,7 +1777,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     const int all_to = pos0 + (row0 + min(128 * h, nrow - 1)) / gq;
     const int all_from = a.window > 0 ? pos0 + (row0 + min(128 * h + 127, nrow - 1)) / gq - a.window + 1 : 0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, t_s = tmem + lanes + 128 * h, t_o = tmem + lanes + 256 + 128 * h;
-    uint8_t *my_p = sp + h * Cfg::PB + r * 128;
+    uint8_t *my_p = sp + 2 * h * Cfg::PB + r * 128;
     float m = -INFINITY, l = 0.f;  // m: what the exponents are taken from
     int e_ref = -1000;             // power of two of O
     uint32_t nan = 0;              // of the keys this row has seen: bit j, V of group j; bit 7, K
@@ -1826,7 +1824,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         for (int k = 1; k < 16; k++) y = fmaxf(y, __uint_as_float(x[p >> 1][16 * (p & 1) + k]));
         top = fmaxf(top, y * f[p]);
       }
-      wait(&v_full[b], (i >> 1) & 1);
+      wait(&v_full[b], (i >> 1) & 1);  // which means too that P V of tile i - 2 has been, and P may be written
       const uint32_t v_say = *reinterpret_cast<const uint32_t *>(v_says[b]);
       const int4 v4 = *reinterpret_cast<const int4 *>(v_exp[b]);
       const int ve[PAGES] = {v4.x, v4.y, v4.z, v4.w};
@@ -1851,7 +1849,6 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         e_ref = e_new;
         move = true;
       }
-      if (i > 0) wait(&pv_done[h], (i - 1) & 1);  // O is whole, and P may be written
       const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int p = 0; p < PAGES; p++) {
@@ -1872,13 +1869,15 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
             part = f2_add(part, f2_pack(y0, y1));
             w[k] = pack_f16x2(y0, y1);
           }
-          *reinterpret_cast<uint4 *>(my_p + (((2 * p + c) ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4 *>(my_p + b * Cfg::PB + (((2 * p + c) ^ (r & 7)) << 4)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
         }
         float s0, s1;
         f2_split(part, s0, s1);
         l = fmaf(s0 + s1, __uint_as_float((uint32_t)(127 - dv) << 23), l);
       }
       if (i > 0 && __any_sync(0xffffffffu, move)) {
+        wait(&pv_done[h], (i - 1) & 1);  // O is whole
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D / 32; c++) {
@@ -1893,6 +1892,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       fence_proxy_async();
       mbar_arrive(&p_full[h]);
     }
+    if (nt > 1) wait(&pv_done[h], (nt - 2) & 1);  // a wait may be one phase behind, not two
     if (nt > 0) wait(&pv_done[h], (nt - 1) & 1);
     tc_fence_after();
     const bool gone = *(volatile int *)&dead;
