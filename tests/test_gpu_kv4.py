@@ -499,6 +499,28 @@ def test_attend_long_cache_and_sharp_scores():
     check_attend(cache.attend(batch, q, scale=-0.5), q, S, 0, scale=-0.5)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_averages_of_very_many_keys(D):
+    """80,000 keys that weigh about alike, for the whole GPU and (hints far too low) for one CTA: the average is some
+    hundredths of the values, and keeps its own digits."""
+    n = 80_000
+    S = Setup(D, 1, [n], [0], spare=0)
+    cache, batch = S.on_gpu()
+    k, v = (torch.from_numpy(S.rng.standard_normal((n, 1, D)).astype(np.float32)).cuda() for _ in range(2))
+    cache.append(batch, k, v)
+    pool = S.d_pool.cpu().numpy()
+    q = torch.from_numpy(S.rng.standard_normal((1, 2, D)).astype(np.float32)).cuda().bfloat16()
+    kc, vc, _, _ = R.unpack(pool, D)
+    for max_kv in (n, 1):
+        one = q3t.KV4Batch(torch.tensor([0, 1], dtype=torch.int32, device="cuda"),
+                           torch.tensor([n], dtype=torch.int32, device="cuda"), 1, max_q=1, max_kv=max_kv)
+        got = cache.attend(one, q).double().cpu().numpy()
+        ref, _ = R.attend(q.double().cpu().numpy(), kc, vc, S.table, [0, 1], [n], D ** -0.5)
+        # a bf16 half step, and every key's weight p s rounded by half a step of 11 bits: independent, so together no
+        # more of the sum of independent values than each of its own
+        assert np.linalg.norm(got - ref) <= (HALF + 3 * 2.0 ** -11) * np.linalg.norm(ref)
+
+
 def test_attend_extreme_queries_and_values():
     """Queries of zeros, tiny and large ones in one row, tiny and large value scales."""
     S = Setup(64, 1, [6], [40])
