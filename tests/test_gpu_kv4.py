@@ -324,6 +324,10 @@ ATTEND = [  # D, kvh, group, new, past, window, hints
     (64, 2, 2, [200], [33], 0, True),
     (128, 3, 1, [77], [0], 0, True),
     (64, 1, 12, [30], [250], 70, True),
+    (128, 1, 8, [1, 1], [5000, 90], 0, True),
+    (128, 2, 5, [1, 1, 1], [3000, 2, 800], 0, True),
+    (64, 1, 12, [1], [4000], 0, True),
+    (128, 2, 3, [2, 1, 0, 3], [900, 1500, 4, 60], 333, True),
 ]
 
 

@@ -674,7 +674,7 @@ Q3T_DEV float part_weight(float m, float l, float M) {
 // A sequence's rows, as the kernel keeps them: token rows from t0, n * heads
 // of a kv head = `total` query rows, the first at position pos0.
 struct SeqRows {
-  int t0, total, pos0, table_row;
+  int t0, total, pos0, table_row, row0;  // row0: of the unit
 };
 // Query rows [row0, row0 + nrow) of it and the pages they see.
 struct Unit {
@@ -704,9 +704,9 @@ struct AttendCfg {
   static constexpr int W = 4;                    // warps of a CTA
   static constexpr int RING = ST * NP * BLK;
   static constexpr int PART = R * (2 + G + D);   // floats of a part: m [R], l [R], z [R][G], o [R][D]
-  static constexpr int MAXSEQ = 512;             // sequences of a launch
-  static constexpr size_t smem(int seqs) {
-    return (size_t)W * RING + W * 2 * PART * 4 + seqs * sizeof(SeqRows) + (seqs + 1) * 4;
+  static constexpr int MAXSEQ = 512;             // units of a launch's list
+  static constexpr size_t smem(int units) {
+    return (size_t)W * RING + W * 2 * PART * 4 + units * sizeof(SeqRows) + (units + 1) * 4;
   }
 };
 
@@ -717,11 +717,11 @@ Q3T_DEV void store_out(const Kv4AttendArgs &a, int t0, int row, int kvh, int d, 
 }
 
 // The step list of a kv head: steps pre[i] .. pre[i + 1] - 1 are those of
-// rows [row0, row0 + R) of sequence i.
+// rows [seq[i].row0, seq[i].row0 + R) of a sequence.
 struct StepList {
   const int *pre;
   const SeqRows *seq;
-  int n, row0;
+  int n;
 };
 
 // Where the copies of a warp's run are: the block of up to 16 steps of one
@@ -755,13 +755,13 @@ struct PageCursor {
       do next_seq++;
       while (L.pre[next_seq + 1] == L.pre[next_seq]);
       next_end = min(L.pre[next_seq + 1] - L.pre[next_seq], left_after);
-      const Unit u = unit_of<R>(L.seq[next_seq], L.row0, gq, a.window, a.c.table_stride);
+      const Unit u = unit_of<R>(L.seq[next_seq], L.seq[next_seq].row0, gq, a.window, a.c.table_stride);
       next_lo = u.pg_lo, next_pages = u.pages;
     }
     look(a, L, next_seq, next_step, next_lo, next_pages, next_ids);
   }
   Q3T_DEV void start(const Kv4AttendArgs &a, const StepList &L, int gq, int s, int at, int to) {
-    const Unit u = unit_of<R>(L.seq[s], L.row0, gq, a.window, a.c.table_stride);
+    const Unit u = unit_of<R>(L.seq[s], L.seq[s].row0, gq, a.window, a.c.table_stride);
     seq = s, step = block = at - L.pre[s], left = to - at;
     end = min(L.pre[s + 1] - L.pre[s], step + left);
     pg_lo = u.pg_lo, pages = u.pages;
@@ -810,7 +810,7 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
     const SeqRows sq = L.seq[s];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int flat = min(L.row0 + (nt * 8 + g) / G, sq.total - 1);  // a row past the end repeats the last one
+      const int flat = min(sq.row0 + (nt * 8 + g) / G, sq.total - 1);  // a row past the end repeats the last one
       const int tok = token_of(flat, gq), head = kvh * gq + flat - tok * gq;
       const uint16_t *qp = a.q + (size_t)(sq.t0 + tok) * a.ldq + (size_t)head * D + 32 * j + 8 * t;
       if (a.vec) {
@@ -861,7 +861,7 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
   int get = 0, parts = 0;
   while (at < to) {
     const SeqRows sq = L.seq[seq];
-    const Unit u = unit_of<R>(sq, L.row0, gq, a.window, a.c.table_stride);
+    const Unit u = unit_of<R>(sq, sq.row0, gq, a.window, a.c.table_stride);
     const int steps = L.pre[seq + 1] - L.pre[seq], i0 = at - L.pre[seq], i1 = min(steps, i0 + (to - at));
     const int pos_lo = u.pos_lo, pos_hi = u.pos_hi;
 
@@ -1169,7 +1169,7 @@ Q3T_DEV void attend_list(const Kv4AttendArgs &a, const StepList &L, int kvh, int
     left_to_join &= ~mine;
     const int last = 31 - __clz(mine), ends = slot[last >> 1][last & 1].ends;
     const SeqRows sq = L.seq[f.seq];
-    const int nrow = min(R, sq.total - L.row0);
+    const int nrow = min(R, sq.total - sq.row0);
     float *dst = parts + (f.begins ? PART : 0);
 #pragma unroll
     for (int e0 = 0; e0 < R * D; e0 += 128) {
@@ -1189,7 +1189,7 @@ Q3T_DEV void attend_list(const Kv4AttendArgs &a, const StepList &L, int kvh, int
         o += w * (p[2 * R + R * Cfg::G + e] + p[2 * R + e / 32]);
       }
       if (f.begins && ends) {
-        if (r < nrow) store_out<D>(a, sq.t0, L.row0 + r, kvh, d, l, o);
+        if (r < nrow) store_out<D>(a, sq.t0, sq.row0 + r, kvh, d, l, o);
       } else {
         dst[2 * R + R * Cfg::G + e] = o;  // with its zeros
         if (d == 0) {
@@ -1202,7 +1202,7 @@ Q3T_DEV void attend_list(const Kv4AttendArgs &a, const StepList &L, int kvh, int
       const int64_t e = L.pre[f.seq + 1] - 1;  // the unit's last step, and the CTA that has it
       int c = (int)(e * ctas / T);
       while (c + 1 < ctas && T * (c + 1) / ctas <= e) c++;
-      left = PartNote{c - ci + 1, sq.t0, L.row0, nrow};
+      left = PartNote{c - ci + 1, sq.t0, sq.row0, nrow};
     }
   }
   if (ctas > 1) {
@@ -1223,27 +1223,29 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) k_kv4_attend(const __gri
   __shared__ int warp_tot[W], one_pre[2];
   __shared__ SeqRows one_seq;
   __shared__ RunSlot slot[W][2];
-  const int B = a.b.num_seqs, n_kv = a.c.n_kv, gq = a.n_heads / n_kv;
+  const int B = a.b.num_seqs, U = a.units, E = B * U, n_kv = a.c.n_kv, gq = a.n_heads / n_kv;
   float *s_part = reinterpret_cast<float *>(ring_all + W * Cfg::RING);   // [W][2][PART]
-  SeqRows *seq = reinterpret_cast<SeqRows *>(s_part + W * 2 * PART);     // [B]
-  int *pre = reinterpret_cast<int *>(seq + B);                           // [B + 1]
+  SeqRows *seq = reinterpret_cast<SeqRows *>(s_part + W * 2 * PART);     // [E], a sequence's U units in turn
+  int *pre = reinterpret_cast<int *>(seq + E);                           // [E + 1]
   pdl_wait();
   pdl_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int carry = 0, more = 0;
-  for (int base = 0; notes && base < B; base += 128) {
-    const int s = base + (int)threadIdx.x;
+  for (int base = 0; notes && base < E; base += 128) {
+    const int e = base + (int)threadIdx.x;
     int incl = 0;
-    if (s < B) {
+    if (e < E) {
+      const int s = e / U;
       SeqRows q;
       int n;
       seq_rows(a.b, s, q.t0, n, q.pos0);
       q.total = n * gq;
       q.table_row = a.b.table_row ? a.b.table_row[s] : a.b.first + s;
+      q.row0 = (e - s * U) * R;
       if (a.big > 0 && q.total > a.big) q.total = 0;  // k_kv4_prompt has it
-      seq[s] = q;
-      incl = unit_steps(unit_of<R>(q, 0, gq, a.window, a.c.table_stride));
-      more |= q.total > R;
+      seq[e] = q;
+      incl = unit_steps(unit_of<R>(q, q.row0, gq, a.window, a.c.table_stride));
+      more |= q.total > U * R;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -1258,39 +1260,40 @@ __global__ void __launch_bounds__(128, NT == 1 ? 3 : 2) k_kv4_attend(const __gri
       if (k < warp) before += warp_tot[k];
       carry += warp_tot[k];
     }
-    if (s < B) pre[s + 1] = before + incl;
+    if (e < E) pre[e + 1] = before + incl;
     __syncthreads();
   }
   if (notes && threadIdx.x == 0) pre[0] = 0;
   more = __syncthreads_or(more);
   // attend_list is here once: its code, twice or three times, would be fetched more than run
   for (int turn = 0;; turn++) {
-    StepList list{pre, seq, B, 0};
+    StepList list{pre, seq, E};
     int kvh = blockIdx.x % n_kv, ci = blockIdx.x / n_kv, ctas = gridDim.x / n_kv;
     if (!notes || turn > 0) {
       int s, i;
-      if (!notes) {  // a CTA to each sequence of a kv head, its units in turn
-        s = ci, i = turn;
+      if (!notes) {  // a CTA to each unit
+        s = ci / U, i = ci - s * U + turn * U;
         if (threadIdx.x == 0) {
           int n;
           seq_rows(a.b, s, one_seq.t0, n, one_seq.pos0);
           one_seq.total = a.big > 0 && n * gq > a.big ? 0 : n * gq;
           one_seq.table_row = a.b.table_row ? a.b.table_row[s] : a.b.first + s;
         }
-      } else {  // rows beyond the first R of a sequence (more than the caller announced): a CTA to each unit
+      } else {  // rows beyond a sequence's U units (more than the caller announced): a CTA to each R of them
         if (!more || !find_item(B, blockIdx.x + (turn - 1) * gridDim.x,
-                                [&](int q) { return max(0, (seq[q].total + R - 1) / R - 1) * n_kv; }, s, i))
+                                [&](int q) { return max(0, (seq[q * U].total + R - 1) / R - U) * n_kv; }, s, i))
           break;
-        kvh = i % n_kv, i = i / n_kv + 1;
-        if (threadIdx.x == 0) one_seq = seq[s];
+        kvh = i % n_kv, i = i / n_kv + U;
+        if (threadIdx.x == 0) one_seq = seq[s * U];
       }
       if (threadIdx.x == 0) {
+        one_seq.row0 = i * R;
         one_pre[0] = 0;
         one_pre[1] = unit_steps(unit_of<R>(one_seq, i * R, gq, a.window, a.c.table_stride));
       }
       __syncthreads();
       if (i * R >= one_seq.total) break;
-      list = StepList{one_pre, &one_seq, 1, i * R};
+      list = StepList{one_pre, &one_seq, 1};
       ci = 0, ctas = 1;
     }
     attend_list<D, NT>(a, list, kvh, ci, ctas, ring_all, s_part, slot, notes ? notes + blockIdx.x : nullptr,
@@ -2124,7 +2127,7 @@ cudaError_t read_launch(const Kv4ReadArgs &a, int windows, cudaStream_t st, bool
 }
 
 template <int D, int NT>
-cudaError_t attend_launch(const Kv4AttendArgs &a, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st, bool pdl) {
+cudaError_t attend_launch(const Kv4AttendArgs &a0, int rows, int max_kv, void *ws, int64_t ws_bytes, cudaStream_t st, bool pdl) {
   using Cfg = AttendCfg<D, NT>;
   static std::atomic<uint64_t> done{0};
   static std::atomic<int> resident{0};  // CTAs that one device holds at once
@@ -2140,16 +2143,31 @@ cudaError_t attend_launch(const Kv4AttendArgs &a, int max_kv, void *ws, int64_t 
     return r;
   });
   if (e != cudaSuccess) return e;
+  Kv4AttendArgs a = a0;
+  a.units = std::max(1, (rows + Cfg::R - 1) / Cfg::R);
+  constexpr int kUnits = Cfg::MAXSEQ;
+  if (a0.b.num_seqs * (int64_t)a.units > kUnits) {  // a part of the sequences at a time
+    const int at_once = kUnits / a.units;
+    for (int s0 = 0; s0 < a0.b.num_seqs; s0 += at_once) {
+      a.b.num_seqs = std::min(at_once, a0.b.num_seqs - s0);
+      a.b.q_start = a0.b.q_start + s0;
+      a.b.kv_len = a0.b.kv_len + s0;
+      if (a0.b.table_row) a.b.table_row = a0.b.table_row + s0;
+      a.b.first = a0.b.first + s0;
+      if ((e = attend_launch<D, NT>(a, rows, max_kv, ws, ws_bytes, st, pdl)) != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+  }
   // one grid that fills the GPU once, fewer where a warp would have less than one step
   const bool windowed = a.window > 0 && (max_kv <= 0 || a.window < max_kv);
   const int64_t keys = windowed ? (int64_t)a.window + 31 : max_kv > 0 ? max_kv : 1 << 20;
   const int64_t pages = std::min<int64_t>(keys / 16 + 1, a.c.table_stride);
-  const int64_t steps = (pages + 1) / 2 * a.b.num_seqs;
-  // A CTA to each sequence and kv head where they all fit the GPU at once and a warp's share is short: no second
+  const int64_t units = (int64_t)a.b.num_seqs * a.units, steps = (pages + 1) / 2 * units;
+  // A CTA to each unit of each kv head where they all fit the GPU at once and a warp's share is short: no second
   // launch to join parts.  The more CTAs, the less an equal division gains (us, whole against divided, D = 128): 8 CTAs
   // of 200 keys 6.7 and 8.0, of 1000 12.4 and 8.4; 32 of 500 9.1 and 8.9; 128 of 500 9.3 and 12.3, of 1000 12.8 and
   // 15.5, of 2500 23.9 and 20.9; 512, which do not fit, of 500 21.6 and 20.5.
-  const int64_t per_warp = ((pages + 1) / 2 + Cfg::W - 1) / Cfg::W, whole = (int64_t)a.b.num_seqs * a.c.n_kv;
+  const int64_t per_warp = ((pages + 1) / 2 + Cfg::W - 1) / Cfg::W, whole = units * a.c.n_kv;
   if (whole <= resident.load() && per_warp <= 2 + whole / 9)
     return launch(k_kv4_attend<D, NT>, dim3((unsigned)whole), Cfg::W * 32, Cfg::smem(1), 1, pdl, st, a, (PartNote *)nullptr,
                   (float *)nullptr);
@@ -2158,7 +2176,7 @@ cudaError_t attend_launch(const Kv4AttendArgs &a, int max_kv, void *ws, int64_t 
   const int ctas = (int)std::max<int64_t>(most, 1), grid = ctas * a.c.n_kv;  // of a kv head, of all
   PartNote *notes = (PartNote *)ws;
   float *parts = (float *)(notes + grid);
-  e = launch(k_kv4_attend<D, NT>, dim3(grid), Cfg::W * 32, Cfg::smem(a.b.num_seqs), 1, pdl, st, a, notes, parts);
+  e = launch(k_kv4_attend<D, NT>, dim3(grid), Cfg::W * 32, Cfg::smem((int)units), 1, pdl, st, a, notes, parts);
   if (e != cudaSuccess || ctas == 1) return e;
   return launch(k_kv4_combine<D, NT>, dim3(grid), 256, 0, 1, false, st, a, (const PartNote *)notes, (const float *)parts);
 }
@@ -2246,23 +2264,11 @@ cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws,
     a.big = kBig;
   }
   const int rows = (some_big ? 1 : max_q) * gq;  // rows of a kv head: one column tile, or two
-  constexpr int kSeqs = AttendCfg<128, 1>::MAXSEQ;
-  for (int s0 = 0; s0 < a0.b.num_seqs; s0 += kSeqs) {  // sequences of one launch
-    a.b.num_seqs = std::min(kSeqs, a0.b.num_seqs - s0);
-    a.b.q_start = a0.b.q_start + s0;
-    a.b.kv_len = a0.b.kv_len + s0;
-    if (a0.b.table_row) a.b.table_row = a0.b.table_row + s0;
-    a.b.first = a0.b.first + s0;
-    cudaError_t e;
-    if (a.c.head_dim == 128)
-      e = rows <= 2 ? attend_launch<128, 1>(a, max_kv, ws, ws_bytes, st, pdl)
-                    : attend_launch<128, 2>(a, max_kv, ws, ws_bytes, st, pdl);
-    else
-      e = rows <= 4 ? attend_launch<64, 1>(a, max_kv, ws, ws_bytes, st, pdl)
-                    : attend_launch<64, 2>(a, max_kv, ws, ws_bytes, st, pdl);
-    if (e != cudaSuccess) return e;
-  }
-  return cudaSuccess;
+  if (a.c.head_dim == 128)
+    return rows <= 2 ? attend_launch<128, 1>(a, rows, max_kv, ws, ws_bytes, st, pdl)
+                     : attend_launch<128, 2>(a, rows, max_kv, ws, ws_bytes, st, pdl);
+  return rows <= 4 ? attend_launch<64, 1>(a, rows, max_kv, ws, ws_bytes, st, pdl)
+                   : attend_launch<64, 2>(a, rows, max_kv, ws, ws_bytes, st, pdl);
 }
 
 }  // namespace q3t

@@ -67,6 +67,7 @@ struct Kv4AttendArgs {
   int vec;            // q and out rows start on 16-byte boundaries
   int *err;           // set (bitwise or) when a bounded wait gave up; nullable
   int big;            // launcher: sequences of more rows are another kernel's (0: none)
+  int units;          // launcher: units of a few rows that a sequence has, as far as announced
 };
 
 struct Kv4ReadArgs {
