@@ -1380,17 +1380,19 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
 // have two buffers each, so the unpacking of a tile, its S, the softmax of the
 // one before and its P V run at once.
 //
-// What bounds it is issuing instructions: a tile of 256 rows x 64 keys takes
-// 3100 cycles and 7900 warp instructions, 64 % of the four schedulers' slots;
-// the tensor pipe is busy 27 %, HBM does not matter.  Unpacking is 40 % of
-// them, which 4-bit keys cost and bf16 ones would not.  A prompt of 4096
-// tokens on 8 kv heads (68.7 GFLOP) takes 122 us, 0.34 of the floor of the
-// products alone.  With loops unrolled throughout, 102 KB of code instead of
-// 62, warps waited for instructions most of the time: 178 us.
+// What bounds it is the softmax warps' way through a tile, 2950 cycles: waits
+// and loads of a few hundred each, 64 exponentials a row, and a share of the
+// schedulers, whose slots are 64 % taken (7900 warp instructions a tile, 40 %
+// of them unpacking, which 4-bit keys cost and bf16 ones would not).  The
+// tensor pipe is busy 27 %, HBM does not matter.  A prompt of 4096 tokens on 8
+// kv heads (68.7 GFLOP) takes 117 us, 0.35 of the products' rate alone.  With
+// loops unrolled throughout, 102 KB of code instead of 62, warps waited for
+// instructions most of the time: 178 us.  One buffer of P, whose P V a softmax
+// then waits for: 122 us.
 //
 // Where tiles of rows cannot fill the GPU, CTAs share the keys of each and
-// k_kv4_join joins their parts: 16 rows of one request on 8000 keys 30 us, and
-// 85 as units of k_kv4_attend.
+// k_kv4_join joins their parts: 32 rows of one request on 8000 keys take 30 us,
+// whole 200.
 //
 // f16 holds q times a power of two per row, K and V times one per page (from
 // the largest value there, 11 bits of each), and p, with V's power relative to
@@ -2248,8 +2250,9 @@ cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws,
   if (a0.b.num_tokens <= 0 || a0.b.num_seqs <= 0) return cudaSuccess;
   Kv4AttendArgs a = a0;
   const int gq = a.n_heads / a.c.n_kv;
-  // Sequences of more rows than this go by tiles on k_kv4_prompt.  At 17 to 32 rows it takes, against k_kv4_attend
-  // (us), 30 and 85 (one sequence, 8000 keys), 106 and 220 (eight), 128 and 264 (64, 1000 keys); at 16 about as much.
+  // Sequences of more rows than this go by tiles on k_kv4_prompt.  With 32 rows it takes, against k_kv4_attend (us,
+  // group of 2), 30 and 34 (one sequence of 8000 keys), 102 and 168 (eight), 127 and 197 (64 of 1000); with 16 rows
+  // k_kv4_attend takes 23, 93 and 108, and a tile as long as with 32.
   constexpr int kBig = 16;
   const bool some_big = max_q <= 0 || (int64_t)max_q * gq > kBig;
   // No sequence is small where all but one at their most leave more than kBig rows for the last.  Elsewhere both
