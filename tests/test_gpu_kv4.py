@@ -419,6 +419,18 @@ def test_attend_of_a_prompt_with_keys_that_are_no_numbers():
     assert nan[210:240, :, 64:96].all() and not nan[210:240, :, :64].any() and not nan[210:240, :, 96:].any()
 
 
+@pytest.mark.parametrize("window", [0, 7])
+def test_attend_of_prompts_with_padding_in_front(window):
+    """Rows at negative positions see nothing and give zeros: some of a tile's, all of one, all of a sequence."""
+    S = Setup(128, 2, [60, 300, 30], [0, 0, 0])
+    q = attend_case(S, 2)
+    S.kv = [25, 20, 0]
+    cache, batch = S.on_gpu()
+    out = cache.attend(batch, q, window=window)
+    assert (out[:35] == 0).all() and (out[60:340] == 0).all() and (out[360:] == 0).all()
+    check_attend(out, q, S, window, key_bits=11)
+
+
 def test_attend_of_a_prompt_with_missing_pages():
     S = Setup(128, 2, [90, 40], [200, 1000])
     q = attend_case(S, 2)

@@ -312,6 +312,14 @@ Q3T_DEV bool quantise(const float v[8], uint32_t n[8], uint32_t &scale_zero) {
 // ---------------------------------------------------------------------------
 constexpr int kAppendThreads = 256, kAppendDeep = 32;
 
+// Rotation of a pair; every product and sum is rounded by itself, so a value
+// does not depend on which of them a compiler fuses.  (Not in pairs: of two
+// f32 at once the assembler fuses a product and a sum that are rounded apart.)
+Q3T_DEV void turn(float &x0, float &x1, float c, float s) {
+  const float y0 = x0, y1 = x1;
+  x0 = __fsub_rn(__fmul_rn(y0, c), __fmul_rn(y1, s));
+  x1 = __fadd_rn(__fmul_rn(y1, c), __fmul_rn(y0, s));
+}
 // {cos, cos, sin, sin} of the pairs f = 32 i + 8 l + e and f + 1, f even, lie in the
 // order [i][e / 2][l]: neighbouring lanes read neighbouring banks
 Q3T_DEV int cs_at(int f) { return (((f >> 5) << 2) + ((f >> 1) & 3)) * 4 + ((f >> 3) & 3); }
@@ -371,7 +379,7 @@ __global__ void __launch_bounds__(kAppendThreads, E == 1 ? 4 : E == 2 ? 3 : 2) k
   // of the rotation by halves (E == 1), for dims 8 C .. + 3 and + 4 .. + 7: where the others of their pairs are (rot % 8 ==
   // 0, so the same element of a lane or the one four away), their sign, and the angles
   int from[2], angle[2];
-  uint64_t sign[2];
+  float sign[2];
   bool turns[2];
 #pragma unroll
   for (int e = 0; e < 2; e++) {
@@ -379,7 +387,7 @@ __global__ void __launch_bounds__(kAppendThreads, E == 1 ? 4 : E == 2 ? 3 : 2) k
     from[e] = o >> 3;
     turns[e] = d < 2 * half;
     angle[e] = turns[e] ? cs_at(min(d, o)) : 0;
-    sign[e] = d < half ? f2_pack(-1.f, -1.f) : f2_pack(1.f, 1.f);
+    sign[e] = d < half ? -1.f : 1.f;
   }
 #pragma unroll 1
   while (item < items) {
@@ -418,8 +426,6 @@ __global__ void __launch_bounds__(kAppendThreads, E == 1 ? 4 : E == 2 ? 3 : 2) k
       }
     }
     if (my_kind < 2 && half) {
-      // (x0 c - x1 s, x1 c + x0 s), every product and sum rounded by itself, so that a value does
-      // not depend on which of them a compiler fuses
       const float4 *f = cs + my_tok * CS;
       if (a.rope.interleaved) {
 #pragma unroll
@@ -429,9 +435,8 @@ __global__ void __launch_bounds__(kAppendThreads, E == 1 ? 4 : E == 2 ? 3 : 2) k
             for (int e = 0; e < 8; e += 4) {
               const float4 u = f[cs_at(4 * C + 16 * i + (e >> 1))];
               float *y = &x[i][e];
-              const uint64_t c0 = f2_pack(u.x, u.x), s0 = f2_pack(-u.z, u.z), c1 = f2_pack(u.y, u.y), s1 = f2_pack(-u.w, u.w);
-              f2_split(f2_add(f2_mul(f2_pack(y[0], y[1]), c0), f2_mul(f2_pack(y[1], y[0]), s0)), y[0], y[1]);
-              f2_split(f2_add(f2_mul(f2_pack(y[2], y[3]), c1), f2_mul(f2_pack(y[3], y[2]), s1)), y[2], y[3]);
+              turn(y[0], y[1], u.x, u.z);
+              turn(y[2], y[3], u.y, u.w);
             }
       } else if constexpr (E == 1) {
         float z[8];
@@ -445,18 +450,17 @@ __global__ void __launch_bounds__(kAppendThreads, E == 1 ? 4 : E == 2 ? 3 : 2) k
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           const float4 u = f[angle[e >> 2] + 4 * (e >> 1 & 1)];
-          const uint64_t y = f2_add(f2_mul(f2_pack(x[0][e], x[0][e + 1]), f2_pack(u.x, u.y)),
-                                    f2_mul(f2_pack(z[e], z[e + 1]), f2_mul(f2_pack(u.z, u.w), sign[e >> 2])));
-          if (turns[e >> 2]) f2_split(y, x[0][e], x[0][e + 1]);
+          const float y0 = __fadd_rn(__fmul_rn(x[0][e], u.x), __fmul_rn(z[e], u.z * sign[e >> 2]));
+          const float y1 = __fadd_rn(__fmul_rn(x[0][e + 1], u.y), __fmul_rn(z[e + 1], u.w * sign[e >> 2]));
+          if (turns[e >> 2]) x[0][e] = y0, x[0][e + 1] = y1;
         }
       } else {  // of a whole row: both of a pair are this lane's
 #pragma unroll
         for (int e = 0; e < 4 * E; e += 2) {
           float *lo = &x[e >> 3][e & 7], *hi = &x[(e >> 3) + E / 2][e & 7];
           const float4 u = f[(4 * (e >> 3) + ((e & 7) >> 1)) * 4 + l];
-          const uint64_t x0 = f2_pack(lo[0], lo[1]), x1 = f2_pack(hi[0], hi[1]), cc = f2_pack(u.x, u.y), ss = f2_pack(u.z, u.w);
-          f2_split(f2_sub(f2_mul(x0, cc), f2_mul(x1, ss)), lo[0], lo[1]);
-          f2_split(f2_add(f2_mul(x1, cc), f2_mul(x0, ss)), hi[0], hi[1]);
+          turn(lo[0], hi[0], u.x, u.z);
+          turn(lo[1], hi[1], u.y, u.w);
         }
       }
     }
@@ -1391,8 +1395,8 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
 // then waits for: 122 us.
 //
 // Where tiles of rows cannot fill the GPU, CTAs share the keys of each and
-// k_kv4_join joins their parts: 32 rows of one request on 8000 keys take 30 us,
-// whole 200.
+// k_kv4_join joins their parts: 32 rows of one request on 8000 keys, 126 tiles,
+// take 30 us.
 //
 // f16 holds q times a power of two per row, K and V times one per page (from
 // the largest value there, 11 bits of each), and p, with V's power relative to
@@ -2371,11 +2375,10 @@ void rope_freqs(const char *what, const q3t_rope *r, double *freqs) {
   if (r->scaling == Q3T_ROPE_BANDS && (!(r->low < r->high) || !std::isfinite(r->low) || !std::isfinite(r->high) ||
                                        r->original < 1))
     FAIL(Q3T_INVALID_INPUT, "%s: band scaling needs low < high and original > 0", what);
-  // theta^(-2 i / rot) step by step in 80 bits: 64 steps are off by 2^-57, and 64 powers would be 2 us of every append
-  const long double step = rot ? std::pow((long double)r->theta, -2.0L / rot) : 1.0L;
-  long double power = 1.0L;
-  for (int i = 0; i < rot / 2; i++, power *= step) {
-    double f = (double)power;
+  for (int i = 0; i < rot / 2; i++) {
+    // (64 powers are 2 us of an append's host time; theta^(2 / rot) multiplied up, even in 80 bits, gives other last
+    // bits than the formula, and at far positions now and then another digit)
+    double f = std::pow((double)r->theta, -2.0 * i / rot);
     if (r->scaling == Q3T_ROPE_LINEAR) f /= r->factor;
     if (r->scaling == Q3T_ROPE_BANDS) {
       const double turns = r->original * f / (2.0 * M_PI);
