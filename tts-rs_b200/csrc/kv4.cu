@@ -1499,10 +1499,12 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   using Cfg = PromptCfg<D>;
   constexpr int G = Cfg::G, BLK = Cfg::BLK, ROWS = Cfg::ROWS, KEYS = Cfg::KEYS, PAGES = Cfg::PAGES;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[21];
+  __shared__ uint64_t bars[25];
   uint64_t *k_full = bars, *v_full = bars + 2, *k_freed = bars + 4, *v_freed = bars + 6;  // by buffer
   uint64_t *s_full = bars + 8, *s_freed = bars + 12;                                     // by half and buffer
-  uint64_t *p_full = bars + 16, *pv_done = bars + 18, *q_full = bars + 20;               // by half
+  // by half and buffer too, although O is one: a softmax thread may arrive for tile i + 1 before another has for tile i,
+  // and a thread that asks for a phase may find one or two more done (a parity names only the next one)
+  uint64_t *p_full = bars + 16, *pv_done = bars + 20, *q_full = bars + 24;
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) float k_fac[8][PAGES];
   __shared__ __align__(16) int v_exp[2][PAGES];
@@ -1515,10 +1517,10 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   pdl_wait();
   const int n_kv = a.c.n_kv, gq = a.n_heads / n_kv, kvh = blockIdx.x % n_kv;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 17 && lane < 21) {
+  if (warp == 17 && lane < 25) {
     // arrivals: the unpacking warps; both halves' products; the scores, and what K's warps say of the tile;
     // the softmax threads of a half; P V; all softmax threads
-    const int n = lane < 4 ? PAGES : lane < 12 ? 2 : lane < 18 ? 128 : lane < 20 ? 1 : 256;
+    const int n = lane < 4 ? PAGES : lane < 12 ? 2 : lane < 20 ? 128 : lane < 24 ? 1 : 256;
     mbar_init(&bars[lane], n);
     fence_mbar_init();
     if (lane == 0) dead = 0;
@@ -1781,14 +1783,14 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       for (int i = 0; i < nt; i++) {
         const int b = i & 1;
         wait(&v_full[b], (i >> 1) & 1);
-        wait(&p_full[h], i & 1);
+        wait(&p_full[2 * h + b], (i >> 1) & 1);
         if (*(volatile int *)&dead) break;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < KEYS / 16; k++)
           umma_kf16(tmem + 256 + 128 * h, dp + ((b * Cfg::PB + 32 * k) >> 4), dv + ((b * Cfg::VB + 32 * k) >> 4), id_o,
                     i > 0 || k > 0);
-        umma_commit(&pv_done[h]);
+        umma_commit(&pv_done[2 * h + b]);
         umma_commit(&v_freed[b]);
         if (i >= other) umma_commit(&v_freed[b]);
       }
@@ -1904,7 +1906,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         l = fmaf(s0 + s1, __uint_as_float((uint32_t)(127 - dv) << 23), l);
       }
       if (i > 0 && __any_sync(0xffffffffu, move)) {
-        wait(&pv_done[h], (i - 1) & 1);  // O is whole
+        wait(&pv_done[2 * h + (b ^ 1)], ((i - 1) >> 1) & 1);  // O is whole
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < D / 32; c++) {
@@ -1917,10 +1919,9 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       }
       tc_fence_before();
       fence_proxy_async();
-      mbar_arrive(&p_full[h]);
+      mbar_arrive(&p_full[2 * h + b]);
     }
-    if (nt > 1) wait(&pv_done[h], (nt - 2) & 1);  // a wait may be one phase behind, not two
-    if (nt > 0) wait(&pv_done[h], (nt - 1) & 1);
+    if (nt > 0) wait(&pv_done[2 * h + ((nt - 1) & 1)], ((nt - 1) >> 1) & 1);
     tc_fence_after();
     const bool gone = *(volatile int *)&dead;
     const float up = exp2f((float)max(e_ref, -126)), inv = l == 0.f ? 0.f : 1.f / l;
