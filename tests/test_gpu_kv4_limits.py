@@ -1,0 +1,21 @@
+"""The 4-bit key/value cache operators at the ends of what their arguments may
+be: the widest groups, windows, lengths and scales."""
+import numpy as np
+import pytest
+
+import kv4_ref as R
+import q3t
+from test_gpu_kv4 import HALF, Setup, attend_case, check_attend
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.mark.parametrize("D, group", [(128, 2100), (64, 4200), (128, 17)])
+def test_attend_of_groups_wider_than_a_launch_lists(D, group):
+    """Without hints the rows of one token are more than the decoding kernel lists, and every sequence is a prompt."""
+    S = Setup(D, 1, [1, 2], [300, 40])
+    q = attend_case(S, group)
+    cache, batch = S.on_gpu(0, 0)
+    check_attend(cache.attend(batch, q), q, S, 0, key_bits=11)

@@ -2268,7 +2268,7 @@ cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws,
     const int thr = none_small ? 0 : kBig;
     const cudaError_t e = a.c.head_dim == 128 ? prompt_launch<128>(a, thr, ws, ws_bytes, st, pdl)
                                               : prompt_launch<64>(a, thr, ws, ws_bytes, st, pdl);
-    if (e != cudaSuccess || none_small) return e;
+    if (e != cudaSuccess || none_small || gq > kBig) return e;  // (one row of a group of over kBig is no small sequence)
     a.big = kBig;
   }
   const int rows = (some_big ? 1 : max_q) * gq;  // rows of a kv head: one column tile, or two
