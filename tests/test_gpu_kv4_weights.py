@@ -1,0 +1,153 @@
+"""Attention over the 4-bit cache within what its roundings are worth by weight.
+
+A row's error is held to the root of the sum of squares of every rounding's
+half step, each times the weight that it enters with: roundings of different
+keys are independent, so this is sqrt(3) times what they are expected to make.
+A value that has next to no weight adds nothing to the bound, however large."""
+import math
+
+import numpy as np
+import pytest
+
+import kv4_ref as R
+import q3t
+from test_gpu_kv4 import HALF, Setup, attend_case
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+H16 = 2.0 ** -11  # half a step of f16, relative to the value
+
+
+def weighed(q, S, scale, window, prompt, pool=None):
+    """(out, square of the bound) [T, heads, D] in float64 on the GPU."""
+    k_all, v_all, _, v_s = (torch.from_numpy(np.ascontiguousarray(x)).cuda() for x in
+                            R.unpack(S.pool if pool is None else pool, S.D))
+    q = q.double()
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    group = q.shape[1] // S.kvh
+    for s, n in enumerate(S.kv):
+        rows = slice(int(S.q_start[s]), int(S.q_start[s + 1]))
+        pos = torch.arange(n - S.new[s], n, device="cuda")[:, None]
+        at = [S.slot(s, p) for p in range(n)]
+        pg, sl = (torch.tensor([x[i] for x in at], device="cuda") for i in range(2))
+        key = torch.arange(n, device="cuda")[None, :]
+        see = (key <= pos) & ((key > pos - window) if window else True)
+        for h in range(q.shape[1]):
+            x, k, v = q[rows, h], k_all[pg, h // group, sl], v_all[pg, h // group, sl]
+            digits = 15 * v_s[pg, h // group, sl]
+            y = (x @ k.T * scale).masked_fill(~see, -math.inf)
+            w = torch.softmax(y, -1)
+            o = w @ v
+            # scores: exponents and their largest in 32 bits, to 2^-22 of each; for prompts K in 11 bits
+            y0 = y.masked_fill(~see, 0.0).abs()
+            ds = ((y0 + y0.amax(-1, keepdim=True) + 32) * 2.0 ** -22) ** 2
+            if prompt:
+                ds = ds + (scale * H16) ** 2 * (x * x) @ (k * k).T
+            e = w * w * ds
+            sq = e @ (v * v) - 2 * o * (e @ v) + o * o * e.sum(-1, keepdim=True)
+            # weights in 11 bits, for prompts values too; for decoding the weight is of the digits, at most 15 of them
+            sq = sq + H16 ** 2 * ((w * w) @ (2 * v * v if prompt else digits * digits))
+            # the smallest weights: f16 has steps of 2^-24, 2^-21 of the row's largest weight times value
+            sq = sq + n * (2.0 ** -21 * (w * v.abs().amax(-1)).amax(-1, keepdim=True)) ** 2
+            # values in f16 next to a larger one of the same key (16 keys where none is 2^10 times another)
+            sq = sq + n * (2.0 ** -29 * (w * v.abs().amax(-1)).amax(-1, keepdim=True)) ** 2
+            out[rows, h], bound[rows, h] = o, sq
+    return out, bound
+
+
+def check_weighed(got, q, S, window=0, scale=None, prompt=True, pool=None):
+    ref, sq = weighed(q, S, S.D ** -0.5 if scale is None else scale, window, prompt, pool)
+    err = got.double() - ref
+    assert torch.isfinite(got).all()
+    # the output's own rounding; and over all of a head's rows, roundings of different elements do not add up
+    whole = ((HALF * ref) ** 2 + sq).sum((0, 2)).sqrt()
+    assert (err.norm(dim=(0, 2)) <= whole).all(), (err.norm(dim=(0, 2)) / whole).max()
+    # an element: six deviations of the sum of its roundings (a rounding's is its half step over sqrt(3))
+    each = HALF * ref.abs() + 6 / math.sqrt(3) * sq.sqrt() + 1e-37
+    assert (err.abs() <= each).all(), (err.abs() / each).max()
+
+
+SHAPES = [  # D, kvh, group, new, past, window
+    (128, 1, 2, [600], [0], 0),
+    (128, 2, 2, [140], [700], 0),
+    (128, 2, 2, [20], [1500], 0),
+    (128, 1, 3, [100, 9, 60], [300, 900, 0], 150),
+    (64, 2, 4, [70, 10, 33], [450, 17, 5], 0),
+    (64, 1, 8, [40], [1100], 333),
+]
+
+
+@pytest.mark.parametrize("D, kvh, group, new, past, window", SHAPES)
+@pytest.mark.parametrize("workspace", [64 << 10, q3t.KV4_WORKSPACE])
+def test_prompts(D, kvh, group, new, past, window, workspace, monkeypatch):
+    """Ordinary values, tiles whole and with their keys divided."""
+    monkeypatch.setattr(q3t, "KV4_WORKSPACE", workspace)
+    S = Setup(D, kvh, new, past)
+    q = attend_case(S, group)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q, window=window), q, S, window)
+
+
+@pytest.mark.parametrize("D, kvh, group, new, past, window", [
+    (128, 2, 2, [1, 1, 2, 1], [700, 31, 2000, 4], 0), (64, 2, 4, [1, 1], [900, 77], 0), (128, 1, 5, [1, 3], [3000, 60], 100),
+    (64, 1, 12, [1], [4000], 0)])
+def test_decoding(D, kvh, group, new, past, window):
+    S = Setup(D, kvh, new, past)
+    q = attend_case(S, group)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q, window=window), q, S, window, prompt=False)
+
+
+def outlier_case(D, new, past, times, at, score, seed=0, group=2):
+    """Keys at positions `at` have values `times` the others' and, for every query, scores about `score` beside the
+    others' few."""
+    S = Setup(D, 1, [new], [past], seed=seed)
+    g, n = S.rng, S.kv[0]
+    k, v = (g.standard_normal((1, n, D)).astype(np.float32) for _ in range(2))
+    x = g.standard_normal((S.T, group, D)).astype(np.float32)
+    x[..., 0] = 8.0
+    k[0, at, 0] = score / (8 * D ** -0.5)
+    v[0, at] *= np.float32(times)
+    S.fill([k], [v])
+    return S, torch.from_numpy(x).cuda().bfloat16()
+
+
+# where the large values are: next to keys that have weight, in a page of their own, at the end of every page (rows of
+# a prompt before such a key must not see it, and share a page with it)
+PLACES = {"one": lambda n: [21], "page": lambda n: list(range(32, 48)), "ends": lambda n: list(range(15, n, 16))}
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", [(120, 90), (24, 1000), (300, 0)])
+@pytest.mark.parametrize("where", PLACES)
+@pytest.mark.parametrize("power", [9, 12, 16, 20, 26, 60])
+def test_prompts_with_large_values_of_no_weight(D, new, past, where, power):
+    S, q = outlier_case(D, new, past, 2.0 ** power, PLACES[where](new + past), -90.0)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", [(120, 90), (24, 1000)])
+@pytest.mark.parametrize("power", [12, 20, 40])
+def test_prompts_with_large_values_of_little_weight(D, new, past, power):
+    """Weight times value is that of the other keys, so both count."""
+    S, q = outlier_case(D, new, past, 2.0 ** power, [21, 60, 61], -power * math.log(2))
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", [(120, 90), (24, 1000)])
+@pytest.mark.parametrize("power", [-12, -30, -60])
+def test_prompts_with_small_values_of_most_weight(D, new, past, power):
+    """One key has nearly all the weight and next to no value: the others' values, by their small weights, are the
+    result."""
+    S, q = outlier_case(D, new, past, 2.0 ** power, [3], 12.0)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S)
+    S, q = outlier_case(D, new, past, 0.0, [3], 12.0)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S)

@@ -1389,20 +1389,26 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
 // schedulers, whose slots are 64 % taken (7900 warp instructions a tile, 40 %
 // of them unpacking, which 4-bit keys cost and bf16 ones would not).  The
 // tensor pipe is busy 27 %, HBM does not matter.  A prompt of 4096 tokens on 8
-// kv heads (68.7 GFLOP) takes 117 us, 0.35 of the products' rate alone.  With
+// kv heads (68.7 GFLOP) takes 120 us, 0.35 of the products' rate alone.  With
 // loops unrolled throughout, 102 KB of code instead of 62, warps waited for
 // instructions most of the time: 178 us.  One buffer of P, whose P V a softmax
-// then waits for: 122 us.
+// then waits for, is 5 us more; V's powers after the weights 3.5 us (by the
+// largest value alone, which is wrong where that has no weight, 116.6 us).
 //
 // Where tiles of rows cannot fill the GPU, CTAs share the keys of each and
 // k_kv4_join joins their parts: 32 rows of one request on 8000 keys, 126 tiles,
 // take 30 us.
 //
-// f16 holds q times a power of two per row, K and V times one per page (from
-// the largest value there, 11 bits of each), and p, with V's power relative to
-// the largest a row has seen.  A page's power of K enters with the score's
-// scale.  m, l, S and O are in 32 bits; m is moved, and O with it, only when a
-// score passes it by 2^8, which p in f16 can hold.
+// f16 holds q times a power of two per row, K times one per page and V times
+// one per page (from the largest value there, 11 bits of each), or per key where
+// a page has keys of less than 2^-10 of its largest.  A page's power of K enters
+// with the score's scale, V's with p: P of a key is 2^(score + V's power - ref),
+// and l sums it without V's power.  So ref follows the largest weight times value
+// that a row sees, not the largest value: one that has no weight takes no bits of
+// the others, nor does one that the row may not see.  l, S and O are in 32 bits;
+// ref is moved, and O with it, only when P would pass 2^15, and then to a P of 2^7,
+// so that P has all its bits from 2^-14 to there.  (K of a key below 2^-28 of the
+// largest of its page, and V's dims below that of their key's largest, lose bits.)
 //
 // What a row may not see must not touch it: K and V of keys that no row of the
 // tile sees are zeros, and a group that is no number becomes zeros too and is
@@ -1507,9 +1513,11 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   uint64_t *p_full = bars + 16, *pv_done = bars + 20, *q_full = bars + 24;
   __shared__ uint32_t tmem_slot;
   __shared__ __align__(16) float k_fac[8][PAGES];
-  __shared__ __align__(16) int v_exp[2][PAGES];
+  __shared__ __align__(16) float v_exp[2][PAGES], v_one[2][PAGES];     // of a page: V's power, and 2^-power
+  __shared__ __align__(16) float vk_exp[2][KEYS], vk_one[2][KEYS];  // the same of every key
   __shared__ uint8_t k_bad[8][KEYS], v_bad[2][KEYS];  // a key's groups that are no numbers: any of K's; of V's, by bit
-  __shared__ __align__(4) uint8_t k_says[8][PAGES], v_says[2][PAGES];  // of a page: bit 0 it is there, bit 1 such groups
+  // of a page: bit 0 it is there, bit 1 such groups, bit 2 keys of V have powers of their own
+  __shared__ __align__(4) uint8_t k_says[8][PAGES], v_says[2][PAGES];
   __shared__ int dead;  // a wait gave up
   uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t *sq = base, *sk = sq + 2 * Cfg::QB, *sv = sk + 2 * Cfg::KB, *sp = sv + 2 * Cfg::VB, *scales = sp + 4 * Cfg::PB,
@@ -1692,11 +1700,22 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         top = fmaxf(top, fmaxf(fabsf(z), fabsf(fmaf(15.f, bf2f(en[x] & 0xffffu), z))));
       }
       // (of values >= 0 the largest bits are the largest value's)
-      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fminf(top, FLT_MAX))));
+      top = fminf(top, FLT_MAX);
+      const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
       bad |= __shfl_xor_sync(0xffffffffu, bad, 16);  // lanes l and l + 16 hold a token's groups
       const int some = __any_sync(0xffffffffu, bad != 0u), token = 16 * w + 2 * (lane >> 2 & 3) + (lane & 1) + 8 * (lane >> 1 & 1);
       // {s, z} in f16, where every lane finds them
-      const float f = to_2p14(top);
+      float f = to_2p14(most);
+      bool own_powers = false;
+      if (is_v) {
+        // A key of zeros has a power that is small, so that it does not hold ref up, but lets l see its weight; no power is
+        // so small that a sum of 2^15 2^-power leaves 32 bits.
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const int key = key0 + 2 * (lane >> 2 & 3) + (lane & 1) + 8 * (lane >> 1 & 1);
+        own_powers = __any_sync(0xffffffffu, here && key <= pos_hi && key >= key_lo && top < most * 0x1p-10f);
+        const float from_top = own_powers ? top : most;
+        f = from_top == 0.f ? 0x1p60f : fminf(to_2p14(from_top), 0x1p90f);
+      }
 #pragma unroll
       for (int x = 0; x < EPL; x++)
         *reinterpret_cast<uint32_t *>(sc + 4 * (lane + 32 * x)) =
@@ -1720,10 +1739,13 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
             *reinterpret_cast<uint2 *>(to + (16 * m + 8) * 128) = make_uint2(o[1], o[3]);
           }
         }
-        if (lane < 16) v_bad[b][token] = (uint8_t)bad;
+        if (lane < 16) {
+          v_bad[b][token] = (uint8_t)bad;
+          vk_exp[b][token] = (float)-exponent(f), vk_one[b][token] = f;
+        }
         if (lane == 0) {
-          v_says[b][w] = (uint8_t)(2 * some);
-          v_exp[b][w] = -exponent(f);
+          v_says[b][w] = (uint8_t)(2 * some + 4 * own_powers);
+          v_exp[b][w] = (float)-exponent(f), v_one[b][w] = f;
         }
       } else {
         // rows are keys, D / 64 atoms of 64 dims; digits of keys g and g + 8
@@ -1807,8 +1829,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     const int all_from = a.window > 0 ? pos0 + (row0 + min(128 * h + 127, nrow - 1)) / gq - a.window + 1 : 0;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, t_s = tmem + lanes + 128 * h, t_o = tmem + lanes + 256 + 128 * h;
     uint8_t *my_p = sp + 2 * h * Cfg::PB + r * 128;
-    float m = -INFINITY, l = 0.f;  // m: what the exponents are taken from
-    int e_ref = -1000;             // power of two of O
+    float ref = -INFINITY, l = 0.f;  // ref: what exponents are taken from, those of O and l
     uint32_t nan = 0;              // of the keys this row has seen: bit j, V of group j; bit 7, K
 #pragma unroll 1
     for (int i = 0; i < nt; i++) {
@@ -1845,45 +1866,56 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
             if (!(y >> k & 1)) x[c][k] = 0xff800000u;
         }
       }
-      float top = -INFINITY;
+      float most[PAGES];  // of a page's scores
+      auto largest = [&] {
 #pragma unroll
-      for (int p = 0; p < PAGES; p++) {
-        float y = __uint_as_float(x[p >> 1][16 * (p & 1)]);
+        for (int p = 0; p < PAGES; p++) {
+          float y = __uint_as_float(x[p >> 1][16 * (p & 1)]);
 #pragma unroll
-        for (int k = 1; k < 16; k++) y = fmaxf(y, __uint_as_float(x[p >> 1][16 * (p & 1) + k]));
-        top = fmaxf(top, y * f[p]);
-      }
+          for (int k = 1; k < 16; k++) y = fmaxf(y, __uint_as_float(x[p >> 1][16 * (p & 1) + k]));
+          most[p] = y * f[p];
+        }
+      };
+      largest();
       wait(&v_full[b], (i >> 1) & 1);  // which means too that P V of tile i - 2 has been, and P may be written
       const uint32_t v_say = *reinterpret_cast<const uint32_t *>(v_says[b]);
-      const int4 v4 = *reinterpret_cast<const int4 *>(v_exp[b]);
-      const int ve[PAGES] = {v4.x, v4.y, v4.z, v4.w};
+      const float4 v4 = *reinterpret_cast<const float4 *>(v_exp[b]), o4 = *reinterpret_cast<const float4 *>(v_one[b]);
+      float ve[PAGES] = {v4.x, v4.y, v4.z, v4.w}, one[PAGES] = {o4.x, o4.y, o4.z, o4.w};
+      const bool own_powers = v_say & 0x04040404u;
+      if (own_powers) {  // V's powers into the scores, key by key
+#pragma unroll
+        for (int k = 0; k < KEYS; k += 4) {
+          const float4 e = *reinterpret_cast<const float4 *>(&vk_exp[b][k]);
+          uint32_t *y = &x[k >> 5][k & 31];
+          const uint64_t ff = f2_pack(f[k >> 4], f[k >> 4]);
+          float y0, y1, y2, y3;
+          f2_split(f2_fma(f2_pack(__uint_as_float(y[0]), __uint_as_float(y[1])), ff, f2_pack(e.x, e.y)), y0, y1);
+          f2_split(f2_fma(f2_pack(__uint_as_float(y[2]), __uint_as_float(y[3])), ff, f2_pack(e.z, e.w)), y2, y3);
+          y[0] = __float_as_uint(y0), y[1] = __float_as_uint(y1), y[2] = __float_as_uint(y2), y[3] = __float_as_uint(y3);
+        }
+#pragma unroll
+        for (int p = 0; p < PAGES; p++) f[p] = 1.f, ve[p] = one[p] = 0.f;  // (l has its share below)
+        largest();
+      }
       if ((k_say | v_say) & 0x02020202u)
 #pragma unroll 1
         for (int k = 0; k < KEYS; k++)
           if (see[k >> 5] >> (k & 31) & 1) nan |= v_bad[b][k] | (uint32_t)k_bad[q][k] << 7;
-      int e_new = e_ref;  // pages that this row sees nothing of do not count
-#pragma unroll
-      for (int p = 0; p < PAGES; p++)
-        if (see[p >> 1] >> 16 * (p & 1) & 0xffffu) e_new = max(e_new, ve[p]);
-      float scale_o = 1.f;
+      float scale_o = 1.f, top = -INFINITY;
       bool move = false;
-      if (top > m + 8.f) {  // the first time, or past what p in f16 holds
-        scale_o = m == -INFINITY ? 0.f : ex2(m - top);
-        m = top;
+#pragma unroll
+      for (int p = 0; p < PAGES; p++) top = fmaxf(top, most[p] + ve[p]);
+      if (top > ref + 15.f) {  // the first time, or past what P is to hold
+        const float to = top - 7.f;
+        scale_o = ref == -INFINITY ? 0.f : ex2(ref - to);
+        ref = to;
         l *= scale_o;
         move = true;
       }
-      if (e_new > e_ref) {
-        scale_o *= ex2((float)(e_ref - e_new));  // (0 the first time)
-        e_ref = e_new;
-        move = true;
-      }
-      const float mu = m == -INFINITY ? 0.f : m;
+      const float mu = ref == -INFINITY ? 0.f : ref;
 #pragma unroll
       for (int p = 0; p < PAGES; p++) {
-        // p with V's power in it, and the sum without; far below the largest V it does not matter how far
-        const int dv = min(max(ve[p] - e_ref, -100), 0);
-        const float c0 = (float)dv - mu;
+        const float c0 = ve[p] - mu;
         const uint64_t ff = f2_pack(f[p], f[p]), cc = f2_pack(c0, c0);
         uint64_t part = 0;
 #pragma unroll
@@ -1897,13 +1929,27 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
             y0 = ex2(y0), y1 = ex2(y1);
             part = f2_add(part, f2_pack(y0, y1));
             w[k] = pack_f16x2(y0, y1);
+            x[p >> 1][at] = __float_as_uint(y0), x[p >> 1][at + 1] = __float_as_uint(y1);
           }
           *reinterpret_cast<uint4 *>(my_p + b * Cfg::PB + (((2 * p + c) ^ (r & 7)) << 4)) =
               make_uint4(w[0], w[1], w[2], w[3]);
         }
         float s0, s1;
         f2_split(part, s0, s1);
-        l = fmaf(s0 + s1, __uint_as_float((uint32_t)(127 - dv) << 23), l);
+        l = fmaf(s0 + s1, one[p], l);
+      }
+      if (own_powers) {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int k = 0; k < KEYS; k += 4) {
+          const float4 o = *reinterpret_cast<const float4 *>(&vk_one[b][k]);
+          const uint32_t *y = &x[k >> 5][k & 31];
+          sum = f2_fma(f2_pack(__uint_as_float(y[0]), __uint_as_float(y[1])), f2_pack(o.x, o.y), sum);
+          sum = f2_fma(f2_pack(__uint_as_float(y[2]), __uint_as_float(y[3])), f2_pack(o.z, o.w), sum);
+        }
+        float s0, s1;
+        f2_split(sum, s0, s1);
+        l += s0 + s1;
       }
       if (i > 0 && __any_sync(0xffffffffu, move)) {
         wait(&pv_done[2 * h + (b ^ 1)], ((i - 1) >> 1) & 1);  // O is whole
@@ -1924,10 +1970,15 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     if (nt > 0) wait(&pv_done[2 * h + ((nt - 1) & 1)], ((nt - 1) >> 1) & 1);
     tc_fence_after();
     const bool gone = *(volatile int *)&dead;
-    const float up = exp2f((float)max(e_ref, -126)), inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     float *part = splits > 1 ? ks.parts + (size_t)blockIdx.x * Cfg::PART + threadIdx.x : nullptr;
     const bool in_tile = (int)threadIdx.x < nrow;
-    if (part && in_tile) part[0] = m, part[ROWS] = gone ? __uint_as_float(0x7fc00000u) : l;
+    // a part weighs l 2^ref, here as a number from 1 to 2 and an exponent: ref has V's powers, which may be far apart
+    if (part && in_tile) {
+      const int e = l == 0.f ? 0 : exponent(l);
+      part[0] = ref + (float)e;
+      part[ROWS] = gone ? __uint_as_float(0x7fc00000u) : l * __uint_as_float((uint32_t)(127 - min(e, 126)) << 23);
+    }
 #pragma unroll 1
     for (int c = 0; c < D / 32; c++) {
       uint32_t x[32];
@@ -1945,8 +1996,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         float4 *to = reinterpret_cast<float4 *>(part - threadIdx.x + 2 * ROWS) + threadIdx.x;
 #pragma unroll
         for (int k = 0; k < 8; k++)
-          if (in_tile) to[(8 * c + k) * ROWS] = make_float4(__uint_as_float(x[4 * k]) * f1 * up, __uint_as_float(x[4 * k + 1]) * f1 * up,
-                                               __uint_as_float(x[4 * k + 2]) * f1 * up, __uint_as_float(x[4 * k + 3]) * f1 * up);
+          if (in_tile) to[(8 * c + k) * ROWS] = make_float4(__uint_as_float(x[4 * k]) * f1, __uint_as_float(x[4 * k + 1]) * f1,
+                                               __uint_as_float(x[4 * k + 2]) * f1, __uint_as_float(x[4 * k + 3]) * f1);
         continue;
       }
 #pragma unroll
@@ -1954,7 +2005,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         uint32_t y[4];
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          y[e] = pack_bf16x2(__uint_as_float(x[8 * k + 2 * e]) * f1 * up, __uint_as_float(x[8 * k + 2 * e + 1]) * f1 * up);
+          y[e] = pack_bf16x2(__uint_as_float(x[8 * k + 2 * e]) * f1, __uint_as_float(x[8 * k + 2 * e + 1]) * f1);
         *q_at(threadIdx.x, 4 * c + k) = make_uint4(y[0], y[1], y[2], y[3]);  // (this half's S are done with Q)
       }
     }
@@ -1995,8 +2046,8 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
 // Joins the parts of k_kv4_prompt's tiles, where it divided the keys: a thread
 // has a row, eight dims of it (32 to a thread, one part after the other, took
 // 33 us for 18 parts: all of it waiting for loads).  A part's o is divided by
-// its l already, so a part weighs l 2^m; parts come in order, and the result
-// does not depend on timing.
+// its l already, so a part weighs l 2^m (l from 1 to 2, or 0); parts come in
+// order, and the result does not depend on timing.
 template <int D>
 __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4AttendArgs a, PromptSplit sp) {
   using Cfg = PromptCfg<D>;
