@@ -19,3 +19,17 @@ def test_attend_of_groups_wider_than_a_launch_lists(D, group):
     q = attend_case(S, group)
     cache, batch = S.on_gpu(0, 0)
     check_attend(cache.attend(batch, q), q, S, 0, key_bits=11)
+
+
+@pytest.mark.parametrize("new, kv", [([60, 300, 30], [25, 20, 0]), ([6, 1, 3], [3, 1, 0]), ([5, 70], [1, 40])])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 3])
+@pytest.mark.parametrize("hints", [True, False])
+def test_attend_of_padding_under_the_widest_windows(new, kv, window, hints):
+    """A window beyond every position is none, for rows that share a unit or a tile with ones in front of position 0."""
+    S = Setup(128, 2, new, [0] * len(new))
+    q = attend_case(S, 2)
+    S.kv = kv
+    cache, batch = S.on_gpu(*(() if hints else (0, 0)))
+    out = cache.attend(batch, q, window=window)
+    assert torch.equal(out, cache.attend(batch, q))
+    check_attend(out, q, S, 0, key_bits=11)

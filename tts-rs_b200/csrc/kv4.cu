@@ -686,6 +686,9 @@ struct Unit {
 };
 // token of a query row: a decode step has one, and no division then
 Q3T_DEV int token_of(int row, int gq) { return row < gq ? 0 : row / gq; }
+// the first key that the row at `pos` sees: a difference only where it does not pass 0, as `pos` may be far below it and
+// `window` near the largest number
+Q3T_DEV int first_key(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
 template <int R>
 Q3T_DEV Unit unit_of(const SeqRows &s, int row0, int gq, int window, int table_stride) {
   Unit u;
@@ -693,7 +696,7 @@ Q3T_DEV Unit unit_of(const SeqRows &s, int row0, int gq, int window, int table_s
   u.nrow = min(R, s.total - row0);
   u.pos_lo = s.pos0 + token_of(row0, gq);
   u.pos_hi = s.pos0 + token_of(row0 + max(u.nrow, 1) - 1, gq);
-  u.pg_lo = window > 0 ? max(0, u.pos_lo - window + 1) >> 4 : 0;
+  u.pg_lo = first_key(u.pos_lo, window) >> 4;
   u.pages = u.pos_hi < 0 ? 0 : max(0, min((u.pos_hi >> 4) + 1, table_stride) - u.pg_lo);  // none past the table
   return u;
 }
@@ -903,7 +906,7 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
       qs[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
       sc[nt] = __shfl_sync(0xffffffffu, a.scale == 0.f ? 1.f : a.scale * 0x1p24f / f, 8 * t);
       lim[nt] = sq.pos0 + token_of(min(u.row0 + (nt * 8 + 2 * t) / G, sq.total - 1), gq);
-      low[nt] = a.window > 0 ? lim[nt] - a.window + 1 : 0;
+      low[nt] = first_key(lim[nt], a.window);
     }
     int next = seq;  // the unit after this one, its queries on their way
     if (i1 - i0 < to - at) {
@@ -985,7 +988,7 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
         // the slot holds, scales that are no numbers included, does not count
         const bool there = here >> k & 1;
         const int key0 = (p0 + k) * 16;
-        if (!there || key0 + 15 > pos_lo || (a.window > 0 && key0 < pos_hi - a.window + 1)) {
+        if (!there || key0 + 15 > pos_lo || key0 < first_key(pos_hi, a.window)) {
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             const int key = key0 + g + 8 * h;
@@ -1546,7 +1549,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   const int total = n * gq, row0 = ((total + ROWS - 1) / ROWS - 1 - i_rev) * ROWS;  // the longest tiles first
   const int nrow = min(ROWS, total - row0);
   const int pos_lo = pos0 + row0 / gq, pos_hi = pos0 + (row0 + nrow - 1) / gq;
-  const int key_lo = a.window > 0 ? max(0, pos_lo - a.window + 1) : 0;
+  const int key_lo = first_key(pos_lo, a.window);
   int pg_lo = key_lo >> 4;
   // tiles of keys that the first 128 rows see, and the others; both begin at page pg_lo
   auto pages_to = [&](int pos) { return pos < 0 ? 0 : max(0, min((pos >> 4) + 1, a.c.table_stride) - pg_lo); };
@@ -1823,10 +1826,10 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     const int h = threadIdx.x >> 7, r = threadIdx.x & 127, nt = h ? nt1 : nt0;
     int tok, hd;
     row_at(threadIdx.x, tok, hd);
-    const int lim = pos0 + tok, low = a.window > 0 ? lim - a.window + 1 : 0;
+    const int lim = pos0 + tok, low = first_key(lim, a.window);
     // keys that all rows of this half see
     const int all_to = pos0 + (row0 + min(128 * h, nrow - 1)) / gq;
-    const int all_from = a.window > 0 ? pos0 + (row0 + min(128 * h + 127, nrow - 1)) / gq - a.window + 1 : 0;
+    const int all_from = first_key(pos0 + (row0 + min(128 * h + 127, nrow - 1)) / gq, a.window);
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, t_s = tmem + lanes + 128 * h, t_o = tmem + lanes + 256 + 128 * h;
     uint8_t *my_p = sp + 2 * h * Cfg::PB + r * 128;
     float ref = -INFINITY, l = 0.f;  // ref: what exponents are taken from, those of O and l
