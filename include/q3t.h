@@ -629,12 +629,13 @@ q3t_status q3t_kv4_append(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch
 /* Attention of the batch's query rows over the cache: the row at position p
  * sees the sequence's keys 0..p (window > 0: the last `window` of them), the
  * appended ones among them; out = softmax(scale q . k) v in bf16, query head h
- * reading kv head h / (num_heads / num_kv_heads).  Keys whose position has no
- * page are not seen; a row that sees no key gives zeros.  out must not
- * overlap q.  workspace: device memory on a 16-byte boundary that this call
- * alone uses while it runs (calls that may overlap, and graphs that may replay
- * at once, need one each); it needs no initialisation and holds nothing
- * between calls.  64 KiB at least; Q3T_KV4_WORKSPACE serves the widest launch. */
+ * reading kv head h / (num_heads / num_kv_heads).  |scale| is at most 2^127.
+ * Keys whose position has no page are not seen; a row that sees no key gives
+ * zeros.  out must not overlap q.  workspace: device memory on a 16-byte
+ * boundary that this call alone uses while it runs (calls that may overlap, and
+ * graphs that may replay at once, need one each); it needs no initialisation
+ * and holds nothing between calls.  64 KiB at least; Q3T_KV4_WORKSPACE serves
+ * the widest launch. */
 #define Q3T_KV4_WORKSPACE (20 << 20)
 q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, int num_heads, const uint16_t *q,
                           int64_t q_stride, float scale, int window, uint16_t *out, int64_t out_stride,

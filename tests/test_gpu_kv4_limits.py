@@ -33,3 +33,16 @@ def test_attend_of_padding_under_the_widest_windows(new, kv, window, hints):
     out = cache.attend(batch, q, window=window)
     assert torch.equal(out, cache.attend(batch, q))
     check_attend(out, q, S, 0, key_bits=11)
+
+
+@pytest.mark.parametrize("new, past", [([1, 1], [40, 21]), ([30, 1], [70, 5])])
+@pytest.mark.parametrize("scale, rows", [(1e-20, 1.0), (-1e-38, 1.0), (1e35, 1e-35), (-3e37, 1e-37), (1e-36, 1e36)])
+def test_attend_of_extreme_scales(new, past, scale, rows):
+    """Scales near both ends of 32 bits, over rows of zeros and ones whose scores come out ordinary or as nothing."""
+    S = Setup(128, 1, new, past)
+    q = attend_case(S, 2) * rows
+    q[-1, 0] = 0
+    q[0, 1] = 0
+    cache, batch = S.on_gpu()
+    out = cache.attend(batch, q, scale=scale)
+    check_attend(out, q, S, 0, scale=float(np.float32(scale)), key_bits=11)

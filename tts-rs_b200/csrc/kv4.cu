@@ -904,7 +904,9 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
       sum *= f * 0x1p-24f;
       qs[nt][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
       qs[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-      sc[nt] = __shfl_sync(0xffffffffu, a.scale == 0.f ? 1.f : a.scale * 0x1p24f / f, 8 * t);
+      // (2^24 where it can neither pass 32 bits nor vanish before its time; never 0, as -inf times it has to stay that)
+      const float back = f < 1.f && f > -1.f ? a.scale / f * 0x1p24f : a.scale * (0x1p24f / f);
+      sc[nt] = __shfl_sync(0xffffffffu, a.scale == 0.f ? 1.f : fminf(fmaxf(back, FLT_MIN), FLT_MAX), 8 * t);
       lim[nt] = sq.pos0 + token_of(min(u.row0 + (nt * 8 + 2 * t) / G, sq.total - 1), gq);
       low[nt] = first_key(lim[nt], a.window);
     }
@@ -2511,7 +2513,7 @@ extern "C" q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_b
     if (num_heads < 1 || num_heads > (1 << 16) || num_heads % a.c.n_kv)
       FAIL(Q3T_INVALID_INPUT, "%s: num_heads %d is not a multiple of the %d kv heads within 65536", what, num_heads,
            a.c.n_kv);
-    if (!std::isfinite(scale)) FAIL(Q3T_INVALID_INPUT, "%s: scale must be finite", what);
+    if (!(std::fabs(scale) <= 0x1p127f)) FAIL(Q3T_INVALID_INPUT, "%s: scale %g is not within 2^127", what, (double)scale);
     if (window < 0) FAIL(Q3T_INVALID_INPUT, "%s: negative window", what);
     if (a.b.num_seqs == 0 || a.b.num_tokens == 0) return;
     check_rows(what, "q", q, q_stride, num_heads, a.c.head_dim, 2);
