@@ -46,3 +46,21 @@ def test_attend_of_extreme_scales(new, past, scale, rows):
     cache, batch = S.on_gpu()
     out = cache.attend(batch, q, scale=scale)
     check_attend(out, q, S, 0, scale=float(np.float32(scale)), key_bits=11)
+
+
+@pytest.mark.parametrize("kv", [-(2 ** 31), -(2 ** 31) + 5, -7])
+@pytest.mark.parametrize("new", [[2, 1], [30, 40]])
+def test_lengths_below_zero_are_padding(kv, new):
+    """Every row is in front of position 0: an append skips it, attend and read give zeros."""
+    S = Setup(128, 2, new, [40, 30])
+    q = attend_case(S, 2)
+    S.kv = [kv, kv]
+    cache, batch = S.on_gpu(0, 0)
+    before = S.d_pool.clone()
+    k, v = (torch.randn(S.T, 2, 128, device="cuda") for _ in range(2))
+    q_out = torch.full_like(q, 3.0)
+    cache.append(batch, k, v, q=q.float(), q_out=q_out)
+    assert torch.equal(S.d_pool, before) and (q_out == 3.0).all()
+    assert all((t == 0).all() for t in cache.read(batch))
+    for window in (0, 5):
+        assert (cache.attend(batch, q, window=window) == 0).all()

@@ -37,12 +37,13 @@ namespace {
 // Which rows a CTA works on
 // ---------------------------------------------------------------------------
 // Token rows [t0, t0 + n) of sequence s, clamped to the call's rows; the
-// last sits at position kv_len - 1.
+// last sits at position kv_len - 1.  (A length below 0 is as one of 0: all its
+// rows are in front of position 0, and no position passes 32 bits.)
 Q3T_DEV void seq_rows(const Kv4Batch &b, int s, int &t0, int &n, int &pos0) {
   const int lo = min(max(b.q_start[s], 0), b.num_tokens), hi = min(max(b.q_start[s + 1], lo), b.num_tokens);
   t0 = lo;
   n = hi - lo;
-  pos0 = b.kv_len[s] - n;
+  pos0 = max(b.kv_len[s], 0) - n;
 }
 
 // Page of positions [16 p, 16 p + 16) of sequence s; -1 where the table or
