@@ -151,3 +151,59 @@ def test_prompts_with_small_values_of_most_weight(D, new, past, power):
     S, q = outlier_case(D, new, past, 0.0, [3], 12.0)
     cache, batch = S.on_gpu()
     check_weighed(cache.attend(batch, q), q, S)
+
+
+DECODING = [(1, 200), (1, 9000), (3, 700)]  # a warp's, many CTAs' and a few rows of which the last key is the last row's
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", DECODING)
+@pytest.mark.parametrize("where", [*PLACES, "last"])
+@pytest.mark.parametrize("power", [12, 20, 30, 40, 100])
+def test_decoding_with_large_values_of_no_weight(D, new, past, where, power):
+    n = new + past
+    S, q = outlier_case(D, new, past, 2.0 ** power, [n - 1] if where == "last" else PLACES[where](n), -120.0)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S, prompt=False)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", DECODING)
+@pytest.mark.parametrize("power", [12, 40, 80, -12, -60])
+def test_decoding_with_weight_and_size_apart(D, new, past, power):
+    """Large values of little weight, that count as much as the others; small values, or none, of most weight."""
+    S, q = outlier_case(D, new, past, 2.0 ** power, [21, 60, 61], -power * math.log(2) if power > 0 else 12.0)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S, prompt=False)
+    S, q = outlier_case(D, new, past, 0.0, [3], 12.0)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S, prompt=False)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", [(1, 200), (1, 9000), (24, 1000)])
+@pytest.mark.parametrize("low, high", [(-100, 100), (100, -100), (-90, 20)])
+def test_sizes_that_grow_and_shrink_along_the_cache(D, new, past, low, high):
+    """Parts of a row's keys whose values are hundreds of powers of two apart: each counts by its weight."""
+    S = Setup(D, 1, [new], [past])
+    g, n = S.rng, S.kv[0]
+    k, v = (g.standard_normal((1, n, D)) for _ in range(2))
+    v *= 2.0 ** np.round(np.linspace(low, high, n))[None, :, None]
+    S.fill([k.astype(np.float32)], [v.astype(np.float32)])
+    q = torch.from_numpy(g.standard_normal((S.T, 2, D)).astype(np.float32)).cuda().bfloat16()
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S, prompt=new > 1)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", [(1, 200), (1, 9000), (24, 1000)])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 120, -(2.0 ** -90)])
+def test_constant_values(D, new, past, size):
+    """Groups without a scale: digits of zeros, and the zero is the value."""
+    S = Setup(D, 1, [new], [past])
+    g, n = S.rng, S.kv[0]
+    k = g.standard_normal((1, n, D)).astype(np.float32)
+    S.fill([k], [np.full((1, n, D), size, np.float32)])
+    q = torch.from_numpy(g.standard_normal((S.T, 2, D)).astype(np.float32)).cuda().bfloat16()
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S, prompt=new > 1)

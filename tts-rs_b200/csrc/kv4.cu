@@ -635,10 +635,13 @@ __global__ void __launch_bounds__(kReadThreads) k_kv4_read(const __grid_constant
 // 94).  Short ones are bound by both ends: 64 of 100 to 1500 keys 27 us.
 //
 // f16 holds q times a power of two per row (its 11 bits keep a bf16 q whole
-// down to 2^-25 of the row's largest) and p s, where p carries a power of two
-// per warp that follows the largest value scale (m is offset by its logarithm,
-// so l and o carry it too and it leaves with the division): p s is rounded to
-// 11 bits, as against the 8 of the output.  All sums, m and l are in 32 bits.
+// down to 2^-25 of the row's largest) and p s, which is rounded to 11 bits, as
+// against the 8 of the output.  p is taken from a reference that follows the
+// largest weight times scale that a row has seen, not the largest scale: p s is
+// at most 2^15, and 2^10 where the reference moves, so it has all its bits down
+// to 2^-24 of the row's largest, and values that have no weight, or that the row
+// may not see, cost the others nothing.  l and o carry the reference too, and it
+// leaves with the division.  All sums, references and l are in 32 bits.
 // ---------------------------------------------------------------------------
 Q3T_DEV void mma_f16(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
@@ -653,6 +656,11 @@ Q3T_DEV uint32_t pack_f16x2(float lo, float hi) {
 Q3T_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+Q3T_DEV float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 // 2^(14 - exponent of x), so that x times it lies in [2^14, 2^15)
@@ -918,18 +926,17 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
       load_q(next, raw_q);
     }
 
-    // p = 2^(x sc - mu), mu = m sc - lv: m the largest x = score / sc so far,
-    // lv the power of two that p carries
-    float m[NT], mu[NT], l[NT], zac[NT][2], acc[NT][MT][4];
+    // p = 2^(x sc - mu), mu = ref where a key has been seen and 0 before: ref follows the largest weight times size,
+    // x sc + log2 of a key's size, so that p s is up to 2^15
+    float ref[NT], mu[NT], l[NT], zac[NT][2], acc[NT][MT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      m[nt] = -INFINITY;
+      ref[nt] = -INFINITY;
       mu[nt] = 0.f;
       l[nt] = zac[nt][0] = zac[nt][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; i++) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
     }
-    float lv = 0.f, vcap = 0.f;  // and the largest value scale that it is good for
 
     for (int it = i0; it < i1; it++) {
       copies();
@@ -1006,41 +1013,41 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
           }
         }
       }
-      // ---- running maximum, largest value scale ----
-      float top = 0.f, mx[NT];
+      // ---- largest weight times size ----
+      float top[NT];
 #pragma unroll
-      for (int i = 0; i < 4 * NP; i++) top = fmaxf(top, bf2f(vz[i >> 2][i >> 1 & 1][i & 1] & 0xffffu));
-      bool moved = top > vcap;
+      for (int nt = 0; nt < NT; nt++) top[nt] = -INFINITY;
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        mx[nt] = m[nt];
+      for (int i = 0; i < 2 * NP; i++) {
+        // A key's size is its largest scale.  Zeros count too, from 2^20 times that on, so that p times them stays in 32
+        // bits, and so do sizes below 2^-86, for p's own sake.
+        const uint32_t v0 = vz[i >> 1][i & 1][0], v1 = vz[i >> 1][i & 1][1];
+        const float zero = fmaxf(fabsf(__uint_as_float(v0 & 0xffff0000u)), fabsf(__uint_as_float(v1 & 0xffff0000u)));
+        const float size = fmaxf(fmaxf(bf2f(v0 & 0xffffu), bf2f(v1 & 0xffffu)), fmaxf(zero * 0x1p-20f, 0x1p-86f));
+        const float e = lg2(size);
 #pragma unroll
-        for (int i = 0; i < 2 * NP; i++) mx[nt] = fmaxf(mx[nt], x[nt][i >> 1][i & 1]);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) mx[nt] = fmaxf(mx[nt], __shfl_xor_sync(0xffffffffu, mx[nt], o));
-        moved |= mx[nt] != m[nt];
+        for (int nt = 0; nt < NT; nt++) top[nt] = fmaxf(top[nt], fmaf(x[nt][i >> 1][i & 1], sc[nt], e));
       }
+      bool moved = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) moved |= top[nt] > ref[nt] + 15.f;
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (top > vcap) {  // p s < 2^15
-          const int e = max(exponent(top), -86);
-          lv = (float)(14 - e);
-          vcap = __uint_as_float((uint32_t)(min(e + 1, 127) + 127) << 23);
-        }
-#pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          const float to = (mx[nt] == -INFINITY ? 0.f : mx[nt] * sc[nt]) - lv;
-          const float f = m[nt] == -INFINITY ? 0.f : ex2(mu[nt] - to);  // nothing summed yet, or as much as p shrinks
-          m[nt] = mx[nt];
-          mu[nt] = to;
-          l[nt] *= f;
-          zac[nt][0] *= f;
-          zac[nt][1] *= f;
 #pragma unroll
-          for (int i = 0; i < MT; i++)
+          for (int o = G == 4 ? 1 : 4; o < 32; o = o == 1 ? 4 : 2 * o)  // over a row's keys, and its lanes' groups
+            top[nt] = fmaxf(top[nt], __shfl_xor_sync(0xffffffffu, top[nt], o));
+          if (top[nt] > ref[nt] + 15.f) {  // the first time, or past what p s is to hold
+            const float to = top[nt] - 10.f, f = ref[nt] == -INFINITY ? 0.f : ex2(ref[nt] - to);
+            ref[nt] = mu[nt] = to;
+            l[nt] *= f;
+            zac[nt][0] *= f;
+            zac[nt][1] *= f;
 #pragma unroll
-            for (int e = 0; e < 4; e++) acc[nt][i][e] *= f;
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) acc[nt][i][e] *= f;
+          }
         }
       }
       // ---- p, p s and the value product ----
@@ -1109,12 +1116,16 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
         zac[nt][1] += __shfl_xor_sync(0xffffffffu, zac[nt][1], o);
       }
       const int r = (nt * 8 + 2 * t) / G, ja = 2 * t % G;
+      // l as a number from 1 to 2 and an exponent, which ref takes: refs may be so far apart that one of two parts of
+      // like weight would have none.  (0 and no number stay that.)
+      const int el = l[nt] == 0.f ? 0 : min(exponent(l[nt]), 126);
+      const float fl = __uint_as_float((uint32_t)(127 - el) << 23);
       if (g == 0) {
-        p_z[r * G + ja] = zac[nt][0];
-        p_z[r * G + ja + 1] = zac[nt][1];
+        p_z[r * G + ja] = zac[nt][0] * fl;
+        p_z[r * G + ja + 1] = zac[nt][1] * fl;
         if (ja == 0) {
-          p_m[r] = m[nt] == -INFINITY ? m[nt] : mu[nt];
-          p_l[r] = l[nt];
+          p_m[r] = ref[nt] + (float)el;
+          p_l[r] = l[nt] * fl;
         }
       }
 #pragma unroll
@@ -1122,8 +1133,8 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
 #pragma unroll
         for (int e = 0; e < 2; e++)
           if (ja + e == i / 2) {  // digits were n 2^-24 and 16 n 2^-24
-            p_o[r * D + 16 * i + g] = acc[nt][i][e] * 0x1p24f;
-            p_o[r * D + 16 * i + 8 + g] = acc[nt][i][2 + e] * 0x1p20f;
+            p_o[r * D + 16 * i + g] = acc[nt][i][e] * 0x1p24f * fl;
+            p_o[r * D + 16 * i + 8 + g] = acc[nt][i][2 + e] * 0x1p20f * fl;
           }
     }
     __syncwarp();
