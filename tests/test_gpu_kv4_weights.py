@@ -207,3 +207,15 @@ def test_constant_values(D, new, past, size):
     q = torch.from_numpy(g.standard_normal((S.T, 2, D)).astype(np.float32)).cuda().bfloat16()
     cache, batch = S.on_gpu()
     check_weighed(cache.attend(batch, q), q, S, prompt=new > 1)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", [(120, 90), (24, 1000), (300, 0)])
+@pytest.mark.parametrize("where", PLACES)
+@pytest.mark.parametrize("power", [9, 16, 30, 40, 90])
+def test_prompts_with_large_keys_that_rows_do_not_see_or_score_low(D, new, past, where, power):
+    """A key of large dims beside ordinary ones in its page: rows in front of it do not see it, rows behind it score it
+    far below the others."""
+    S, q = outlier_case(D, new, past, 1.0, PLACES[where](new + past), -2.0 ** power)
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S)

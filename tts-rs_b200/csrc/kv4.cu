@@ -1416,16 +1416,15 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
 // k_kv4_join joins their parts: 32 rows of one request on 8000 keys, 126 tiles,
 // take 30 us.
 //
-// f16 holds q times a power of two per row, K times one per page and V times
-// one per page (from the largest value there, 11 bits of each), or per key where
-// a page has keys of less than 2^-10 of its largest.  A page's power of K enters
-// with the score's scale, V's with p: P of a key is 2^(score + V's power - ref),
+// f16 holds q times a power of two per row, K and V times one per page (from the
+// largest value there, 11 bits of each), or per key where a page has keys of less
+// than 2^-10 of its largest.  K's power enters with the score's scale, V's with p: P of a key is 2^(score + V's power - ref),
 // and l sums it without V's power.  So ref follows the largest weight times value
 // that a row sees, not the largest value: one that has no weight takes no bits of
 // the others, nor does one that the row may not see.  l, S and O are in 32 bits;
 // ref is moved, and O with it, only when P would pass 2^15, and then to a P of 2^7,
-// so that P has all its bits from 2^-14 to there.  (K of a key below 2^-28 of the
-// largest of its page, and V's dims below that of their key's largest, lose bits.)
+// so that P has all its bits from 2^-14 to there.  (Dims below 2^-28 of their
+// key's largest lose bits.)
 //
 // What a row may not see must not touch it: K and V of keys that no row of the
 // tile sees are zeros, and a group that is no number becomes zeros too and is
@@ -1529,11 +1528,11 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
   // and a thread that asks for a phase may find one or two more done (a parity names only the next one)
   uint64_t *p_full = bars + 16, *pv_done = bars + 20, *q_full = bars + 24;
   __shared__ uint32_t tmem_slot;
-  __shared__ __align__(16) float k_fac[8][PAGES];
+  __shared__ __align__(16) float k_fac[8][PAGES], kk_fac[8][KEYS];  // 2^-power of a page of K, and of keys that have their own
   __shared__ __align__(16) float v_exp[2][PAGES], v_one[2][PAGES];     // of a page: V's power, and 2^-power
   __shared__ __align__(16) float vk_exp[2][KEYS], vk_one[2][KEYS];  // the same of every key
   __shared__ uint8_t k_bad[8][KEYS], v_bad[2][KEYS];  // a key's groups that are no numbers: any of K's; of V's, by bit
-  // of a page: bit 0 it is there, bit 1 such groups, bit 2 keys of V have powers of their own
+  // of a page: bit 0 it is there, bit 1 such groups, bit 2 its keys have powers of their own
   __shared__ __align__(4) uint8_t k_says[8][PAGES], v_says[2][PAGES];
   __shared__ int dead;  // a wait gave up
   uint8_t *base = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -1722,17 +1721,14 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       bad |= __shfl_xor_sync(0xffffffffu, bad, 16);  // lanes l and l + 16 hold a token's groups
       const int some = __any_sync(0xffffffffu, bad != 0u), token = 16 * w + 2 * (lane >> 2 & 3) + (lane & 1) + 8 * (lane >> 1 & 1);
       // {s, z} in f16, where every lane finds them
-      float f = to_2p14(most);
-      bool own_powers = false;
-      if (is_v) {
-        // A key of zeros has a power that is small, so that it does not hold ref up, but lets l see its weight; no power is
-        // so small that a sum of 2^15 2^-power leaves 32 bits.
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        const int key = key0 + 2 * (lane >> 2 & 3) + (lane & 1) + 8 * (lane >> 1 & 1);
-        own_powers = __any_sync(0xffffffffu, here && key <= pos_hi && key >= key_lo && top < most * 0x1p-10f);
-        const float from_top = own_powers ? top : most;
-        f = from_top == 0.f ? 0x1p60f : fminf(to_2p14(from_top), 0x1p90f);
-      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      const int key = key0 + 2 * (lane >> 2 & 3) + (lane & 1) + 8 * (lane >> 1 & 1);
+      const bool own_powers = __any_sync(0xffffffffu, here && key <= pos_hi && key >= key_lo && top < most * 0x1p-10f);
+      if (!own_powers) top = most;
+      float f = to_2p14(top);
+      // A key of V that is zeros has a power that is small, so that it does not hold ref up, but lets l see its weight; no
+      // power of V is so small that a sum of 2^15 2^-power leaves 32 bits.
+      if (is_v) f = top == 0.f ? 0x1p60f : fminf(f, 0x1p90f);
 #pragma unroll
       for (int x = 0; x < EPL; x++)
         *reinterpret_cast<uint32_t *>(sc + 4 * (lane + 32 * x)) =
@@ -1784,9 +1780,10 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
         // K of tile i + 7 waits for a score of tile i + 5, that for a softmax to be
         // done with tile i + 2, that for V, which waits for every P V of tile i.
         if (lane < 16) k_bad[i & 7][token] = bad != 0u;
+        if (own_powers && lane < 16) kk_fac[i & 7][token] = 1.f / f;
         if (lane == 0) {
           k_fac[i & 7][w] = 1.f / f;
-          k_says[i & 7][w] = (uint8_t)(here + 2 * some);
+          k_says[i & 7][w] = (uint8_t)(here + 2 * some + 4 * own_powers);
         }
       }
       fence_proxy_async();
@@ -1858,7 +1855,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       tmem_ld32_async(t_s + KEYS * b + 32, x[1]);
       const uint32_t k_say = *reinterpret_cast<const uint32_t *>(k_says[q]);
       const float4 k4 = *reinterpret_cast<const float4 *>(k_fac[q]);
-      const bool edge = key0 + KEYS - 1 > all_to || key0 < all_from || (k_say & 0x01010101u) != 0x01010101u;
+      const bool edge = key0 + KEYS - 1 > all_to || key0 < all_from || (k_say & 0x05050505u) != 0x01010101u;
       // a score of page p is its column times f[p]; zero rows and pages keep it off 0 and infinity
       float f[PAGES] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
@@ -1868,6 +1865,16 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
       mbar_arrive(&s_freed[2 * h + b]);
       uint32_t see[2] = {0xffffffffu, 0xffffffffu};
       if (edge) {
+        if (k_say & 0x04040404u) {  // keys' own powers into their scores
+#pragma unroll
+          for (int k = 0; k < KEYS; k++) {
+            const float own = fminf(fmaxf(q_back * kk_fac[q][k], 0x1p-100f), 0x1p100f);
+            x[k >> 5][k & 31] =
+                __float_as_uint(__uint_as_float(x[k >> 5][k & 31]) * (k_say >> (8 * (k >> 4) + 2) & 1 ? own : f[k >> 4]));
+          }
+#pragma unroll
+          for (int p = 0; p < PAGES; p++) f[p] = 1.f;
+        }
         // bits of the keys that this row sees
         const int last = lim - key0, first = low - key0;
 #pragma unroll
