@@ -21,7 +21,7 @@ H16 = 2.0 ** -11  # half a step of f16, relative to the value
 
 
 def weighed(q, S, scale, window, prompt, pool=None):
-    """(out, square of the bound) [T, heads, D] in float64 on the GPU."""
+    """(out, square of the bound) [T, heads, D] in float64 on the GPU.  prompt: whose roundings, None for either's."""
     k_all, v_all, _, v_s = (torch.from_numpy(np.ascontiguousarray(x)).cuda() for x in
                             R.unpack(S.pool if pool is None else pool, S.D))
     q = q.double()
@@ -33,7 +33,8 @@ def weighed(q, S, scale, window, prompt, pool=None):
         at = [S.slot(s, p) for p in range(n)]
         pg, sl = (torch.tensor([x[i] for x in at], device="cuda") for i in range(2))
         key = torch.arange(n, device="cuda")[None, :]
-        see = (key <= pos) & ((key > pos - window) if window else True)
+        see = (key <= pos) & ((key > pos - window) if window else True) & (pg >= 0) & (pg < S.P)
+        pg = pg.clamp(0, S.P - 1)
         for h in range(q.shape[1]):
             x, k, v = q[rows, h], k_all[pg, h // group, sl], v_all[pg, h // group, sl]
             digits = 15 * v_s[pg, h // group, sl]
@@ -43,12 +44,13 @@ def weighed(q, S, scale, window, prompt, pool=None):
             # scores: exponents and their largest in 32 bits, to 2^-22 of each; for prompts K in 11 bits
             y0 = y.masked_fill(~see, 0.0).abs()
             ds = ((y0 + y0.amax(-1, keepdim=True) + 32) * 2.0 ** -22) ** 2
-            if prompt:
+            if prompt is not False:
                 ds = ds + (scale * H16) ** 2 * (x * x) @ (k * k).T
             e = w * w * ds
             sq = e @ (v * v) - 2 * o * (e @ v) + o * o * e.sum(-1, keepdim=True)
             # weights in 11 bits, for prompts values too; for decoding the weight is of the digits, at most 15 of them
-            sq = sq + H16 ** 2 * ((w * w) @ (2 * v * v if prompt else digits * digits))
+            kept = 0 if prompt is False else 2 * v * v
+            sq = sq + H16 ** 2 * ((w * w) @ (kept if prompt else kept + digits * digits))
             # the smallest weights: f16 has steps of 2^-24, 2^-21 of the row's largest weight times value
             sq = sq + n * (2.0 ** -21 * (w * v.abs().amax(-1)).amax(-1, keepdim=True)) ** 2
             # values in f16 next to a larger one of the same key (16 keys where none is 2^10 times another)
@@ -98,6 +100,28 @@ def test_decoding(D, kvh, group, new, past, window):
     q = attend_case(S, group)
     cache, batch = S.on_gpu()
     check_weighed(cache.attend(batch, q, window=window), q, S, window, prompt=False)
+
+
+def test_prompts_with_missing_pages():
+    S = Setup(128, 2, [90, 40, 3], [200, 1000, 300])
+    q = attend_case(S, 2)
+    S.table[0, [1, 3, 15]] = -1
+    S.table[1, 4:60] = S.P + 7
+    S.table[2, 2] = -9
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S, prompt=None)
+
+
+@pytest.mark.parametrize("hints", [None, (0, 0), (1, 1)])
+def test_chunks_beside_decoding(hints):
+    g = np.random.default_rng(3)
+    new = [int(n) for n in g.choice([1, 1, 1, 2, 0, 19, 33], 40)]
+    past = [int(n) for n in g.integers(0, 700, 40)]
+    S = Setup(128, 2, new, past)
+    q = attend_case(S, 2)
+    cache, batch = S.on_gpu(*(hints or ()))
+    for window in (0, 200):
+        check_weighed(cache.attend(batch, q, window=window), q, S, window, prompt=None)
 
 
 def outlier_case(D, new, past, times, at, score, seed=0, group=2):
