@@ -635,7 +635,13 @@ q3t_status q3t_kv4_append(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch
  * boundary that this call alone uses while it runs (calls that may overlap, and
  * graphs that may replay at once, need one each); it needs no initialisation
  * and holds nothing between calls.  64 KiB at least; Q3T_KV4_WORKSPACE serves
- * the widest launch. */
+ * the widest launch.
+ * Sums, maxima and the softmax are in 32 bits; weights enter the products in 11
+ * bits, and in calls with sequences of more than 16 rows of a kv head (prompts)
+ * cached keys and values do too, each relative to itself, down to 2^-24 of the
+ * row's largest weight times value and 2^-28 of a key's largest dim.
+ * Waits inside the kernels are bounded: one that gives up, which takes a fault
+ * of the device, leaves its rows NaN (the call has returned OK by then). */
 #define Q3T_KV4_WORKSPACE (20 << 20)
 q3t_status q3t_kv4_attend(const q3t_kv4_cache *cache, const q3t_kv4_batch *batch, int num_heads, const uint16_t *q,
                           int64_t q_stride, float scale, int window, uint16_t *out, int64_t out_stride,

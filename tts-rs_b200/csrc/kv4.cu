@@ -303,11 +303,13 @@ Q3T_DEV bool quantise(const float v[8], uint32_t n[8], uint32_t &scale_zero) {
 // four lanes a group of 32, and a warp two rows (D = 128) or four of one kind.
 // Blocks are put together in shared memory, and a window that fills its page
 // is written in 16-byte pieces, any other in the bytes that its tokens own.
-// Bound by issuing instructions, not by bytes: 8100 rows of 32 heads take
-// 52 us, 2.1 TB/s.  With 32 dims to a lane (E = D / 32) the sums and shuffles
+// Bound by latency at few warps, not by bytes: a lane's 32 dims take 118
+// registers, which leaves 16 warps to an SM, and these wait for fixed latencies,
+// shuffles and shared memory (a prompt of 4096 rows: 48 % of the issue slots, 11 %
+// of DRAM).  8100 rows of 32 heads take 53 us, 2.1 TB/s.  With 32 dims to a lane (E = D / 32) the sums and shuffles
 // per element are fewer, but the code is longer, and a decoding step, which
 // goes through it once, spends its time fetching it.  Eight dims to a lane and
-// 32 (D = 128): 64 rows 6.3 and 11.2 us, 8100 rows 65 and 52 us; so prompts,
+// 32 (D = 128): 64 rows 6.1 and 11.2 us, 8100 rows 65 and 53 us; so prompts,
 // of 32 rows and more to a sequence, take the second, unless only a part of
 // their rows turns by halves (the others of its pairs are other lanes').
 // ---------------------------------------------------------------------------
@@ -533,7 +535,7 @@ __global__ void __launch_bounds__(kAppendThreads, E == 1 ? 4 : E == 2 ? 3 : 2) k
 // Read: one CTA per (window, head split) brings its blocks to shared memory
 // and writes the rows n s + z, rounded once to bf16.  A thread takes whole
 // words of digits: eight of a key, or the 64 of 16 dims of four tokens' values.
-// Bound by HBM: 64 sequences of 100 to 1500 tokens, 314 MB, in 60 us, 0.80 of
+// Bound by HBM: 64 sequences of 100 to 1500 tokens, 314 MB, in 59 us, 0.81 of
 // the measured copy rate (a byte at a time: 109 us).
 // ---------------------------------------------------------------------------
 constexpr int kReadThreads = 256;
@@ -615,8 +617,9 @@ __global__ void __launch_bounds__(kReadThreads) k_kv4_read(const __grid_constant
 // dims x 16 keys of V) and the 8 columns are (query row r, group j): column
 // (r, j) of the score product holds q in the dims of group j and zeros
 // elsewhere, its accumulator is the group's share of the score; column (r, j)
-// of the value product holds p s_j.  So no lane computes what no one needs:
-// a lane scales the shares of two columns for two keys, one shuffle joins the
+// of the value product holds p s_j.  (Most of the score products are with zeros;
+// with few rows the tensor pipe is 24 % busy all the same.)  Every lane has work of
+// its own: it scales the shares of two columns for two keys, one shuffle joins the
 // groups of a row, and p s goes from the accumulator's order to the operand's
 // by one matrix transpose per 8 keys.
 //
@@ -630,9 +633,9 @@ __global__ void __launch_bounds__(kReadThreads) k_kv4_read(const __grid_constant
 // by k_kv4_combine from the workspace.  Nothing is kept between calls.
 //
 // Long caches are bound by HBM: 64 requests of 4096 keys on 8 kv heads, 336
-// MB, take 67 us, 0.76 of the measured copy rate, and the loads alone take as
-// long; one of 131071 keys 39 us (in units of CTAs that end with a sequence
-// 94).  Short ones are bound by both ends: 64 of 100 to 1500 keys 27 us.
+// MB, take 65 us, 0.79 of the measured copy rate; one of 131071 keys 37 us (in
+// units of CTAs that end with a sequence 94).  Short ones are bound by both ends,
+// filling the ring and joining the parts: 64 of 100 to 1500 keys 26 us.
 //
 // f16 holds q times a power of two per row (its 11 bits keep a bf16 q whole
 // down to 2^-25 of the row's largest) and p s, which is rounded to 11 bits, as
@@ -1396,21 +1399,20 @@ __global__ void __launch_bounds__(256) k_kv4_combine(const __grid_constant__ Kv4
 //   O += P V      M 128 rows, N D, K 64 keys        (TMEM)
 // Two such halves share every unpacked tile of keys.  Warps 0-7 are the
 // softmax (a thread to a row), 8-15 unpack (a warp to a page of K or of V of
-// the tile), 16-19 issue the products, one lane to each half's S and P V (one
-// lane for all four spent its time issuing: 540 cycles for an S).  K, V and S
+// the tile), 16-19 issue the products, one lane to each half's S and P V (with
+// one for both halves' S and one for both P V a prompt took 9 us more).  K, V and S
 // have two buffers each, so the unpacking of a tile, its S, the softmax of the
 // one before and its P V run at once.
 //
-// What bounds it is the softmax warps' way through a tile, 2950 cycles: waits
-// and loads of a few hundred each, 64 exponentials a row, and a share of the
-// schedulers, whose slots are 64 % taken (7900 warp instructions a tile, 40 %
-// of them unpacking, which 4-bit keys cost and bf16 ones would not).  The
-// tensor pipe is busy 27 %, HBM does not matter.  A prompt of 4096 tokens on 8
-// kv heads (68.7 GFLOP) takes 120 us, 0.35 of the products' rate alone.  With
+// What bounds it is the softmax warps' way through a tile: waits for S, V and
+// TMEM loads, 64 exponentials a row, and a share of the schedulers, whose slots
+// are 59 % taken, by the unpacking warps too (which 4-bit keys cost and bf16 ones
+// would not).  The tensor pipe is busy 23 %, HBM 2 %.  A prompt of 4096 tokens on
+// 8 kv heads (68.7 GFLOP) takes 120 us, 0.35 of the products' rate alone.  With
 // loops unrolled throughout, 102 KB of code instead of 62, warps waited for
 // instructions most of the time: 178 us.  One buffer of P, whose P V a softmax
-// then waits for, is 5 us more; V's powers after the weights 3.5 us (by the
-// largest value alone, which is wrong where that has no weight, 116.6 us).
+// then waits for, is 5 us more; powers of two that follow the weights, and keys'
+// own, 3.4 us (a page's alone are wrong beside a large value without weight).
 //
 // Where tiles of rows cannot fill the GPU, CTAs share the keys of each and
 // k_kv4_join joins their parts: 32 rows of one request on 8000 keys, 126 tiles,
@@ -2247,8 +2249,8 @@ cudaError_t attend_launch(const Kv4AttendArgs &a0, int rows, int max_kv, void *w
   const int64_t units = (int64_t)a.b.num_seqs * a.units, steps = (pages + 1) / 2 * units;
   // A CTA to each unit of each kv head where they all fit the GPU at once and a warp's share is short: no second
   // launch to join parts.  The more CTAs, the less an equal division gains (us, whole against divided, D = 128): 8 CTAs
-  // of 200 keys 6.7 and 8.0, of 1000 12.4 and 8.4; 32 of 500 9.1 and 8.9; 128 of 500 9.3 and 12.3, of 1000 12.8 and
-  // 15.5, of 2500 23.9 and 20.9; 512, which do not fit, of 500 21.6 and 20.5.
+  // of 200 keys 6.8 and 8.2, of 1000 12.1 and 8.7; 32 of 500 9.2 and 9.0; 128 of 500 9.4 and 12.3, of 1000 12.7 and
+  // 15.3, of 2500 23.7 and 20.4; 512, which do not fit, of 500 21.5 and 20.1.
   const int64_t per_warp = ((pages + 1) / 2 + Cfg::W - 1) / Cfg::W, whole = units * a.c.n_kv;
   if (whole <= resident.load() && per_warp <= 2 + whole / 9)
     return launch(k_kv4_attend<D, NT>, dim3((unsigned)whole), Cfg::W * 32, Cfg::smem(1), 1, pdl, st, a, (PartNote *)nullptr,
@@ -2331,8 +2333,8 @@ cudaError_t kv4_attend(const Kv4AttendArgs &a0, int max_q, int max_kv, void *ws,
   Kv4AttendArgs a = a0;
   const int gq = a.n_heads / a.c.n_kv;
   // Sequences of more rows than this go by tiles on k_kv4_prompt.  With 32 rows it takes, against k_kv4_attend (us,
-  // group of 2), 30 and 34 (one sequence of 8000 keys), 102 and 168 (eight), 127 and 197 (64 of 1000); with 16 rows
-  // k_kv4_attend takes 23, 93 and 108, and a tile as long as with 32.
+  // group of 2, D = 128), 30 and 33 (one sequence of 8000 keys), 107 and 162 (eight), 132 and 189 (64 of 1000), but 22 and
+  // 16 with one of 1000; with 16 rows k_kv4_attend takes 23, 88 and 104, and a tile as long as with 32.
   constexpr int kBig = 16;
   const bool some_big = max_q <= 0 || (int64_t)max_q * gq > kBig;
   // No sequence is small where all but one at their most leave more than kBig rows for the last.  Elsewhere both
