@@ -64,3 +64,21 @@ def test_lengths_below_zero_are_padding(kv, new):
     assert all((t == 0).all() for t in cache.read(batch))
     for window in (0, 5):
         assert (cache.attend(batch, q, window=window) == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_read_of_values_near_the_largest(D, dtype):
+    """Of -3.2e38 .. 3.2e38 in one group 15 steps are 6.4e38, beyond 32 bits, but no value that is kept is."""
+    S = Setup(D, 2, [33], [5])
+    cache, batch = S.on_gpu()
+    x = torch.from_numpy((3.2e38 * S.rng.uniform(-1, 1, (2, S.T, 2, D))).astype(np.float32)).cuda().to(dtype)
+    x[..., ::32], x[..., 1::32] = -3.2e38, 3.2e38
+    cache.append(batch, *x)
+    kc, vc, _, _ = R.unpack(S.d_pool.cpu().numpy(), D)
+    for got, stored in zip(cache.read(batch), (kc, vc)):
+        got = got.double().cpu().numpy()
+        for row, s, p in S.places():
+            pg, c = S.slot(s, p)
+            ref = stored[pg, :, c]
+            assert (np.abs(got[row] - ref) <= HALF * np.abs(ref) + 2.0 ** -22 * 3.2e38).all()

@@ -557,8 +557,9 @@ __global__ void __launch_bounds__(kReadThreads) k_kv4_read(const __grid_constant
   cp_async_commit();
   cp_async_wait<0>();
   __syncthreads();
+  // (n s is exact in 32 bits, but may pass them where n s + z does not)
   auto value = [](uint32_t n, uint32_t sz) {
-    return __fadd_rn(__fmul_rn(__uint_as_float(0x4b000000u | n) - 0x1p23f, bf2f(sz & 0xffffu)), __uint_as_float(sz & 0xffff0000u));
+    return fmaf(__uint_as_float(0x4b000000u | n) - 0x1p23f, bf2f(sz & 0xffffu), __uint_as_float(sz & 0xffff0000u));
   };
   if (a.k)  // four threads to a row, the dims as in append
     for (int x = threadIdx.x; x < 4 * nk * w.n; x += kReadThreads) {
