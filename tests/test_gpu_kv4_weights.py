@@ -243,3 +243,17 @@ def test_prompts_with_large_keys_that_rows_do_not_see_or_score_low(D, new, past,
     S, q = outlier_case(D, new, past, 1.0, PLACES[where](new + past), -2.0 ** power)
     cache, batch = S.on_gpu()
     check_weighed(cache.attend(batch, q), q, S)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new, past", [(1, 200), (1, 9000), (3, 900), (24, 1000), (300, 0)])
+@pytest.mark.parametrize("spread", [True, False])
+def test_values_near_the_largest(D, new, past, spread):
+    """Groups of -3.2e38 .. 3.2e38, whose scale times 15 leaves 32 bits, or of 3.2e38 alone, which many keys sum up."""
+    S = Setup(D, 1, [new], [past])
+    g, n = S.rng, S.kv[0]
+    v = 3.2e38 * (g.uniform(-1, 1, (1, n, D)) if spread else np.ones((1, n, D)))
+    S.fill([g.standard_normal((1, n, D)).astype(np.float32)], [v.astype(np.float32)])
+    q = torch.from_numpy((3 * g.standard_normal((S.T, 2, D))).astype(np.float32)).cuda().bfloat16()
+    cache, batch = S.on_gpu()
+    check_weighed(cache.attend(batch, q), q, S, prompt=new * 2 > 16)

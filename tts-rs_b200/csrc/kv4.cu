@@ -681,6 +681,9 @@ Q3T_DEV uint32_t transpose8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+// A part's l lies in [2^kPartL, 2^(kPartL + 1)): with it o is so far below the values that neither the largest ones nor
+// the sum of a thousand parts leave 32 bits.
+constexpr int kPartL = -11;
 // weight of a part with running maximum m and sum l under the joint maximum
 // M; a part without keys has none, one with NaN scores keeps them
 Q3T_DEV float part_weight(float m, float l, float M) {
@@ -1120,9 +1123,9 @@ Q3T_DEV void attend_run(const Kv4AttendArgs &a, const StepList &L, int kvh, int 
         zac[nt][1] += __shfl_xor_sync(0xffffffffu, zac[nt][1], o);
       }
       const int r = (nt * 8 + 2 * t) / G, ja = 2 * t % G;
-      // l as a number from 1 to 2 and an exponent, which ref takes: refs may be so far apart that one of two parts of
-      // like weight would have none.  (0 and no number stay that.)
-      const int el = l[nt] == 0.f ? 0 : min(exponent(l[nt]), 126);
+      // l as a number of kPartL and an exponent, which ref takes: refs may be so far apart that one of two parts of like
+      // weight would have none.  (0 and no number stay that.)
+      const int el = l[nt] == 0.f ? 0 : min(max(exponent(l[nt]) - kPartL, -126), 126);
       const float fl = __uint_as_float((uint32_t)(127 - el) << 23);
       if (g == 0) {
         p_z[r * G + ja] = zac[nt][0] * fl;
@@ -2000,11 +2003,11 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
     const float inv = l == 0.f ? 0.f : 1.f / l;
     float *part = splits > 1 ? ks.parts + (size_t)blockIdx.x * Cfg::PART + threadIdx.x : nullptr;
     const bool in_tile = (int)threadIdx.x < nrow;
-    // a part weighs l 2^ref, here as a number from 1 to 2 and an exponent: ref has V's powers, which may be far apart
+    // a part weighs l 2^ref, here as a number of kPartL and an exponent: ref has V's powers, which may be far apart
     if (part && in_tile) {
-      const int e = l == 0.f ? 0 : exponent(l);
+      const int e = l == 0.f ? 0 : min(max(exponent(l) - kPartL, -126), 126);
       part[0] = ref + (float)e;
-      part[ROWS] = gone ? __uint_as_float(0x7fc00000u) : l * __uint_as_float((uint32_t)(127 - min(e, 126)) << 23);
+      part[ROWS] = gone ? __uint_as_float(0x7fc00000u) : l * __uint_as_float((uint32_t)(127 - e) << 23);
     }
 #pragma unroll 1
     for (int c = 0; c < D / 32; c++) {
@@ -2073,7 +2076,7 @@ __global__ void __launch_bounds__(PromptCfg<D>::THREADS, 1) k_kv4_prompt(const _
 // Joins the parts of k_kv4_prompt's tiles, where it divided the keys: a thread
 // has a row, eight dims of it (32 to a thread, one part after the other, took
 // 33 us for 18 parts: all of it waiting for loads).  A part's o is divided by
-// its l already, so a part weighs l 2^m (l from 1 to 2, or 0); parts come in
+// its l already, so a part weighs l 2^m (l as kPartL has it); parts come in
 // order, and the result does not depend on timing.
 template <int D>
 __global__ void __launch_bounds__(256) k_kv4_join(const __grid_constant__ Kv4AttendArgs a, PromptSplit sp) {
