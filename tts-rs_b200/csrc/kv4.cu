@@ -2415,6 +2415,7 @@ Kv4View view_of(const char *what, const q3t_kv4_cache *c) {
          c->table_stride);
   if (!c->pool || !c->page_table) FAIL(Q3T_INVALID_INPUT, "%s: null pool or page table", what);
   if (!aligned(c->pool, 16)) FAIL(Q3T_INVALID_INPUT, "%s: the pool must start on a 16-byte boundary", what);
+  if (!aligned(c->page_table, 4)) FAIL(Q3T_INVALID_INPUT, "%s: the page table is not aligned to its entries", what);
   return Kv4View{(uint8_t *)c->pool, c->page_table, c->num_pages, c->num_kv_heads, c->head_dim, c->table_rows,
                  c->table_stride};
 }
@@ -2427,6 +2428,8 @@ Kv4Batch batch_of(const char *what, const q3t_kv4_batch *b) {
   if (b->max_q_len < 0 || b->max_kv_len < 0)
     FAIL(Q3T_INVALID_INPUT, "%s: negative max_q_len or max_kv_len", what);
   if (b->num_seqs > 0 && (!b->q_start || !b->kv_len)) FAIL(Q3T_INVALID_INPUT, "%s: null q_start or kv_len", what);
+  if (!aligned(b->q_start, 4) || !aligned(b->kv_len, 4) || !aligned(b->table_row, 4))
+    FAIL(Q3T_INVALID_INPUT, "%s: q_start, kv_len or table_row is not aligned to its entries", what);
   return Kv4Batch{b->num_seqs, b->num_tokens, b->q_start, b->kv_len, b->table_row, 0};
 }
 
@@ -2493,6 +2496,8 @@ extern "C" q3t_status q3t_kv4_append(const q3t_kv4_cache *cache, const q3t_kv4_b
     if (rows->dtype != Q3T_F32 && rows->dtype != Q3T_BF16) FAIL(Q3T_INVALID_INPUT, "%s: unknown dtype %d", what, rows->dtype);
     if (rows->num_heads < 0 || rows->num_heads > (1 << 16))
       FAIL(Q3T_INVALID_INPUT, "%s: num_heads %d outside 0..65536", what, rows->num_heads);
+    if (!aligned(rows->q_gamma, 4) || !aligned(rows->k_gamma, 4))
+      FAIL(Q3T_INVALID_INPUT, "%s: q_gamma or k_gamma is not aligned to its elements", what);
     if (rope && rope->rotary_dim > a.c.head_dim)
       FAIL(Q3T_INVALID_INPUT, "%s: rotary_dim %d exceeds head_dim %d", what, rope->rotary_dim, a.c.head_dim);
     if ((rows->q_gamma || rows->k_gamma) && !(rows->eps >= 0.f && std::isfinite(rows->eps)))
